@@ -160,6 +160,71 @@ class SparseMaskArgs(Structure):
         ("q_pos0", c_int64), ("k_pos0", c_int64), ("causal", c_int32),
     ]
 
+
+class QkNormRopeArgs(Structure):
+    """Mirror of enl_qk_norm_rope_args."""
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "q_out", "k_out")] + [
+        ("batch", c_int32), ("seq", c_int32), ("num_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+    ] + [(f"{t}_stride_{d}", c_int64) for t in ("q", "k", "v", "qo", "ko")
+         for d in ("b", "s", "h")] + [
+        ("in_dtype", c_int32), ("out_dtype", c_int32),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float),
+        ("rope_cos", c_void_p), ("rope_sin", c_void_p), ("rope_rows", c_int64),
+        ("pos0", c_int64), ("start", c_void_p),
+        ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("page_stride_p", c_int64), ("page_stride_h", c_int64), ("page_stride_s", c_int64),
+        ("num_pages", c_int32), ("page_size", c_int32),
+        ("block_table", c_void_p), ("table_stride_b", c_int64), ("max_pages", c_int32),
+        ("n_new", c_void_p),
+    ]
+
+
+class QkNormRopeBackwardArgs(Structure):
+    """Mirror of enl_qk_norm_rope_backward_args."""
+    _fields_ = [(n, c_void_p) for n in ("dq_out", "dk_out", "q", "k", "dq", "dk", "dq_weight",
+                                        "dk_weight")] + [
+        ("batch", c_int32), ("seq", c_int32), ("num_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+    ] + [(f"{t}_stride_{d}", c_int64) for t in ("dqo", "dko", "q", "k", "dq", "dk")
+         for d in ("b", "s", "h")] + [
+        ("in_dtype", c_int32), ("grad_dtype", c_int32), ("out_dtype", c_int32),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float),
+        ("rope_cos", c_void_p), ("rope_sin", c_void_p), ("rope_rows", c_int64),
+        ("pos0", c_int64), ("start", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class PagedDecodeArgs(Structure):
+    """Mirror of enl_paged_decode_args."""
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_h", c_int64),
+        ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("page_stride_p", c_int64), ("page_stride_h", c_int64), ("page_stride_s", c_int64),
+        ("num_pages", c_int32), ("page_size", c_int32),
+        ("block_table", c_void_p), ("table_stride_b", c_int64), ("max_pages", c_int32),
+        ("seq_lens", c_void_p),
+        ("o", c_void_p), ("o_stride_b", c_int64), ("o_stride_h", c_int64), ("lse", c_void_p),
+        ("batch", c_int32), ("num_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32), ("window", c_int32), ("sinks", c_int32),
+        ("alibi_slopes", c_void_p), ("scale", c_float),
+        ("in_dtype", c_int32), ("out_dtype", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class SampleArgs(Structure):
+    """Mirror of enl_sample_args."""
+    _fields_ = [
+        ("logits", c_void_p), ("stride_b", c_int64), ("dtype", c_int32),
+        ("batch", c_int32), ("vocab", c_int32), ("u", c_void_p),
+        ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p),
+        ("temperature_all", c_float), ("top_k_all", c_int32), ("top_p_all", c_float),
+        ("min_p_all", c_float), ("tokens", c_void_p),
+    ]
+
+
 # Exported symbol -> (argtypes, restype). Kept in sync with include/enl_attn.h
 # (a CPU test checks every declared symbol is exported and bound here).
 SIGNATURES = {
@@ -202,6 +267,12 @@ SIGNATURES = {
     "enl_project_workspace_bytes": ([POINTER(ProjectArgs)], c_size_t),
     "enl_split_bf16": ([c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p],
                        c_int32),
+    "enl_qk_norm_rope": ([POINTER(QkNormRopeArgs), c_void_p], c_int32),
+    "enl_qk_norm_rope_backward": ([POINTER(QkNormRopeBackwardArgs), c_void_p], c_int32),
+    "enl_qk_norm_rope_backward_workspace_bytes": ([POINTER(QkNormRopeBackwardArgs)], c_size_t),
+    "enl_attn_decode_paged": ([POINTER(PagedDecodeArgs), c_void_p], c_int32),
+    "enl_paged_decode_workspace_bytes": ([POINTER(PagedDecodeArgs)], c_size_t),
+    "enl_sample_tokens": ([POINTER(SampleArgs), c_void_p], c_int32),
     "enl_selftest_exp2": ([c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p], c_int32),
 }
 
@@ -219,7 +290,11 @@ def load() -> ctypes.CDLL:
             "`python -m enilnets_b200.build`; there is no CPU fallback for the attention path.")
     lib = ctypes.CDLL(str(LIB_PATH))
     for name, (argtypes, restype) in SIGNATURES.items():
-        fn = getattr(lib, name)
+        try:
+            fn = getattr(lib, name)
+        except AttributeError:
+            raise RuntimeError(f"{LIB_PATH.name} has no {name}: rebuild it with "
+                               "`python -m enilnets_b200.build --force`.") from None
         fn.argtypes = argtypes
         fn.restype = restype
     if lib.enl_abi_version() != ABI_VERSION:

@@ -296,4 +296,96 @@ cudaError_t launch_lin_tc(const CUtensorMap& tq, const CUtensorMap& tk, const CU
 size_t linear_workspace_bytes(int B, int H, int Hkv, int S, int Df, int D, int causal);
 int linear_attn_max_features();
 
+// Per-head norm and rotation (enl_qknorm.cu). Operand 0 is q, 1 is k, 2 is v
+// (only with pages). Element strides throughout.
+struct QkRopeParams {
+  int B, S, H, Hkv, D;
+  const void* x[3];
+  long long x_sb[3], x_ss[3], x_sh[3];
+  void* y[2];  // y[1] null with pages
+  long long y_sb[2], y_ss[2], y_sh[2];
+  int in_fp32, out_fp32;
+  const float* w[2];  // norm weights, both or neither
+  float eps;
+  const float* cos_t;  // (rows, D / 2) tables, both or neither
+  const float* sin_t;
+  long long rows, pos0;
+  const int* start;  // (B) or null
+  void* pages[2];    // k and v pools, or null
+  long long p_sp, p_sh, p_ss;
+  int n_pages, page_size;
+  const int* table;
+  long long t_sb;
+  int max_pages;
+  const int* n_new;
+};
+cudaError_t launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream);
+
+struct QkRopeBwdParams {
+  int B, S, H, Hkv, D;
+  const void* dy[2];
+  long long dy_sb[2], dy_ss[2], dy_sh[2];
+  const void* x[2];
+  long long x_sb[2], x_ss[2], x_sh[2];
+  void* dx[2];
+  long long dx_sb[2], dx_ss[2], dx_sh[2];
+  float* dw[2];
+  int in_fp32, grad_fp32, out_fp32;
+  const float* w[2];
+  float eps;
+  const float* cos_t;
+  const float* sin_t;
+  long long rows, pos0;
+  const int* start;
+  float* partial;  // (n_blocks, 2, D)
+  int n_blocks;
+};
+// Blocks of the backward's grid (they bound the partial sums' size).
+int qk_rope_bwd_blocks(int B, int S, int H, int Hkv, int D, int n_sms);
+cudaError_t launch_qk_norm_rope_backward(const QkRopeBwdParams& p, cudaStream_t stream);
+
+// Paged decode (enl_paged.cu).
+struct PagedDecodeParams {
+  const void* q;
+  long long q_sb, q_sh;
+  const void* k;
+  const void* v;
+  long long p_sp, p_sh, p_ss;
+  int n_pages, page_size;
+  const int* table;
+  long long t_sb;
+  int max_pages;
+  const int* lens;
+  void* o;
+  long long o_sb, o_sh;
+  float* lse;
+  int B, H, Hkv, D;
+  int window, sinks;
+  const float* alibi;
+  float scale;
+  int in_fp32, out_fp32;
+  void* workspace;
+  int n_sms;
+};
+size_t paged_decode_workspace(int B, int H, int Hkv, int D, int n_sms);
+cudaError_t launch_paged_decode(const PagedDecodeParams& p, cudaStream_t stream);
+
+// Sampling (enl_sample.cu).
+struct SampleParams {
+  const void* logits;
+  long long stride;
+  int fp32, B, V;
+  const float* u;
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+  long long* tokens;
+  int n_sms;
+};
+cudaError_t launch_sample(const SampleParams& p, cudaStream_t stream);
+
 }  // namespace enl

@@ -2,6 +2,7 @@
 // error word, so they are compiled together rather than with relocatable
 // device code.
 #include "enl_abi.cu"
+#include "enl_abi_serving.cu"
 #include "enl_prefill.cu"
 #include "enl_decode.cu"
 #include "enl_kvcache.cu"
@@ -12,3 +13,6 @@
 #include "enl_sparse.cu"
 #include "enl_backward.cu"
 #include "enl_gemm.cu"
+#include "enl_qknorm.cu"
+#include "enl_paged.cu"
+#include "enl_sample.cu"

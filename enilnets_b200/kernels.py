@@ -716,3 +716,388 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws_bytes
     nat.check(lib.enl_linear_attention(ctypes.byref(a), _stream()), "enl_linear_attention")
     return (out, new_state) if return_state else out
+
+
+# ------------------------------------------------- serving over paged caches
+def _same_device(q: torch.Tensor, *named) -> None:
+    """Every given tensor (None skipped) sits on q's device, which is the
+    current one: launches go to its current stream."""
+    dev = q.device
+    for name, t in named:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not {dev}")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {dev}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+def _require_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> None:
+    """t is a contiguous (n,) CUDA tensor of the dtype."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (n,) or not t.is_cuda \
+            or not t.is_contiguous():
+        got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name} must be a contiguous {dtype} ({n},) CUDA tensor, got {got}")
+
+
+def _heads4(name: str, t: torch.Tensor, shape, dtypes=_DTYPES) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or \
+            t.shape != shape or t.stride(-1) != 1:
+        got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name} must be a bf16/fp32 CUDA tensor of shape {tuple(shape)} with a "
+                         f"contiguous last (head) dimension, got {got}")
+
+
+def _norm_rope_operands(D: int, q_weight, k_weight, rope):
+    """(weight pointers, table pointers, table rows) after their checks."""
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight come in pairs")
+    wq = wk = cos = sin = None
+    rows = 0
+    if q_weight is not None:
+        _require_vector("q_weight", q_weight, D, torch.float32)
+        _require_vector("k_weight", k_weight, D, torch.float32)
+        wq, wk = q_weight.data_ptr(), k_weight.data_ptr()
+    if rope is not None:
+        cos_t, sin_t = rope
+        for name, t in (("cos", cos_t), ("sin", sin_t)):
+            _require_cuda(name, t, torch.float32)
+            if t.dim() != 2 or t.shape[1] * 2 != D or not t.is_contiguous():
+                raise ValueError(f"rope {name} must be a contiguous fp32 (rows, {D // 2}) table, "
+                                 f"got {tuple(t.shape)}")
+        if cos_t.shape != sin_t.shape:
+            raise ValueError("rope tables must have one shape")
+        cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
+    return wq, wk, cos, sin, rows
+
+
+def _page_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, B: int,
+               Hkv: int, D: int, dtype: torch.dtype) -> None:
+    """Checks of a paged cache's pools and block table."""
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.dim() != 4 \
+                or t.stride(-1) != 1:
+            got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+            raise ValueError(f"{name} must be a {dtype} (num_pages, {Hkv}, page_size, {D}) CUDA "
+                             f"tensor with a contiguous head dimension, got {got}")
+    _, h, _, d = k_pages.shape
+    if h != Hkv or d != D or k_pages.shape != v_pages.shape or \
+            k_pages.stride() != v_pages.stride():
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must "
+                         f"share shape (num_pages, {Hkv}, page_size, {D}) and strides")
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or \
+            not block_table.is_cuda or block_table.dim() != 2 or block_table.shape[0] != B or \
+            block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be an int32 ({B}, max_pages) CUDA tensor with "
+                         "contiguous rows")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6, rope=None,
+                 pos0: int = 0, start: Optional[torch.Tensor] = None, out=None,
+                 out_dtype: Optional[torch.dtype] = None):
+    """RMS norm of each query and key head with the position rotation, in one
+    pass: z = w * x / sqrt(mean(x^2) + eps) over the head, then rotate-half
+    (nn/forward.py:80-88).
+
+    q: (B, S, H, D), k: (B, S, Hkv, D) head views, bf16 or fp32, D a multiple
+    of 8 up to 128. q_weight, k_weight: fp32 (D,), or both None for the
+    rotation alone. rope: (cos, sin) fp32 (rows, D / 2) tables, or None for the
+    norm alone; token s of row b uses table row pos0 + start[b] + s (start: int32
+    (B,), None = 0). out=(q_out, k_out) writes into given views, which may be q
+    and k themselves. Returns (q_out, k_out), in out_dtype (default: q's).
+    """
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or not isinstance(k, torch.Tensor) or \
+            k.dim() != 4:
+        raise ValueError("q and k must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
+    B, S, H, D = q.shape
+    Hkv = k.shape[2]
+    dt = q.dtype
+    _heads4("q", q, (B, S, H, D))
+    _heads4("k", k, (B, S, Hkv, D), (dt,))
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    if out is None:
+        out_dtype = out_dtype or dt
+        q_out = torch.empty((B, S, H, D), dtype=out_dtype, device=q.device)
+        k_out = torch.empty((B, S, Hkv, D), dtype=out_dtype, device=q.device)
+    else:
+        q_out, k_out = out
+    _heads4("q_out", q_out, (B, S, H, D))
+    _heads4("k_out", k_out, (B, S, Hkv, D), (q_out.dtype,))
+    if start is not None:
+        _require_vector("start", start, B, torch.int32)
+    _same_device(q, ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("start", start),
+                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]),
+                 ("q_out", q_out), ("k_out", k_out))
+    a = nat.QkNormRopeArgs(
+        q.data_ptr(), k.data_ptr(), None, q_out.data_ptr(), k_out.data_ptr(), B, S, H, Hkv, D,
+        *q.stride()[:3], *k.stride()[:3], 0, 0, 0, *q_out.stride()[:3], *k_out.stride()[:3],
+        _DTYPES[dt], _DTYPES[q_out.dtype], wq, wk, eps, cos, sin, rows, pos0, _ptr(start))
+    nat.check(nat.load().enl_qk_norm_rope(ctypes.byref(a), _stream()), "enl_qk_norm_rope")
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                        v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor, *,
+                        n_new: Optional[torch.Tensor] = None,
+                        q_weight: Optional[torch.Tensor] = None,
+                        k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, rope=None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qk_norm_rope for new tokens of a paged cache, with the append fused in:
+    the normalised and rotated keys and the values go straight into the pages.
+
+    q: (B, S, H, D), k, v: (B, S, Hkv, D) head views of the projections;
+    k_pages, v_pages: (num_pages, Hkv, page_size, D) pools of the same dtype
+    with equal strides; block_table: int32 (B, max_pages). Token s of row b is
+    position p = start[b] + s (start: int32 (B,), the row's cached length): its
+    rotation uses table row p, its key and value go to slot p % page_size of
+    page block_table[b, p // page_size]. n_new: int32 (B,) counts of real tokens
+    per row; the others cache nothing and their queries come out zero. Weights and
+    rope may be None (no norm / no rotation). Returns the queries (B, S, H, D).
+    """
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or not isinstance(k, torch.Tensor) or \
+            k.dim() != 4:
+        raise ValueError("q and k must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
+    B, S, H, D = q.shape
+    Hkv = k.shape[2]
+    dt = q.dtype
+    _heads4("q", q, (B, S, H, D))
+    _heads4("k", k, (B, S, Hkv, D), (dt,))
+    _heads4("v", v, (B, S, Hkv, D), (dt,))
+    _page_pool(k_pages, v_pages, block_table, B, Hkv, D, dt)
+    _require_vector("start", start, B, torch.int32)
+    if n_new is not None:
+        _require_vector("n_new", n_new, B, torch.int32)
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    if out is None:
+        out = torch.empty((B, S, H, D), dtype=dt, device=q.device)
+    _heads4("out", out, (B, S, H, D), (dt,))
+    _same_device(q, ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages),
+                 ("block_table", block_table), ("start", start), ("n_new", n_new),
+                 ("q_weight", q_weight), ("k_weight", k_weight),
+                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]), ("out", out))
+    if B * S == 0:
+        return out
+    a = nat.QkNormRopeArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, B, S, H, Hkv, D,
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], 0, 0, 0,
+        _DTYPES[dt], _DTYPES[dt], wq, wk, eps, cos, sin, rows, 0, start.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0],
+        k_pages.shape[2], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        _ptr(n_new))
+    nat.check(nat.load().enl_qk_norm_rope(ctypes.byref(a), _stream()), "enl_qk_norm_rope")
+    return out
+
+
+def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: Optional[torch.Tensor],
+                          k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor] = None,
+                          k_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                          rope=None, pos0: int = 0, start: Optional[torch.Tensor] = None,
+                          out=None, out_dtype: Optional[torch.dtype] = None):
+    """Gradients of qk_norm_rope(q, k, q_weight, k_weight, ...).
+
+    dq_out, dk_out: gradients of its outputs, bf16 or fp32 (attention_backward
+    writes fp32); q, k: its inputs (None allowed without weights: the rotation's
+    adjoint does not need them). Returns (dq, dk, d_q_weight, d_k_weight): dq,
+    dk in out_dtype (default: q's, else the gradient's dtype), or in
+    out=(dq, dk); the weight gradients fp32 (D,), summed over every token and
+    head in a fixed order, None without weights.
+    """
+    if not isinstance(dq_out, torch.Tensor) or dq_out.dim() != 4 or \
+            not isinstance(dk_out, torch.Tensor) or dk_out.dim() != 4:
+        raise ValueError("dq_out and dk_out must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
+    B, S, H, D = dq_out.shape
+    Hkv = dk_out.shape[2]
+    gdt = dq_out.dtype
+    _heads4("dq_out", dq_out, (B, S, H, D))
+    _heads4("dk_out", dk_out, (B, S, Hkv, D), (gdt,))
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    norm = wq is not None
+    in_dt = gdt
+    if norm:
+        _heads4("q", q, (B, S, H, D))
+        in_dt = q.dtype
+        _heads4("k", k, (B, S, Hkv, D), (in_dt,))
+    elif q is not None:
+        in_dt = q.dtype
+    dev = dq_out.device
+    if out is None:
+        out_dtype = out_dtype or in_dt
+        dq = torch.empty((B, S, H, D), dtype=out_dtype, device=dev)
+        dk = torch.empty((B, S, Hkv, D), dtype=out_dtype, device=dev)
+    else:
+        dq, dk = out
+    _heads4("dq", dq, (B, S, H, D))
+    _heads4("dk", dk, (B, S, Hkv, D), (dq.dtype,))
+    if start is not None:
+        _require_vector("start", start, B, torch.int32)
+    x_q, x_k = (q, k) if norm else (None, None)
+    _same_device(dq_out, ("dk_out", dk_out), ("q", x_q), ("k", x_k), ("q_weight", q_weight),
+                 ("k_weight", k_weight), ("start", start), ("dq", dq), ("dk", dk),
+                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]))
+    dwq = dwk = None
+    if norm:
+        dwq = torch.empty((D,), dtype=torch.float32, device=dev)
+        dwk = torch.empty((D,), dtype=torch.float32, device=dev)
+    if B * S == 0:
+        if norm:
+            dwq.zero_()
+            dwk.zero_()
+        return dq, dk, dwq, dwk
+    none3 = (0, 0, 0)
+    a = nat.QkNormRopeBackwardArgs(
+        dq_out.data_ptr(), dk_out.data_ptr(), _ptr(x_q), _ptr(x_k), dq.data_ptr(), dk.data_ptr(),
+        _ptr(dwq), _ptr(dwk), B, S, H, Hkv, D, *dq_out.stride()[:3], *dk_out.stride()[:3],
+        *(q.stride()[:3] if norm else none3), *(k.stride()[:3] if norm else none3),
+        *dq.stride()[:3], *dk.stride()[:3], _DTYPES[in_dt], _DTYPES[gdt], _DTYPES[dq.dtype],
+        wq, wk, eps, cos, sin, rows, pos0, _ptr(start))
+    lib = nat.load()
+    need = lib.enl_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
+    if need:
+        ws = _workspace(dev, need)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    nat.check(lib.enl_qk_norm_rope_backward(ctypes.byref(a), _stream()),
+              "enl_qk_norm_rope_backward")
+    return dq, dk, dwq, dwk
+
+
+_zeroed: dict = {}
+
+
+def _zeroed_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch of attention_decode_paged, one per (device, stream) like
+    _workspace, zeroed when it is made: its kernels leave the counters in it at
+    zero for the next call."""
+    key = (device.index, _stream())
+    ws = _zeroed.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        _zeroed[key] = ws
+    return ws
+
+
+def paged_decode_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int,
+                                 head_dim: int) -> int:
+    """Bytes attention_decode_paged needs as its workspace at these sizes."""
+    a = nat.PagedDecodeArgs()
+    a.batch, a.num_heads, a.num_kv_heads, a.head_dim = batch, num_heads, num_kv_heads, head_dim
+    return int(nat.load().enl_paged_decode_workspace_bytes(ctypes.byref(a)))
+
+
+def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                           window: Optional[int] = None, sinks: int = 0,
+                           alibi_slopes: Optional[torch.Tensor] = None,
+                           scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                           out_dtype: Optional[torch.dtype] = None,
+                           workspace: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of one new token per sequence over a paged cache.
+
+    q: (B, H, D), the token at position seq_lens[b] - 1 of each sequence;
+    k_pages, v_pages: (num_pages, Hkv, page_size, D) pools of q's dtype (bf16 or
+    fp32) with equal strides; block_table: int32 (B, max_pages); seq_lens: int32
+    (B,) cached lengths, the new token included. All positions up to the query's
+    are seen, or with a window those at most `window` back and the sequence's
+    first `sinks`. H % Hkv == 0 with any ratio; D a multiple of 8 up to 128.
+    A sequence of length 0 gives zeros and an LSE of -inf. workspace: a zeroed
+    uint8 tensor of paged_decode_workspace_bytes (kept per stream by default; a
+    CUDA graph that replays beside other calls needs its own).
+    Returns out (B, H, D) in out_dtype (default: q's) [and lse (B, H) fp32].
+    """
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES or \
+            not q.is_cuda or q.stride(2) != 1:
+        raise ValueError("q must be a bf16/fp32 (batch, heads, head_dim) CUDA tensor with a "
+                         "contiguous head dimension")
+    B, H, D = q.shape
+    dt, dev = q.dtype, q.device
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
+        raise ValueError("k_pages must be a 4-D CUDA tensor (num_pages, kv_heads, page_size, "
+                         "head_dim)")
+    Hkv = k_pages.shape[1]
+    _page_pool(k_pages, v_pages, block_table, B, Hkv, D, dt)
+    _require_vector("seq_lens", seq_lens, B, torch.int32)
+    if window is not None and window < 0:
+        raise ValueError(f"window must be >= 0 or None, got {window}")
+    if sinks < 0 or (sinks > 0 and window is None):
+        raise ValueError(f"sinks={sinks} must be >= 0, and needs a window")
+    if alibi_slopes is not None:
+        _require_vector("alibi_slopes", alibi_slopes, H, torch.float32)
+    if out is None:
+        out = torch.empty((B, H, D), device=dev, dtype=out_dtype or dt)
+    elif out.dim() != 3 or out.shape != q.shape or out.dtype not in _DTYPES or \
+            out.stride(2) != 1:
+        raise ValueError(f"out must be ({B}, {H}, {D}) bf16/fp32 with a contiguous head dimension")
+    lse = torch.empty((B, H), device=dev, dtype=torch.float32) if return_lse else None
+    _same_device(q, ("k_pages", k_pages), ("v_pages", v_pages), ("block_table", block_table),
+                 ("seq_lens", seq_lens), ("alibi_slopes", alibi_slopes), ("out", out),
+                 ("workspace", workspace))
+    if B > 0:
+        a = nat.PagedDecodeArgs(
+            q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+            *k_pages.stride()[:3], k_pages.shape[0], k_pages.shape[2], block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), out.data_ptr(),
+            out.stride(0), out.stride(1), _ptr(lse), B, H, Hkv, D,
+            -1 if window is None else window, sinks, _ptr(alibi_slopes),
+            1.0 / math.sqrt(D) if scale is None else scale, _DTYPES[dt], _DTYPES[out.dtype])
+        lib = nat.load()
+        if workspace is None:
+            workspace = _zeroed_workspace(
+                dev, lib.enl_paged_decode_workspace_bytes(ctypes.byref(a)))
+        a.workspace = workspace.data_ptr()
+        a.workspace_bytes = workspace.numel() * workspace.element_size()
+        nat.check(lib.enl_attn_decode_paged(ctypes.byref(a), _stream()), "enl_attn_decode_paged")
+    return (out, lse) if return_lse else out
+
+
+def _per_row(name: str, value, B: int, dtype: torch.dtype, off):
+    """(device pointer or None, scalar) of a setting given per row or for all."""
+    if value is None:
+        return None, off
+    if isinstance(value, torch.Tensor):
+        _require_vector(name, value, B, dtype)
+        return value.data_ptr(), off
+    return None, value
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=None,
+                  top_p=None, min_p=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token id per row of logits, drawn with the given uniform numbers
+    (generative/text_generation.py:118-134, with min-p).
+
+    logits: (B, V) bf16 or fp32 with contiguous rows; u: fp32 (B,) in [0, 1).
+    temperature (0: greedy), top_k (0 or None: off), top_p (>= 1 or None: off)
+    and min_p (0 or None: off) are numbers for all rows or (B,) tensors (fp32,
+    top_k int32). Of the softmax of logits / temperature: the top_k largest (ties:
+    lowest index first), of those the smallest leading set whose mass reaches
+    top_p, of those the ones at least min_p times the largest; the token is the
+    first index whose running sum, in index order, exceeds u times the kept mass,
+    as numpy.random.choice draws. Weights are summed as whole numbers, so a row's
+    token does not depend on the rest of the batch. NaN logits count as -inf; a
+    row without a logit above -inf gives -1. Returns int64 (B,).
+    """
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or \
+            logits.dtype not in _DTYPES or not logits.is_cuda or \
+            (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be a bf16/fp32 (batch, vocab) CUDA tensor with contiguous "
+                         "rows")
+    B, V = logits.shape
+    _require_vector("u", u, B, torch.float32)
+    t_ptr, t_all = _per_row("temperature", temperature, B, torch.float32, 1.0)
+    k_ptr, k_all = _per_row("top_k", top_k, B, torch.int32, 0)
+    p_ptr, p_all = _per_row("top_p", top_p, B, torch.float32, 1.0)
+    m_ptr, m_all = _per_row("min_p", min_p, B, torch.float32, 0.0)
+    if not (t_all >= 0.0 and k_all >= 0 and p_all >= 0.0 and 0.0 <= m_all <= 1.0):
+        raise ValueError(f"temperature={t_all} top_k={k_all} top_p={p_all} must be >= 0 and "
+                         f"min_p={m_all} within [0, 1]")
+    if out is None:
+        out = torch.empty((B,), dtype=torch.int64, device=logits.device)
+    else:
+        _require_vector("out", out, B, torch.int64)
+    _same_device(logits, ("u", u), ("out", out),
+                 *((n, t) for n, t in (("temperature", temperature), ("top_k", top_k),
+                                       ("top_p", top_p), ("min_p", min_p))
+                   if isinstance(t, torch.Tensor)))
+    a = nat.SampleArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], B, V,
+                       u.data_ptr(), t_ptr, k_ptr, p_ptr, m_ptr, t_all, k_all, p_all, m_all,
+                       out.data_ptr())
+    nat.check(nat.load().enl_sample_tokens(ctypes.byref(a), _stream()), "enl_sample_tokens")
+    return out

@@ -434,6 +434,164 @@ int enl_sparse_build_masks(const enl_sparse_mask_args* args, void* stream);
 int enl_attn_prefill_sparse(const enl_prefill_args* args, const enl_sparse_layout* layout,
                             void* stream);
 
+/* ------------------------------------------------- serving over paged caches */
+/* A paged key-value cache: two pools of pages, k_pages and v_pages
+ * (num_pages, num_kv_heads, page_size, head_dim) described by element strides
+ * (page, kv head, slot; the head dim contiguous), shared by K and V, and a
+ * block table (batch, max_pages) of page numbers: position p of sequence b is
+ * slot p % page_size of page block_table[b, p / page_size]. Sequences of any
+ * lengths share the pools; no reference counterpart (nn/kvcache.py:23-66 keeps
+ * one contiguous array per batch). */
+typedef struct enl_qk_norm_rope_args {
+  const void* q; /* (batch, seq, num_heads, head_dim), in_dtype */
+  const void* k; /* (batch, seq, num_kv_heads, head_dim) */
+  const void* v; /* as k; read only with k_pages (copied into the pages), else may be NULL */
+  void* q_out;   /* (batch, seq, num_heads, head_dim), out_dtype; may be q itself */
+  void* k_out;   /* (batch, seq, num_kv_heads, head_dim), out_dtype; NULL with k_pages */
+  int32_t batch, seq, num_heads, num_kv_heads, head_dim;
+  int64_t q_stride_b, q_stride_s, q_stride_h; /* element strides */
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t qo_stride_b, qo_stride_s, qo_stride_h;
+  int64_t ko_stride_b, ko_stride_s, ko_stride_h;
+  int32_t in_dtype, out_dtype; /* ENL_DTYPE_BF16 or ENL_DTYPE_FP32; equal with k_pages */
+  const float* q_weight;       /* (head_dim) fp32 norm weights, 16-byte aligned; both or */
+  const float* k_weight;       /* neither (NULL: no norm, only the rotation) */
+  float eps;
+  const float* rope_cos; /* (rope_rows, head_dim / 2) fp32 tables as nn/forward.py:46-55 */
+  const float* rope_sin; /* computes them, 16-byte aligned; both NULL: no rotation */
+  int64_t rope_rows;
+  int64_t pos0;         /* token s of row b sits at position pos0 + start[b] + s */
+  const int32_t* start; /* device (batch,); NULL = zeros; required with k_pages */
+  /* With k_pages: normalised and rotated keys, and the values as they are, go
+   * to the cache at those positions instead of k_out. */
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride_p, page_stride_h, page_stride_s;
+  int32_t num_pages, page_size;
+  const int32_t* block_table; /* device (batch, max_pages), rows table_stride_b apart */
+  int64_t table_stride_b;
+  int32_t max_pages;
+  const int32_t* n_new; /* device (batch,): tokens s >= n_new[b] are padding: nothing is
+                           cached for them and their q_out is zero. NULL = none; only
+                           with k_pages */
+} enl_qk_norm_rope_args;
+
+/* For each head x of q and k, in one pass: z = w * x / sqrt(mean(x^2) + eps)
+ * (RMS norm over the head), then the rotate-half position rotation
+ * (nn/forward.py:80-88). fp32 arithmetic, one rounding to out_dtype. head_dim
+ * a multiple of 8 up to 128. A position outside the tables or a page outside
+ * the pool records an error in the device error word (code 2); that token's
+ * outputs are zero and it is not cached. */
+int enl_qk_norm_rope(const enl_qk_norm_rope_args* args, void* stream);
+
+typedef struct enl_qk_norm_rope_backward_args {
+  const void* dq_out; /* gradients of q_out / k_out, grad_dtype */
+  const void* dk_out;
+  const void* q; /* the forward's inputs, in_dtype; may be NULL without norm weights */
+  const void* k;
+  void* dq; /* gradients of q / k, out_dtype; may be dq_out / dk_out themselves */
+  void* dk;
+  float* dq_weight; /* (head_dim) fp32, with norm weights */
+  float* dk_weight;
+  int32_t batch, seq, num_heads, num_kv_heads, head_dim;
+  int64_t dqo_stride_b, dqo_stride_s, dqo_stride_h;
+  int64_t dko_stride_b, dko_stride_s, dko_stride_h;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t dq_stride_b, dq_stride_s, dq_stride_h;
+  int64_t dk_stride_b, dk_stride_s, dk_stride_h;
+  int32_t in_dtype, grad_dtype, out_dtype;
+  const float* q_weight;
+  const float* k_weight;
+  float eps;
+  const float* rope_cos;
+  const float* rope_sin;
+  int64_t rope_rows;
+  int64_t pos0;
+  const int32_t* start;
+  void* workspace; /* >= enl_qk_norm_rope_backward_workspace_bytes(), 16-byte aligned */
+  size_t workspace_bytes;
+} enl_qk_norm_rope_backward_args;
+
+/* Gradients of enl_qk_norm_rope: with dz the gradient turned back by the
+ * token's angles (nn/backward.py:300-308), xh = x / sqrt(mean(x^2) + eps) and
+ * g = w * dz: dx = (g - xh mean(g xh)) / sqrt(mean(x^2) + eps), dw the sum of
+ * dz * xh over every token and head, added in a fixed order. */
+int enl_qk_norm_rope_backward(const enl_qk_norm_rope_backward_args* args, void* stream);
+
+/* Workspace bytes of enl_qk_norm_rope_backward: the per-block partial sums of
+ * the weight gradients (0 without norm weights). */
+size_t enl_qk_norm_rope_backward_workspace_bytes(const enl_qk_norm_rope_backward_args* args);
+
+typedef struct enl_paged_decode_args {
+  const void* q; /* (batch, num_heads, head_dim), dtype: the newest token of each sequence */
+  int64_t q_stride_b, q_stride_h;
+  const void* k_pages;
+  const void* v_pages;
+  int64_t page_stride_p, page_stride_h, page_stride_s;
+  int32_t num_pages, page_size;
+  const int32_t* block_table; /* device (batch, max_pages) */
+  int64_t table_stride_b;
+  int32_t max_pages;
+  const int32_t* seq_lens; /* device (batch,): cached positions, the query's own included */
+  void* o;                 /* (batch, num_heads, head_dim), out_dtype */
+  int64_t o_stride_b, o_stride_h;
+  float* lse; /* (batch, num_heads) natural-log LSE, or NULL */
+  int32_t batch, num_heads, num_kv_heads, head_dim;
+  int32_t window;            /* < 0: none; else only keys at most window positions back, */
+  int32_t sinks;             /* and the sequence's first sinks positions, are seen */
+  const float* alibi_slopes; /* device (num_heads,) or NULL */
+  float scale;
+  int32_t in_dtype, out_dtype;
+  void* workspace; /* >= enl_paged_decode_workspace_bytes(), 256-byte aligned, zeroed before
+                      its first use; calls leave it as the next one needs it */
+  size_t workspace_bytes;
+} enl_paged_decode_args;
+
+/* Attention of one new token per sequence over a paged cache: the query of
+ * sequence b sits at position seq_lens[b] - 1. A sequence of length 0 gets a
+ * zero output and an LSE of -inf. Any num_heads / num_kv_heads ratio; head_dim
+ * a multiple of 8 up to 128; bf16 or fp32 (fp32-accurate products either way).
+ * The lengths are read on the device, so a call can sit in a CUDA graph while
+ * they grow. A length above max_pages * page_size is cut to it, and a page
+ * outside the pool counts as masked; both set the device error word (code 2). */
+int enl_attn_decode_paged(const enl_paged_decode_args* args, void* stream);
+
+/* Workspace bytes of enl_attn_decode_paged; depends on the head counts and
+ * sizes only, not on the lengths. */
+size_t enl_paged_decode_workspace_bytes(const enl_paged_decode_args* args);
+
+typedef struct enl_sample_args {
+  const void* logits; /* (batch, vocab) rows stride_b elements apart */
+  int64_t stride_b;
+  int32_t dtype; /* ENL_DTYPE_BF16 or ENL_DTYPE_FP32 */
+  int32_t batch, vocab;
+  const float* u; /* device (batch,): one uniform number in [0, 1) per row */
+  /* Per-row settings on the device, (batch,) each, or NULL for the scalar
+   * below for every row. */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all; /* <= 0: greedy */
+  int32_t top_k_all;     /* <= 0: off */
+  float top_p_all;       /* >= 1: off */
+  float min_p_all;       /* <= 0: off */
+  int64_t* tokens;       /* device out (batch,) */
+} enl_sample_args;
+
+/* One token per row (generative/text_generation.py:118-134, min-p added):
+ * weights w_i = exp((l_i - max l) / T), the temperature_all-scaled softmax
+ * without its divisor; keep the top_k largest (ties: the lowest index first),
+ * of those the smallest leading set whose weight reaches top_p of theirs, and
+ * of those the ones with w_i >= min_p; the token is the first index, in index
+ * order, whose running sum of kept weights exceeds u times their total. Sums
+ * are of whole numbers floor(w_i 2^40), so the token does not depend on the
+ * order of addition. NaN logits count as -inf, a row without any logit above
+ * -inf gives -1. vocab up to 2^22. */
+int enl_sample_tokens(const enl_sample_args* args, void* stream);
+
 /* ------------------------------------------------------------- utilities */
 /* Read (and with clear != 0 reset) the device error word of the current
  * device. Synchronises the device. *code == 0 means no kernel reported. */

@@ -1,0 +1,185 @@
+"""Serving operators without a GPU: the oracle's own consistency, the ABI's
+struct layouts, and the refusals that come before any launch."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from enilnets_b200 import _native
+from oracle import attention_ref
+from oracle import serving_ref as ref
+from tests.test_abi import _c_offsets
+
+
+@pytest.mark.parametrize("cls,cname", [
+    (_native.QkNormRopeArgs, "enl_qk_norm_rope_args"),
+    (_native.QkNormRopeBackwardArgs, "enl_qk_norm_rope_backward_args"),
+    (_native.PagedDecodeArgs, "enl_paged_decode_args"),
+    (_native.SampleArgs, "enl_sample_args")])
+def test_ctypes_struct_layout_matches_c(cls, cname):
+    fields = [f for f, _ in cls._fields_]
+    size, offsets = _c_offsets(cname, fields)
+    assert ctypes.sizeof(cls) == size
+    for f, off in zip(fields, offsets):
+        assert getattr(cls, f).offset == off, f
+
+
+def _rope_args():
+    a = _native.QkNormRopeArgs()
+    a.q = a.k = a.q_out = a.k_out = a.q_weight = a.k_weight = 256
+    a.batch = a.seq = 1
+    a.num_heads, a.num_kv_heads, a.head_dim = 4, 2, 64
+    return a
+
+
+def _call(name, a):
+    lib = _native.load()
+    _native.check(getattr(lib, name)(ctypes.byref(a), None), name)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(num_kv_heads=3), "must divide"), (dict(head_dim=100), "head_dim=100"),
+    (dict(head_dim=136), "head_dim=136"), (dict(in_dtype=5), "in_dtype=5"),
+    (dict(out_dtype=-1), "out_dtype=-1"), (dict(k_weight=None), "come in pairs"),
+    (dict(rope_cos=256), "come in pairs"), (dict(rope_cos=256, rope_sin=256), "rope_rows=0"),
+    (dict(q_weight=None, k_weight=None), "norm weights, rotation tables or both"),
+    (dict(q=None), "q must be non-NULL"), (dict(k_out=8), "k_out must be 16-byte"),
+    (dict(q_stride_s=-64), "multiples of 16 bytes"), (dict(k_stride_h=20), "multiples of 16 bytes"),
+    (dict(n_new=256), "n_new needs k_pages"), (dict(batch=-1), "batch=-1"),
+    (dict(k_pages=256), "v must be non-NULL"),
+    (dict(k_pages=256, v=256), "block_table must be non-NULL"),
+    (dict(k_pages=256, v_pages=256, v=256, block_table=256), "num_pages=0"),
+    (dict(k_pages=256, v_pages=256, v=256, block_table=256, num_pages=1, page_size=1 << 20,
+          max_pages=1 << 11), "below 2\\^31"),
+    (dict(k_pages=256, v_pages=256, v=256, block_table=256, num_pages=1, page_size=16,
+          max_pages=1), "start must be non-NULL"),
+    (dict(k_pages=256, v_pages=256, v=256, block_table=256, num_pages=1, page_size=16,
+          max_pages=1, start=256, out_dtype=1), "must be equal"),
+    (dict(k_pages=256, v_pages=256, v=256, block_table=256, num_pages=1, page_size=16,
+          max_pages=1, start=256, pos0=4), "pos0 must be 0"),
+])
+def test_norm_rope_refusals(change, message):
+    a = _rope_args()
+    for name, value in change.items():
+        setattr(a, name, value)
+    with pytest.raises(ValueError, match=message):
+        _call("enl_qk_norm_rope", a)
+
+
+def test_norm_rope_empty_calls_launch_nothing():
+    a = _rope_args()
+    a.seq = 0
+    _call("enl_qk_norm_rope", a)
+    a.seq, a.batch = 1, 0
+    _call("enl_qk_norm_rope", a)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(seq=0), "seq=0"), (dict(num_heads=5), "must divide"), (dict(grad_dtype=9), "grad_dtype=9"),
+    (dict(q_weight=256), "come in pairs"), (dict(rope_sin=256), "come in pairs"),
+    (dict(), "norm weights, rotation tables or both"),
+    (dict(rope_cos=256, rope_sin=256, rope_rows=4), "dq_out must be non-NULL"),
+])
+def test_norm_rope_backward_refusals(change, message):
+    a = _native.QkNormRopeBackwardArgs()
+    a.batch = a.seq = 1
+    a.num_heads, a.num_kv_heads, a.head_dim = 4, 2, 64
+    for name, value in change.items():
+        setattr(a, name, value)
+    with pytest.raises(ValueError, match=message):
+        _call("enl_qk_norm_rope_backward", a)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(num_heads=3), "must divide"), (dict(head_dim=12), "head_dim=12"),
+    (dict(sinks=-1), "sinks=-1"), (dict(seq_lens=None), "seq_lens must be non-NULL"),
+    (dict(q=None), "q must be non-NULL"), (dict(o=4), "o must be 16-byte"),
+    (dict(page_stride_s=4), "multiples of 16 bytes"), (dict(max_pages=0), "max_pages=0"),
+    (dict(in_dtype=2), "in_dtype=2"), (dict(batch=-3), "batch=-3"),
+])
+def test_paged_decode_refusals(change, message):
+    a = _native.PagedDecodeArgs()
+    a.q = a.k_pages = a.v_pages = a.block_table = a.seq_lens = a.o = 256
+    a.batch, a.num_heads, a.num_kv_heads, a.head_dim = 1, 4, 2, 64
+    a.num_pages = a.max_pages = 2
+    a.page_size = 16
+    for name, value in change.items():
+        setattr(a, name, value)
+    with pytest.raises(ValueError, match=message):
+        _call("enl_attn_decode_paged", a)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(vocab=0), "vocab=0"), (dict(vocab=(1 << 22) + 1), "2\\^22"), (dict(dtype=3), "dtype=3"),
+    (dict(logits=None), "non-NULL"), (dict(u=None), "non-NULL"), (dict(stride_b=10), "stride_b=10"),
+    (dict(logits=257), "aligned"), (dict(batch=-1), "batch=-1"),
+])
+def test_sample_refusals(change, message):
+    a = _native.SampleArgs()
+    a.logits = a.u = a.tokens = 256
+    a.batch, a.vocab, a.stride_b = 2, 100, 100
+    for name, value in change.items():
+        setattr(a, name, value)
+    with pytest.raises(ValueError, match=message):
+        _call("enl_sample_tokens", a)
+
+
+def test_oracle_norm_rope_gradient_matches_differences():
+    rng = np.random.RandomState(3)
+    x, w = rng.standard_normal((2, 3, 2, 16)), 1 + 0.3 * rng.standard_normal(16)
+    cos, sin = attention_ref.rope_tables(5, 16)
+    cos, sin = cos[2:5, None], sin[2:5, None]
+    dy = rng.standard_normal(x.shape)
+    dx, dw = ref.norm_rope_backward(dy, x, w, 1e-6, cos, sin)
+    f = lambda a, b: np.sum(dy * ref.norm_rope(a, b, 1e-6, cos, sin))  # noqa: E731
+    vx, vw = rng.standard_normal(x.shape), rng.standard_normal(16)
+    h = 1e-5
+    assert abs((f(x + h * vx, w) - f(x - h * vx, w)) / (2 * h) - np.sum(dx * vx)) < 1e-7
+    assert abs((f(x, w + h * vw) - f(x, w - h * vw)) / (2 * h) - np.sum(dw * vw)) < 1e-7
+
+
+def test_oracle_paged_decode_equals_contiguous_oracle():
+    rng = np.random.RandomState(4)
+    B, H, Hkv, D, n, page = 2, 4, 2, 8, 37, 5
+    K, V = rng.standard_normal((2, B, Hkv, n, D))
+    q = rng.standard_normal((B, H, D))
+    table = rng.permutation(B * 8).reshape(B, 8)
+    kp, vp = np.full((2, B * 8, Hkv, page, D), np.nan)
+    for b in range(B):
+        for j in range(n):
+            kp[table[b, j // page], :, j % page] = K[b, :, j]
+            vp[table[b, j // page], :, j % page] = V[b, :, j]
+    for window in (None, 0, 6):
+        o, lse = ref.paged_decode(q, kp, vp, table, [n, n], window=window)
+        oref, lref = attention_ref.decode_ref(q, K, V, slot_begin=0, slot_end=n, pos_slot0=0,
+                                              q_pos=n - 1, window=window)
+        np.testing.assert_allclose(o, oref, atol=1e-12)
+        np.testing.assert_allclose(lse, lref, atol=1e-12)
+
+
+def test_oracle_sampling_follows_the_host_sampler():
+    """The draw of one uniform number equals the host path's temperature ->
+    top-k -> top-p -> numpy.random.choice (which inverts the running sum with one
+    random_sample) where the filters keep distinct probabilities."""
+    from enilnets_b200 import generation
+    rng = np.random.RandomState(5)
+    for i in range(50):
+        logits = rng.standard_normal(60) * 3
+        probs = np.exp(logits - logits.max())
+        probs /= probs.sum()
+        T, k, p = (1.0, 0.7, 1.4)[i % 3], (None, 10)[i % 2], (None, 0.8)[i // 2 % 2]
+        np.random.seed(i)
+        u = np.random.random_sample()
+        np.random.seed(i)
+        token = generation.sample_token(probs, T, p, k)
+        assert token in ref.sample_answers(logits, u, T, k or 0, p or 1.0)
+
+
+def test_oracle_sampling_edges():
+    nan, inf = np.nan, np.inf
+    assert ref.sample([-inf, -inf], 0.5) == -1
+    assert ref.sample([nan, 1.0], 0.5) == 1
+    assert ref.sample([2.0, inf, inf], 0.75) == 2
+    assert ref.sample([1.0, 1.0, 1.0], 0.99, top_k=2) == 1   # ties: lowest indices first
+    assert ref.sample([0.0, 1.0, 1.0], 0.9, temperature=0.0) == 1
+    assert ref.sample([0.0, 5.0], 0.999999, top_p=0.0) == 1
