@@ -9,23 +9,25 @@
 // i.e. they are the tokens at or above one 64-bit composite of the logit's
 // order-preserving bits and the complement of the index.
 //
-// One block per row. The first pass streams the row from HBM and keeps only
-// maxima: the row's and, per thread, those of four parts of what it read
-// (2048 groups). What follows reads the row again from L2, and only where it
-// has to:
+// A row belongs to one block, or to a cluster of 2 to 8 when there are fewer rows
+// than SMs (choose_cluster). The first pass streams the row from HBM and keeps
+// only extremes: the row's and, per thread, the maxima of four parts of what it
+// read (2048 groups a block). What follows reads the row again from L2, and only
+// where it has to:
 //  * top-k up to kSmallK: the k-th largest group maximum bounds the k-th largest
 //    logit from below, so only groups at or above it (about k of them) are read
-//    again. Their few candidates are sorted in shared memory, and the rest of
-//    the row is never touched.
+//    again. Their few candidates go to one list in shared memory, where they
+//    are ranked, and the rest of the row is never touched.
+//  * min-p alone: the same with the groups whose maximum weighs min_p or more.
 //  * top-p alone: one more pass for the exact total, then the same with about
-//    kNucleus candidates, provided that they carry the wanted mass.
+//    kNucleus groups, provided that their candidates carry the wanted mass.
 //  * larger top-k, flatter nuclei: a histogram of the logits finds the bin that
 //    the cut falls into, one pass sums what lies above it and collects the bin's
 //    tokens, which are sorted.
 //  * rows that defeat the bins (thousands of equal logits at the cut): bisection
 //    over the composite, one pass per bit.
-// Without a cut (temperature alone, min-p) one pass sums the row in ranges and
-// the range that holds the draw is walked again.
+// With temperature alone one pass sums the row in ranges and the range that
+// holds the draw is walked again.
 #include <cstdint>
 
 #include "enl_common.cuh"
@@ -42,7 +44,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kGroups = 4;       // group maxima per thread
 constexpr int kCap = 2048;       // candidates that fit the shared-memory sort
 constexpr int kSmallK = 1024;    // largest top-k of the group path
-constexpr int kNucleus = 640;    // groups asked for when only top-p cuts
+constexpr int kNucleus = 512;    // groups asked for when only top-p cuts
+constexpr int kRank = 256;       // candidates that are ranked by counting, not sorted
+constexpr int kMaxCluster = 8;
 constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
 constexpr float kOne = 1099511627776.0f;  // 2^40
@@ -104,23 +108,31 @@ struct Vec {
   }
 };
 
-// Running maximum of vectors; NaN is dropped. bf16 stays packed.
+// Running maximum of a group's vectors, and (in `row`) the smallest logit of
+// all of them; NaN is dropped. bf16 stays packed.
 template <bool kF32>
-struct Maximum {
-  float f = -INFINITY;
-  __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY);
+struct Extremes {
+  float f = -INFINITY, g = INFINITY;
+  __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY), l = __float2bfloat162_rn(INFINITY);
 
-  __device__ __forceinline__ void add(const Vec<kF32>& x) {
+  __device__ __forceinline__ void add(const Vec<kF32>& x, Extremes& row) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (kF32)
+      if constexpr (kF32) {
         f = fmaxf(f, __uint_as_float(x.w[i]));
-      else
-        h = __hmax2(h, *reinterpret_cast<const __nv_bfloat162*>(&x.w[i]));
+        row.g = fminf(row.g, __uint_as_float(x.w[i]));
+      } else {
+        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&x.w[i]);
+        h = __hmax2(h, v);
+        row.l = __hmin2(row.l, v);
+      }
     }
   }
-  __device__ __forceinline__ float get() const {
+  __device__ __forceinline__ float max() const {
     return kF32 ? f : fmaxf(__low2float(h), __high2float(h));
+  }
+  __device__ __forceinline__ float min() const {
+    return kF32 ? g : fminf(__low2float(l), __high2float(l));
   }
 };
 
@@ -147,10 +159,11 @@ struct Row {
     else
       return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[mis + i]);
   }
-  __device__ __forceinline__ float logit_or_low(int i) const {
-    return i >= 0 && i < V ? one(i) : -INFINITY;
+  __device__ __forceinline__ float logit_or_nan(int i) const {
+    return i >= 0 && i < V ? one(i) : __uint_as_float(0x7fff0000u);
   }
-  // Vector j; indices outside the row read as -inf (and touch no memory).
+  // Vector j; indices outside the row read as NaN, which counts nowhere (and
+  // touch no memory).
   __device__ __forceinline__ Vec<kF32> get(int j) const {
     Vec<kF32> r;
     if (inside(j)) {
@@ -160,10 +173,10 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (kF32) {
-          r.w[e] = __float_as_uint(logit_or_low(j * E - mis + e));
+          r.w[e] = __float_as_uint(logit_or_nan(j * E - mis + e));
         } else {
-          r.w[e] = __float_as_uint(logit_or_low(j * E - mis + 2 * e)) >> 16 |
-                   __float_as_uint(logit_or_low(j * E - mis + 2 * e + 1));
+          r.w[e] = __float_as_uint(logit_or_nan(j * E - mis + 2 * e)) >> 16 |
+                   __float_as_uint(logit_or_nan(j * E - mis + 2 * e + 1));
         }
       }
     }
@@ -171,17 +184,66 @@ struct Row {
   }
 };
 
+// A composite list entry's token, and its logit's bits.
+__device__ __forceinline__ uint32_t index_of(u64 comp) { return ~(uint32_t)comp; }
+
+struct Pair {
+  u64 a, b;
+};
+
 struct Shared {
   union {
-    u64 list[kCap];         // candidates (composites), sorted in place
-    uint32_t bins[kBins];   // histogram
+    u64 list[kCap];  // candidates (composites)
+    struct {
+      uint32_t bins[kBins];  // histogram: tokens, and the weight of
+      float heavy[kBins];    // those above 2^-10 of the largest
+    };
   };
-  u64 order[kCap];          // kept candidates by index
-  u64 part[kWarps + 1];
+  union {
+    u64 order[kCap];  // kept candidates by index
+    u64 q[kCap];      // whole weights of the list's entries
+    u64 mass[kGroupBins];
+  };
+  u64 part[kWarps];
   float fpart[kWarps];
-  uint32_t gbins[kGroupBins];
-  int count, found;
+  Pair swap[2][kMaxCluster];  // what the cluster's blocks tell each other
+  uint32_t gbins[kGroupBins], gsum[kGroupBins];
+  int groups[kThreads * kGroups];  // first vectors of the groups to read again
+  u64 cut;  // composite found by rank 0
+  int count, found, n_groups;
 };
+
+// ------------------------------------------------------- block and cluster
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Shared-memory address of `p` in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void remote_store(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ u64 remote_load64(uint32_t addr) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t remote_load(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int remote_add(uint32_t addr, int v) {
+  int old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v)
+               : "memory");
+  return old;
+}
 
 __device__ __forceinline__ u64 warp_sum(u64 x) {
 #pragma unroll
@@ -239,75 +301,152 @@ __device__ void block_sort(u64* a, int n) {
 
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
+__device__ __forceinline__ uint32_t draw_part(float u) {
+  return (uint32_t)(fminf(fmaxf(u, 0.0f), 0.99999994f) * 16777216.0f);
+}
+
+// ------------------------------------------------------------------- sampler
 template <bool kF32>
 struct Sampler {
   static constexpr int E = Vec<kF32>::E;
   Row<kF32> row;
   Shared& sm;
-  float top, inv_t, min_p;
-  int per_warp;  // vectors of a warp's contiguous range, a multiple of 32
+  const int n_blocks;   // of the cluster
+  const uint32_t rank;  // of this block
+  int turn = 0;         // exchanges so far
+  float top = 0.0f, inv_t = 1.0f, min_p = 0.0f;
+  int per_warp;   // vectors of a warp's contiguous range, a multiple of 32
+  int per_group;  // steps of 32 vectors of a group (the last may have fewer)
 
-  __device__ Sampler(const void* p, int V, Shared& s) : row(p, V), sm(s) {
-    per_warp = (row.n_vec + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  __device__ Sampler(const void* p, int V, Shared& s, int blocks, uint32_t r)
+      : row(p, V), sm(s), n_blocks(blocks), rank(r) {
+    const int ranges = blocks * kWarps * 32;
+    per_warp = (row.n_vec + ranges - 1) / ranges * 32;
+    per_group = (per_warp / 32 + kGroups - 1) / kGroups;
   }
-  __device__ __forceinline__ int first_vec() const {
-    return (threadIdx.x / 32) * per_warp + threadIdx.x % 32;
+  __device__ __forceinline__ int warp_begin() const {
+    return ((int)rank * kWarps + threadIdx.x / 32) * per_warp;
   }
-  __device__ __forceinline__ int end_vec() const {
-    return min(row.n_vec, (int)(threadIdx.x / 32 + 1) * per_warp);
-  }
+  __device__ __forceinline__ int first_vec() const { return warp_begin() + threadIdx.x % 32; }
+  __device__ __forceinline__ int end_vec() const { return min(row.n_vec, warp_begin() + per_warp); }
+  __device__ __forceinline__ int group_first(int g) const { return first_vec() + 32 * per_group * g; }
   __device__ __forceinline__ float weight(float x) const { return weight_of(x, top, inv_t); }
-  __device__ __forceinline__ u64 whole(u64 comp) const {
-    return whole_of(weight(of_key((uint32_t)(comp >> 32))));
-  }
-
+  __device__ __forceinline__ float logit_of(u64 comp) const { return of_key((uint32_t)(comp >> 32)); }
+  __device__ __forceinline__ u64 whole(u64 comp) const { return whole_of(weight(logit_of(comp))); }
   // Logits below this have no weight.
   __device__ __forceinline__ float cutoff() const {
     return top == INFINITY ? top : top - kLive / inv_t;
   }
 
-  // f(value, index) for every logit that this thread reads.
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    const int end = end_vec();
-    int j = first_vec();
-    for (; j + 96 < end; j += 128) {
-      Vec<kF32> x[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = row.get(j + 32 * u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) f(x[u].at(e), (j + 32 * u) * E - row.mis + e);
-    }
-    for (; j < end; j += 32) {
-      const Vec<kF32> x = row.get(j);
-#pragma unroll
-      for (int e = 0; e < E; ++e) f(x.at(e), j * E - row.mis + e);
+  // Waits for the cluster's blocks; shared memory written before is visible
+  // after, to all of them.
+  __device__ __forceinline__ void sync() const {
+    if (n_blocks == 1) {
+      __syncthreads();
+    } else {
+      asm volatile("barrier.cluster.arrive.release;\n"
+                   "barrier.cluster.wait.acquire;" ::: "memory");
     }
   }
+  // Every block's x and y (the same in all its threads), by rank. Two buffers
+  // in turn: one is written again only after every block has passed the wait
+  // that follows its reading.
+  __device__ __forceinline__ const Pair* exchange(u64 x, u64 y) {
+    Pair* buf = sm.swap[turn & 1];
+    ++turn;
+    if (n_blocks == 1) {
+      __syncthreads();  // the buffer's last readers are done
+      if (threadIdx.x == 0) buf[0] = Pair{x, y};
+    } else if (threadIdx.x < n_blocks) {
+      const uint32_t a = remote(&buf[rank], threadIdx.x);
+      remote_store(a, x);
+      remote_store(a + 8, y);
+    }
+    sync();
+    return buf;
+  }
+  __device__ Pair cluster_sum(u64 x, u64 y) {
+    x = block_sum(x, sm);
+    y = block_sum(y, sm);
+    if (n_blocks == 1) return Pair{x, y};
+    const Pair* p = exchange(x, y);
+    Pair s{0, 0};
+    for (int r = 0; r < n_blocks; ++r) s.a += p[r].a, s.b += p[r].b;
+    return s;
+  }
+  __device__ u64 cluster_sum(u64 x) {
+    x = block_sum(x, sm);
+    if (n_blocks == 1) return x;
+    const Pair* p = exchange(x, 0);
+    u64 s = 0;
+    for (int r = 0; r < n_blocks; ++r) s += p[r].a;
+    return s;
+  }
 
-  // Exact sum of the whole weights of the row.
-  __device__ u64 row_mass() const {
+  // f(value, index) for the logits of vectors j, j + 32, ... below end, four
+  // loads in flight.
+  template <class F>
+  __device__ __forceinline__ void each_in(int j, int end, F f) const {
+    for (; j < end; j += 128) {
+      Vec<kF32> x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + 32 * u < end) x[u] = row.get(j + 32 * u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + 32 * u < end) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) f(x[u].at(e), (j + 32 * u) * E - row.mis + e);
+        }
+    }
+  }
+  // ... for every logit that this thread reads.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    each_in(first_vec(), end_vec(), f);
+  }
+
+  // This thread's sum of the whole weights of its logits.
+  __device__ u64 mass() const {
     u64 s = 0;
     const int end = end_vec();
-    for (int j0 = first_vec(); j0 < end; j0 += 32 * 64) {  // at most 512 tokens a stretch
+    if (top == INFINITY) {  // only the infinite logits weigh anything, 2^40 each
+      each([&](float x, int) { s += x == top ? whole_of(1.0f) : 0; });
+      return s;
+    }
+    for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {  // at most 1024 logits a stretch
       WholeSum w;
-#pragma unroll 4
-      for (int j = j0; j < min(end, j0 + 32 * 64); j += 32) {
+      const int stop = min(end, j0 + 32 * 128);
+#pragma unroll 2
+      for (int j = j0; j < stop; j += 32) {
         const Vec<kF32> x = row.get(j);
 #pragma unroll
-        for (int e = 0; e < E; ++e) w.add(x.at(e) > -INFINITY ? weight(x.at(e)) : 0.0f);
+        for (int e = 0; e < E; ++e) {
+          // NaN and -inf take the bound, whose weight is zero; at the top the
+          // argument is zero.
+          const float a = fmaxf((x.at(e) - top) * inv_t, -100.0f);
+          w.add(expf(a));
+        }
       }
       s += w.total();
     }
-    return block_sum(s, sm);
+    return s;
   }
 
-  // Appends a composite to the list; the list may overflow (count says so).
+  // Adds a composite to rank 0's list; it may overflow (its count says so).
   __device__ __forceinline__ void push(float x, int i) const {
-    const int at = atomicAdd(&sm.count, 1);
-    if (at < kCap) sm.list[at] = composite(x, i);
+    const u64 c = composite(x, i);
+    if (n_blocks == 1) {
+      const int at = atomicAdd(&sm.count, 1);
+      if (at < kCap) sm.list[at] = c;
+    } else {
+      const int at = remote_add(remote(&sm.count, 0), 1);
+      if (at < kCap) remote_store(remote(&sm.list[at], 0), c);
+    }
+  }
+  // Entries pushed, for every block, once all have.
+  __device__ __forceinline__ int list_size() const {
+    return n_blocks == 1 ? sm.count : (int)remote_load(remote(&sm.count, 0));
   }
 
   // Sorts the list (n entries) with the largest composite first.
@@ -317,35 +456,83 @@ struct Sampler {
     block_sort<true>(sm.list, N);
   }
 
-  // In the sorted list: sums of whole weights of this thread's four entries,
-  // before (exclusive) and in all.
-  __device__ u64 list_scan(const u64* list, int n, u64 (&q)[4], u64& total) const {
+  // Whole weights of this thread's four list entries, their sum's place among
+  // the threads (exclusive) and the total.
+  __device__ u64 list_scan(int n, u64 (&q)[4], u64& total) const {
     u64 mine = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = threadIdx.x * 4 + e;
-      q[e] = r < n ? whole(list[r]) : 0;
+      q[e] = r < n ? whole(sm.list[r]) : 0;
       mine += q[e];
     }
     return block_scan(mine, total, sm);
   }
 
-  // Index-order draw among the first n entries of the sorted list.
-  __device__ void draw_from_list(int n, float u, long long* token) const {
-    const int N = pow2_at_least(n);
-    for (int t = threadIdx.x; t < N; t += kThreads) {
-      const u64 c = sm.list[t];
-      sm.order[t] = t < n ? ((u64)(uint32_t)~(uint32_t)c << 32) | (c >> 32) : ~0ull;
+  // ------------------------------------------------------ rank 0: the list
+  // Draws from the list's n entries: the first n_k by rank, of those the
+  // leading run that reaches `bound` (part of the n_k's total when bound is 0
+  // and use_p is set), of those the ones with w >= min_p.
+  __device__ void draw_ranked(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+                              long long* token) const {
+    // Threads share each entry's count over the others.
+    const int shared = kThreads / max(16, pow2_at_least(n));
+    const int i = threadIdx.x / shared, sub = threadIdx.x % shared;
+    const bool live = i < n;
+    if (threadIdx.x < n) sm.q[threadIdx.x] = whole(sm.list[threadIdx.x]);
+    __syncthreads();
+    const u64 mine = live ? sm.list[i] : 0;
+    const u64 q = live ? sm.q[i] : 0;
+    int before_n = 0;
+    u64 before = 0;
+    for (int j = sub; j < n; j += shared)
+      if (sm.list[j] > mine) ++before_n, before += sm.q[j];
+    for (int off = shared / 2; off > 0; off >>= 1) {
+      before_n += __shfl_xor_sync(0xffffffffu, before_n, off);
+      before += __shfl_xor_sync(0xffffffffu, before, off);
     }
+    const bool in_k = live && before_n < n_k;
+    if (use_p && bound == 0)
+      bound = max(share_of(block_sum(in_k && sub == 0 ? q : 0, sm), part), (u64)1);
+    const bool keep = in_k && (!use_p || before < bound) && weight(logit_of(mine)) >= min_p;
+    __syncthreads();  // the weights have been read
+    if (live && sub == 0) sm.q[i] = keep ? q : 0;
+    const u64 target = share_of(block_sum(keep && sub == 0 ? q : 0, sm), draw_part(u));
+    u64 run = 0;
+    for (int j = sub; j < n; j += shared)
+      if (index_of(sm.list[j]) < index_of(mine)) run += sm.q[j];
+    for (int off = shared / 2; off > 0; off >>= 1) run += __shfl_xor_sync(0xffffffffu, run, off);
+    if (keep && sub == 0 && run <= target && target < run + q) *token = index_of(mine);
+  }
+
+  // The same for a long list, by sorting.
+  __device__ void draw_sorted(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+                              long long* token) const {
+    sort_list(n);
+    u64 q[4], total;
+    u64 run = list_scan(n_k, q, total);
+    if (use_p && bound == 0) bound = max(share_of(total, part), (u64)1);
+    u64 keep = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = threadIdx.x * 4 + e;
+      keep += r < n_k && (!use_p || run < bound) && q[e] &&
+              weight(logit_of(sm.list[r])) >= min_p;
+      run += q[e];
+    }
+    n = (int)block_sum(keep, sm);
+    const int N = pow2_at_least(n);
+    for (int t = threadIdx.x; t < N; t += kThreads)
+      sm.order[t] = t < n ? ((u64)index_of(sm.list[t]) << 32) | (sm.list[t] >> 32) : ~0ull;
     block_sort<false>(sm.order, N);
-    u64 q[4], total, mine = 0;
+    u64 mine = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = threadIdx.x * 4 + e;
       q[e] = r < n ? whole_of(weight(of_key((uint32_t)sm.order[r]))) : 0;
       mine += q[e];
     }
-    u64 run = block_scan(mine, total, sm);
+    run = block_scan(mine, total, sm);
     const u64 target = share_of(total, draw_part(u));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -355,31 +542,83 @@ struct Sampler {
     }
   }
 
-  static __device__ __forceinline__ uint32_t draw_part(float u) {
-    return (uint32_t)(fminf(fmaxf(u, 0.0f), 0.99999994f) * 16777216.0f);
+  // Keeps the list's entries in the bins (linear in the logit) up to the one
+  // where their weight reaches `bound`; returns their number. The list carries
+  // at least `bound`.
+  __device__ int shorten(int n, u64 bound, float low) const {
+    const int tid = threadIdx.x;
+    const float range = fminf(top - low, 3.0e38f);
+    const float scale = range > 0.0f ? (float)kGroupBins / range : 0.0f;
+    auto bin_of = [&](float x) { return min(kGroupBins - 1, (int)((top - x) * scale)); };
+    if (tid < kGroupBins) sm.mass[tid] = 0;
+    if (tid == 0) sm.found = kGroupBins - 1;
+    __syncthreads();
+    u64 c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = tid + e * kThreads;
+      c[e] = r < n ? sm.list[r] : 0;
+      if (r < n) atomicAdd(&sm.mass[bin_of(logit_of(c[e]))], whole(c[e]));
+    }
+    __syncthreads();
+    u64 all;
+    const u64 mine = tid < kGroupBins ? sm.mass[tid] : 0;
+    const u64 before = block_scan(mine, all, sm);
+    if (tid == 0) sm.count = 0;
+    if (before < bound && bound <= before + mine) sm.found = tid;
+    __syncthreads();
+    const int cut = sm.found;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c[e] && bin_of(logit_of(c[e])) <= cut) sm.list[atomicAdd(&sm.count, 1)] = c[e];
+    __syncthreads();
+    return sm.count;
   }
 
+  __device__ void draw_from_list(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+                                 long long* token) const {
+    if (n <= kRank)
+      draw_ranked(n, n_k, use_p, bound, part, u, token);
+    else
+      draw_sorted(n, n_k, use_p, bound, part, u, token);
+  }
+
+  // -------------------------------------------------------- whole-row draws
   // Draw among the tokens at or above the composite C with w >= min_p: sums of
-  // the warps' ranges, then of the range that holds the draw.
-  __device__ void draw_from_row(u64 C, float u, long long* token) const {
+  // the blocks' and warps' ranges, then of the range that holds the draw.
+  __device__ void draw_from_row(u64 C, float u, long long* token) {
     auto mass_of = [&](float x, int i) -> u64 {
       if (!(x > -INFINITY)) return 0;  // NaN too
       const float w = weight(x);
       return w >= min_p && (C == 0 || composite(x, i) >= C) ? whole_of(w) : 0;
     };
     u64 mine = 0;
-    each([&](float x, int i) { mine += mass_of(x, i); });
+    if (C == 0 && min_p <= 0.0f) {
+      mine = mass();
+    } else {
+      const float least = C == 0 ? -INFINITY : logit_of(C);
+      each([&](float x, int i) {
+        if (x >= least) mine += mass_of(x, i);
+      });
+    }
     mine = warp_sum(mine);
     __syncthreads();
     if (threadIdx.x % 32 == 0) sm.part[threadIdx.x / 32] = mine;
     __syncthreads();
+    u64 ours = 0;
+    for (int w = 0; w < kWarps; ++w) ours += sm.part[w];
+    const Pair* p = exchange(ours, 0);
     u64 total = 0, before = 0;
-    for (int w = 0; w < kWarps; ++w) total += sm.part[w];
+    for (int r = 0; r < n_blocks; ++r) {
+      if (r < (int)rank) before += p[r].a;
+      total += p[r].a;
+    }
     const u64 target = share_of(total, draw_part(u));
+    if (target < before || target >= before + ours) return;  // another block's
     int w = 0;
     while (w < kWarps - 1 && before + sm.part[w] <= target) before += sm.part[w++];
     // The range in contiguous pieces, one per thread.
-    const int begin = w * per_warp, end = min(row.n_vec, begin + per_warp);
+    const int begin = ((int)rank * kWarps + w) * per_warp, end = min(row.n_vec, begin + per_warp);
     const int piece = (per_warp + kThreads - 1) / kThreads;
     const int j0 = begin + threadIdx.x * piece, j1 = min(end, j0 + piece);
     mine = 0;
@@ -405,16 +644,16 @@ struct Sampler {
   }
 
   // Composite of the last token of the smallest leading run of the tokens at
-  // or above C that holds `need` tokens, or whole weight `need`; 0 if none does.
-  __device__ u64 bisect(u64 need, bool count, u64 C) const {
-    u64 lo = C, hi = composite(top, 0) | 0xffffffffull;  // run at lo: the answer or all
+  // or above C that holds `need` tokens, or whole weight `need`.
+  __device__ u64 bisect(u64 need, bool count, u64 C) {
+    u64 lo = C, hi = composite(top, 0) | 0xffffffffull;
     while (lo < hi) {
       const u64 mid = hi - (hi - lo) / 2;
       u64 s = 0;
       each([&](float x, int i) {
         if (x > -INFINITY && composite(x, i) >= mid) s += count ? 1ull : whole_of(weight(x));
       });
-      if (block_sum(s, sm) >= need)
+      if (cluster_sum(s) >= need)
         lo = mid;
       else
         hi = mid - 1;
@@ -422,31 +661,34 @@ struct Sampler {
     return lo;
   }
 
+  // Rank 0's `cut`, for every block.
+  __device__ __forceinline__ u64 shared_cut() const {
+    sync();
+    return n_blocks == 1 ? sm.cut : remote_load64(remote(&sm.cut, 0));
+  }
+
   // The cuts by histogram (see the head of the file): the composite at or
-  // above which a token is kept. k <= 0: no top-k; bound by top_p part of 2^24.
-  __device__ u64 cut_by_bins(int k, bool use_p, uint32_t part) const {
+  // above which a token is kept. k <= 0: no top-k; `total`: the row's weight
+  // where it is known (else 0); least: the row's smallest logit.
+  __device__ u64 cut_by_bins(int k, bool use_p, uint32_t part, u64 total, float least) {
     const int tid = threadIdx.x;
     // Bins are linear in the logit over the live range [low, top].
-    float low = INFINITY;
-    const float live = cutoff();
-    each([&](float x, int) {
-      if (x > -INFINITY && x >= live) low = fminf(low, x);
-    });
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
-    __syncthreads();
-    if (tid % 32 == 0) sm.fpart[tid / 32] = low;
-    for (int t = tid; t < kBins; t += kThreads) sm.bins[t] = 0;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) low = fminf(low, sm.fpart[w]);
+    const float low = fmaxf(least, cutoff());
     const float range = fminf(top - low, 3.0e38f);
     const float scale = range > 0.0f ? (float)kBins / range : 0.0f;
     auto bin_of = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };
-    each([&](float x, int) {
-      if (x >= low) atomicAdd(&sm.bins[bin_of(x)], 1u);
-    });
+    const int light = bin_of(top - 7.0f / inv_t);  // bins from here: by their centre
+    for (int t = tid; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
     __syncthreads();
-    // This thread's four bins, and the tokens and (roughly) the weight before.
+    each([&](float x, int) {
+      if (!(x >= low)) return;
+      const int b = bin_of(x);
+      atomicAdd(&sm.bins[b], 1u);
+      if (b < light && use_p) atomicAdd(&sm.heavy[b], __expf((x - top) * inv_t));
+    });
+    sync();
+    // This thread's four bins: tokens, and roughly their weight. The rough
+    // weights only choose which bins are looked at; exact sums decide.
     uint32_t c[4];
     float m[4];
     u64 n_mine = 0;
@@ -454,41 +696,48 @@ struct Sampler {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int b = tid * 4 + e;
-      c[e] = sm.bins[b];
-      m[e] = c[e] * expf(-((float)b + 0.5f) * (range / kBins) * inv_t);
+      float heavy = 0.0f;
+      c[e] = 0;
+      for (int r = 0; r < n_blocks; ++r) {
+        c[e] += n_blocks == 1 ? sm.bins[b] : remote_load(remote(&sm.bins[b], r));
+        heavy += n_blocks == 1 ? sm.heavy[b]
+                               : __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+      }
+      m[e] = b < light ? heavy
+                       : (float)c[e] * __expf(-((float)b + 0.5f) * (range / kBins) * inv_t);
       n_mine += c[e];
       m_mine += m[e];
     }
+    if (tid == 0) sm.count = 0;
+    sync();  // the bins have been read: lists may be written over them
     u64 n_all;
     u64 n_before = block_scan(n_mine, n_all, sm);
 
     u64 C = 0;
-    u64 mass_k = 0;  // exact weight of the top-k, once known
+    u64 mass_k = total;  // exact weight of the top-k, once known
     int last_bin = kBins - 1;
     if (k > 0 && (u64)k < n_all) {
-      if (tid == 0) sm.count = 0;
-      __syncthreads();  // the bins have been read; `found` may be written
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (n_before < (u64)k && (u64)k <= n_before + c[e]) {
           sm.found = tid * 4 + e;
-          sm.part[kWarps] = n_before;
+          sm.n_groups = (int)((u64)k - n_before);  // wanted of that bin
         }
         n_before += c[e];
       }
       __syncthreads();
-      const int cut = sm.found;
-      const int need = (int)((u64)k - sm.part[kWarps]);
+      last_bin = sm.found;
+      const int need = sm.n_groups;
       u64 above = 0;
       each([&](float x, int i) {
         if (!(x >= low)) return;
         const int b = bin_of(x);
-        if (b < cut && use_p) above += whole_of(weight(x));
-        if (b == cut) push(x, i);
+        if (b < last_bin && use_p) above += whole_of(weight(x));
+        if (b == last_bin) push(x, i);
       });
-      above = block_sum(above, sm);
-      const int n = sm.count;
-      last_bin = cut;
+      above = cluster_sum(above);
+      sync();
+      const int n = list_size();
       if (n > kCap) {
         C = bisect((u64)k, true, 0);
         if (use_p) {
@@ -496,22 +745,26 @@ struct Sampler {
           each([&](float x, int i) {
             if (x > -INFINITY && composite(x, i) >= C) s += whole_of(weight(x));
           });
-          mass_k = block_sum(s, sm);
+          mass_k = cluster_sum(s);
         }
       } else {
-        sort_list(n);
-        C = sm.list[need - 1];
-        u64 q[4], all;
-        list_scan(sm.list, need, q, all);
-        mass_k = above + all;
+        u64 within = 0;
+        if (rank == 0) {
+          sort_list(n);
+          if (tid == 0) sm.cut = sm.list[need - 1];
+          u64 q[4];
+          list_scan(need, q, within);
+        }
+        C = shared_cut();
+        if (use_p) mass_k = above + exchange(within, 0)[0].a;
       }
-    } else if (use_p) {
-      mass_k = row_mass();
+    } else if (use_p && total == 0) {
+      mass_k = cluster_sum(mass());
     }
     if (!use_p) return C;
 
     // The bin that the mass bound falls into, by the rough weights; it and its
-    // neighbours are collected and the exact sums decide.
+    // neighbours are collected, and the exact sums decide or correct the guess.
     const u64 bound = max(share_of(mass_k, part), (u64)1);
     float m_inc = m_mine;
 #pragma unroll
@@ -521,202 +774,302 @@ struct Sampler {
     }
     __syncthreads();
     if (tid % 32 == 31) sm.fpart[tid / 32] = m_inc;
-    if (tid == 0) sm.found = last_bin, sm.count = 0;
     __syncthreads();
-    float run = m_inc - m_mine;
-    for (int w = 0; w < (int)(tid / 32); ++w) run += sm.fpart[w];
-    const float want = (float)bound / kOne;
+    float rough = m_inc - m_mine;  // before this thread's bins
+    for (int w = 0; w < (int)(tid / 32); ++w) rough += sm.fpart[w];
+    float want = (float)bound / kOne;
+    for (int tries = 0; tries < 4; ++tries) {
+      sync();
+      if (tid == 0) sm.found = last_bin, sm.count = 0;
+      sync();
+      float run = rough;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      run += m[e];
-      if (run >= want) {
-        atomicMin(&sm.found, tid * 4 + e);
-        break;
+      for (int e = 0; e < 4; ++e) {
+        run += m[e];
+        if (run >= want) {
+          atomicMin(&sm.found, tid * 4 + e);
+          break;
+        }
+      }
+      __syncthreads();
+      const int b0 = max(0, sm.found - 1), b1 = min(last_bin, sm.found + 1);
+      u64 above = 0;
+      each([&](float x, int i) {
+        if (!(x >= low)) return;
+        const int b = bin_of(x);
+        if (b > b1 || (b == last_bin && C != 0 && composite(x, i) < C)) return;
+        if (b < b0)
+          above += whole_of(weight(x));
+        else
+          push(x, i);
+      });
+      above = cluster_sum(above);
+      sync();
+      const int n = list_size();
+      if (n > kCap) break;
+      u64 q[4], all = 0;
+      if (rank == 0) list_scan(n, q, all);
+      all = exchange(all, 0)[0].a;
+      if (above < bound && bound <= above + all) {
+        if (rank == 0) {
+          sort_list(n);
+          u64 before = above + list_scan(n, q, all);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (q[e] && before < bound && bound <= before + q[e])
+              sm.cut = sm.list[tid * 4 + e];
+            before += q[e];
+          }
+        }
+        return shared_cut();
+      }
+      // The rough sum at the start of bin b0 is off by what the exact one says.
+      run = rough;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (tid * 4 + e == b0) sm.fpart[0] = run;
+        run += m[e];
+      }
+      __syncthreads();
+      want = sm.fpart[0] + ((float)bound - (float)above) / kOne;
+    }
+    return bisect(bound, false, C);
+  }
+
+  // --------------------------------------------------------------- one row
+  __device__ void run(float T, int k, float top_p, float u, long long* token) {
+    const int tid = threadIdx.x, lane = tid % 32;
+    // Maxima of the thread's groups, and the row's extremes.
+    const int end = end_vec();
+    float gm[kGroups];
+    Extremes<kF32> all;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      Extremes<kF32> m;
+      int j = group_first(g);
+      const int stop = min(end, j + 32 * per_group);
+      for (; j + 224 < stop; j += 256) {
+        Vec<kF32> x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = row.get(j + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m.add(x[i], all);
+      }
+      for (; j < stop; j += 32) m.add(row.get(j), all);
+      gm[g] = m.max();
+    }
+    if (tid < kGroupBins) sm.gbins[tid] = 0;
+    if (tid == 0) sm.count = 0, sm.n_groups = 0, sm.found = 0x7fffffff;
+    float low, least;  // smallest group maximum, smallest logit
+    {
+      float hi = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3])), lo = INFINITY;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        if (gm[g] > -INFINITY) lo = fminf(lo, gm[g]);
+      float mn = all.min();
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+      }
+      if (lane == 0) {
+        sm.fpart[tid / 32] = hi;
+        sm.part[tid / 32] = ((u64)__float_as_uint(lo) << 32) | __float_as_uint(mn);
+      }
+      __syncthreads();
+      top = -INFINITY, low = INFINITY, least = INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        top = fmaxf(top, sm.fpart[w]);
+        low = fminf(low, __uint_as_float((uint32_t)(sm.part[w] >> 32)));
+        least = fminf(least, __uint_as_float((uint32_t)sm.part[w]));
       }
     }
-    __syncthreads();
-    const int b0 = max(0, sm.found - 1), b1 = min(last_bin, sm.found + 1);
-    u64 above = 0;
-    each([&](float x, int i) {
-      if (!(x >= low)) return;
-      const int b = bin_of(x);
-      if (b > b1 || (b == last_bin && C != 0 && composite(x, i) < C)) return;
-      if (b < b0)
-        above += whole_of(weight(x));
-      else
-        push(x, i);
-    });
-    above = block_sum(above, sm);
-    const int n = sm.count;
-    if (n > kCap || n == 0 || above >= bound) return bisect(bound, false, C);
-    sort_list(n);
-    u64 q[4], all;
-    u64 before = above + list_scan(sm.list, n, q, all);
-    if (above + all < bound) return bisect(bound, false, C);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (q[e] && before < bound && bound <= before + q[e])
-        sm.part[kWarps] = sm.list[tid * 4 + e];
-      before += q[e];
-    }
-    __syncthreads();
-    return sm.part[kWarps];
-  }
-};
-
-template <bool kF32>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
-  __shared__ Shared sm;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 32;
-  const float T = p.temperature ? p.temperature[b] : p.temperature_all;
-  const int k = p.top_k ? p.top_k[b] : p.top_k_all;
-  const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-  const float u = p.u[b];
-  Sampler<kF32> s(reinterpret_cast<const uint8_t*>(p.logits) + b * p.stride * (kF32 ? 4 : 2), p.V,
-                  sm);
-  s.min_p = fminf(p.min_p ? p.min_p[b] : p.min_p_all, 1.0f);  // the best token stays
-  s.inv_t = T > 0.0f ? 1.0f / fminf(T, 1.0e38f) : 1.0f;
-  constexpr int E = Vec<kF32>::E;
-
-  // Maxima of the row and of each thread's groups. fmaxf drops NaN.
-  const int v0 = s.first_vec(), v1 = s.end_vec();
-  const int steps = s.per_warp / 32;
-  auto group_first = [&](int g) { return v0 + 32 * (steps * g / kGroups); };
-  auto group_end = [&](int g) { return min(v1, v0 + 32 * (steps * (g + 1) / kGroups)); };
-  float gm[kGroups];
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    Maximum<kF32> m;
-    const int end = group_end(g);
-    int j = group_first(g);
-    for (; j + 224 < end; j += 256) {
-      Vec<kF32> x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = s.row.get(j + 32 * i);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m.add(x[i]);
-    }
-    for (; j < end; j += 32) m.add(s.row.get(j));
-    gm[g] = m.get();
-  }
-  if (tid < kGroupBins) sm.gbins[tid] = 0;
-  if (tid == 0) sm.count = 0, sm.found = 0x7fffffff;
-  {
-    float hi = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3])), lo = INFINITY;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (gm[g] > -INFINITY) lo = fminf(lo, gm[g]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    }
-    if (lane == 0) sm.fpart[tid / 32] = hi, sm.part[tid / 32] = __float_as_uint(lo);
-  }
-  __syncthreads();
-  float top = -INFINITY, low = INFINITY;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    top = fmaxf(top, sm.fpart[w]);
-    low = fminf(low, __uint_as_float((uint32_t)sm.part[w]));
-  }
-  s.top = top;
-  long long* token = p.tokens + b;
-  if (top == -INFINITY) {
-    if (tid == 0) *token = -1;
-    return;
-  }
-  if (!(T > 0.0f)) {
-    // Greedy: the lowest index that holds the maximum.
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (gm[g] == top)
-        for (int j = group_first(g); j < group_end(g); j += 32) {
-          const Vec<kF32> x = s.row.get(j);
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (x.at(e) == top) atomicMin(&sm.found, j * E - s.row.mis + e);
-        }
-    __syncthreads();
-    if (tid == 0) *token = sm.found;
-    return;
-  }
-  const bool use_k = k > 0 && k < p.V, use_p = top_p < 1.0f;
-  const uint32_t part = (uint32_t)(fmaxf(top_p, 0.0f) * 16777216.0f);
-  if (!use_k && !use_p) {
-    s.draw_from_row(0, u, token);
-    return;
-  }
-  if (!use_k || k <= kSmallK) {
-    // Bins over the group maxima; a group's bin also decides which of its
-    // logits are candidates, so the candidates are a leading run up to ties.
-    const float range = fminf(top - low, fminf(kLive / s.inv_t, 3.0e38f));
-    const float scale = range > 0.0f ? (float)kGroupBins / range : 0.0f;
-    const float cutoff = s.cutoff();
-    auto bin_of = [&](float x) { return min(kGroupBins - 1, (int)((top - x) * scale)); };
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (gm[g] > -INFINITY && gm[g] >= cutoff) atomicAdd(&sm.gbins[bin_of(gm[g])], 1u);
-    __syncthreads();
-    // The first bin up to which the groups suffice (all of them if none does).
-    const u64 want = use_k ? (u64)k : (u64)kNucleus;
-    u64 all, mine = tid < kGroupBins ? sm.gbins[tid] : 0;
-    const u64 before = block_scan(mine, all, sm);
-    if (tid == 0) sm.found = kGroupBins - 1;
-    __syncthreads();
-    if (tid < kGroupBins && before < want && want <= before + mine) sm.found = tid;
-    __syncthreads();
-    const int cut = sm.found;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (gm[g] > -INFINITY && gm[g] >= cutoff && bin_of(gm[g]) <= cut)
-        for (int j = group_first(g); j < group_end(g); j += 32) {
-          const Vec<kF32> x = s.row.get(j);
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (x.at(e) > -INFINITY && x.at(e) >= cutoff && bin_of(x.at(e)) <= cut)
-              s.push(x.at(e), j * E - s.row.mis + e);
-        }
-    __syncthreads();
-    const int n = sm.count;
-    if (n <= kCap) {
-      u64 bound = ~0ull, q[4], total;
-      bool enough = true;
-      if (!use_k) {
-        bound = max(share_of(s.row_mass(), part), (u64)1);
-        s.list_scan(sm.list, n, q, total);
-        enough = total >= bound;
+    if (n_blocks > 1) {
+      const Pair* p = exchange(__float_as_uint(top),
+                               ((u64)__float_as_uint(low) << 32) | __float_as_uint(least));
+      for (int r = 0; r < n_blocks; ++r) {
+        top = fmaxf(top, __uint_as_float((uint32_t)p[r].a));
+        low = fminf(low, __uint_as_float((uint32_t)(p[r].b >> 32)));
+        least = fminf(least, __uint_as_float((uint32_t)p[r].b));
       }
-      if (enough) {
-        s.sort_list(n);
-        const int n_k = use_k ? min(n, k) : n;
-        u64 run = s.list_scan(sm.list, n_k, q, total);
-        if (use_k && use_p) bound = max(share_of(total, part), (u64)1);
-        u64 keep = 0;
+    }
+    if (top == -INFINITY) {
+      if (rank == 0 && tid == 0) *token = -1;
+      return;
+    }
+    if (!(T > 0.0f)) {
+      // Greedy: the lowest index that holds the maximum.
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        if (gm[g] == top)
+          each_in(group_first(g), min(end, group_first(g) + 32 * per_group), [&](float x, int i) {
+            if (x == top) atomicMin(&sm.found, i);
+          });
+      __syncthreads();
+      int best = sm.found;
+      if (n_blocks > 1) {
+        const Pair* p = exchange((u64)best, 0);
+        for (int r = 0; r < n_blocks; ++r) best = min(best, (int)p[r].a);
+      }
+      if (rank == 0 && tid == 0) *token = best;
+      return;
+    }
+    const bool use_k = k > 0 && k < row.V, use_p = top_p < 1.0f;
+    const uint32_t part = (uint32_t)(fmaxf(top_p, 0.0f) * 16777216.0f);
+    const bool by_weight = !use_k && !use_p;
+    if (by_weight && min_p <= 0.0f) {
+      draw_from_row(0, u, token);
+      return;
+    }
+    u64 total = 0;
+    if (!use_k || k <= kSmallK) {
+      // Which logits are candidates goes by bins over the group maxima, so that
+      // they are a leading run up to ties; with min-p alone by the weight.
+      const float live = cutoff();
+      const float range = fminf(top - low, fminf(kLive / inv_t, 3.0e38f));
+      const float scale = range > 0.0f ? (float)kGroupBins / range : 0.0f;
+      auto bin_of = [&](float x) { return min(kGroupBins - 1, (int)((top - x) * scale)); };
+      int cut = 0;
+      if (!by_weight) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          if (gm[g] > -INFINITY && gm[g] >= live) atomicAdd(&sm.gbins[bin_of(gm[g])], 1u);
+        sync();
+        const uint32_t* counts = sm.gbins;
+        if (n_blocks > 1) {
+          if (tid < kGroupBins) {
+            uint32_t c = 0;
+            for (int r = 0; r < n_blocks; ++r) c += remote_load(remote(&sm.gbins[tid], r));
+            sm.gsum[tid] = c;
+          }
+          __syncthreads();
+          counts = sm.gsum;
+        }
+        // The first bin up to which the groups suffice (the last if none does);
+        // every warp finds it for itself.
+        const uint32_t want = use_k ? (uint32_t)k : (uint32_t)kNucleus;
+        uint32_t c[kGroupBins / 32], mine = 0;
+#pragma unroll
+        for (int e = 0; e < kGroupBins / 32; ++e) mine += c[e] = counts[lane * (kGroupBins / 32) + e];
+        uint32_t inc = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
+          if (lane >= off) inc += y;
+        }
+        uint32_t run = inc - mine;
+        int at = kGroupBins - 1;
+#pragma unroll
+        for (int e = kGroupBins / 32 - 1; e >= 0; --e) {
+          uint32_t upto = run;
+#pragma unroll
+          for (int f = 0; f <= e; ++f) upto += c[f];
+          if (upto >= want) at = lane * (kGroupBins / 32) + e;
+        }
+        cut = __reduce_min_sync(0xffffffffu, at);
+      }
+      auto candidate = [&](float x) {
+        return x > -INFINITY && x >= live && (by_weight ? weight(x) >= min_p : bin_of(x) <= cut);
+      };
+      // The groups to read again, then their vectors shared among all threads.
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        if (candidate(gm[g])) sm.groups[atomicAdd(&sm.n_groups, 1)] = group_first(g);
+      __syncthreads();
+      const int items = sm.n_groups * per_group;
+      u64 listed = 0;
+      for (int it0 = tid; it0 < items; it0 += 4 * kThreads) {
+        Vec<kF32> x[4];
+        int at[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = tid * 4 + e;
-          keep += r < n_k && run < bound && q[e] &&
-                  s.weight(of_key((uint32_t)(sm.list[r] >> 32))) >= s.min_p;
-          run += q[e];
+          // Step s of a group, unless past the end of the group's warp range.
+          const int it = it0 + e * kThreads;
+          at[e] = -1;
+          if (it < items) {
+            const int f = sm.groups[it / per_group], j = f + it % per_group * 32;
+            if (j < min(row.n_vec, (f / per_warp + 1) * per_warp)) at[e] = j;
+          }
+          if (at[e] >= 0) x[e] = row.get(at[e]);
         }
-        s.draw_from_list((int)block_sum(keep, sm), u, token);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at[e] >= 0) {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+              if (candidate(x[e].at(i))) {
+                push(x[e].at(i), at[e] * E - row.mis + i);
+                listed += whole_of(weight(x[e].at(i)));
+              }
+          }
+      }
+      if (!use_k && use_p) {
+        const Pair s = cluster_sum(mass(), listed);
+        total = s.a;
+        listed = s.b;
+      }
+      sync();
+      const int n = list_size();
+      const u64 bound = !use_k && use_p ? max(share_of(total, part), (u64)1) : 0;
+      if (n <= kCap && (use_k || !use_p || listed >= bound)) {
+        if (rank == 0) {
+          const int m = bound && n > kRank ? shorten(n, bound, low) : n;
+          draw_from_list(m, use_k ? min(n, k) : m, use_p, bound, part, u, token);
+        }
         return;
       }
     }
-    __syncthreads();
+    draw_from_row(cut_by_bins(use_k ? k : 0, use_p, part, total, least), u, token);
   }
-  s.draw_from_row(s.cut_by_bins(use_k ? k : 0, use_p, part), u, token);
+
+};
+
+template <bool kF32>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p, int n_blocks) {
+  __shared__ Shared sm;
+  const int b = blockIdx.x / n_blocks;
+  Sampler<kF32> s(reinterpret_cast<const uint8_t*>(p.logits) + b * p.stride * (kF32 ? 4 : 2), p.V,
+                  sm, n_blocks, n_blocks > 1 ? cluster_rank() : 0);
+  const float T = p.temperature ? p.temperature[b] : p.temperature_all;
+  s.inv_t = T > 0.0f ? 1.0f / fminf(T, 1.0e38f) : 1.0f;
+  s.min_p = fminf(p.min_p ? p.min_p[b] : p.min_p_all, 1.0f);  // the best token stays
+  s.run(T, p.top_k ? p.top_k[b] : p.top_k_all, p.top_p ? p.top_p[b] : p.top_p_all, p.u[b],
+        p.tokens + b);
+  if (n_blocks > 1) s.sync();  // no block's shared memory goes while another reads it
+}
+
+// Blocks per row: as many as keep two a SM, a power of two up to 8, with at least
+// one vector for each thread.
+int choose_cluster(int B, int V, bool fp32, int n_sms) {
+  const int per_block = kThreads * (fp32 ? 4 : 8);
+  int c = 1;
+  while (c < kMaxCluster && (long long)B * c * 2 <= 2 * n_sms && (long long)c * per_block < V)
+    c *= 2;
+  return c;
+}
+
+template <bool kF32>
+cudaError_t launch(const SampleParams& p, cudaStream_t stream) {
+  const int c = choose_cluster(p.B, p.V, kF32, p.n_sms);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)p.B * c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)c, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = c > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<kF32>, p, c);
 }
 
 }  // namespace smp
 
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t stream) {
-  if (p.fp32)
-    smp::sample_kernel<true><<<p.B, smp::kThreads, 0, stream>>>(p);
-  else
-    smp::sample_kernel<false><<<p.B, smp::kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return p.fp32 ? smp::launch<true>(p, stream) : smp::launch<false>(p, stream);
 }
 
 }  // namespace enl
