@@ -31,6 +31,7 @@
 // output. fp32: each factor is split into two tf32 parts (values into three) and
 // the three (four) largest products are added, about 2^-21 of each.
 #include <algorithm>
+#include <atomic>
 
 #include "enl_common.cuh"
 #include "enl_kernels.h"
@@ -775,9 +776,16 @@ cudaError_t launch(const PagedDecodeParams& p, cudaStream_t stream) {
   const long long tiles = (long long)p.B * p.Hkv * ((G + C::NT * 8 - 1) / (C::NT * 8)) *
                           ((most + C::kKeys - 1) / C::kKeys);
   const int grid = (int)std::min<long long>(tiles, (long long)p.n_sms * C::kPerSm);
-  cudaError_t e = cudaFuncSetAttribute(paged_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       C::kSmem);
+  static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(paged_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
   paged_kernel<C><<<grid, C::kThreads, C::kSmem, stream>>>(p);
   return cudaGetLastError();
 }

@@ -719,76 +719,97 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
 
 
 # ------------------------------------------------- serving over paged caches
-def _same_device(q: torch.Tensor, *named) -> None:
-    """Every given tensor (None skipped) sits on q's device, which is the
-    current one: launches go to its current stream."""
-    dev = q.device
-    for name, t in named:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not {dev}")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {dev}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+# A decode step makes several of these calls per layer, each a few microseconds
+# of GPU time, so their host side is kept short: one test per operand (the
+# message is built only on failure), one struct built from positional values.
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index
+_current_device = torch._C._cuda_getDevice
 
 
-def _require_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> None:
-    """t is a contiguous (n,) CUDA tensor of the dtype."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (n,) or not t.is_cuda \
-            or not t.is_contiguous():
-        got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ValueError(f"{name} must be a contiguous {dtype} ({n},) CUDA tensor, got {got}")
+def _describe(t) -> str:
+    if not isinstance(t, torch.Tensor):
+        return type(t).__name__
+    return f"{t.dtype} {tuple(t.shape)} on {t.device}"
 
 
-def _heads4(name: str, t: torch.Tensor, shape, dtypes=_DTYPES) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or \
-            t.shape != shape or t.stride(-1) != 1:
-        got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ValueError(f"{name} must be a bf16/fp32 CUDA tensor of shape {tuple(shape)} with a "
-                         f"contiguous last (head) dimension, got {got}")
+def _device_of(name: str, t, dims: str) -> int:
+    """Index of the CUDA device that t, the call's first operand, is on; it
+    must be the current one, on whose stream the call is launched."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims.count(",") + 1 or \
+            t.dtype not in _DTYPES or not t.is_cuda:
+        raise ValueError(f"{name} must be a bf16/fp32 ({dims}) CUDA tensor, got {_describe(t)}")
+    dev = t.get_device()
+    if dev != _current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return dev
 
 
-def _norm_rope_operands(D: int, q_weight, k_weight, rope):
-    """(weight pointers, table pointers, table rows) after their checks."""
+def _require_vector(name: str, t, n: int, dtype: torch.dtype, dev: int) -> int:
+    """The address of a contiguous (n,) tensor of the dtype on device dev."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev or \
+            t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous {dtype} ({n},) tensor on cuda:{dev}, got "
+                         f"{_describe(t)}")
+    return t.data_ptr()
+
+
+def _require_heads(name: str, t, shape, dtype, dev: int):
+    """The strides of a head view of the shape, dtype (None: bf16 or fp32) and
+    device."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.get_device() != dev or \
+            (t.dtype not in _DTYPES if dtype is None else t.dtype is not dtype):
+        raise ValueError(f"{name} must be a {dtype or 'bf16/fp32'} {tuple(shape)} tensor on "
+                         f"cuda:{dev}, got {_describe(t)}")
+    st = t.stride()
+    if st[-1] != 1:
+        raise ValueError(f"{name} must have a contiguous last (head) dimension")
+    return st[:-1]
+
+
+def _norm_rope_operands(D: int, q_weight, k_weight, rope, dev: int):
+    """(weight addresses, table addresses, table rows) after their checks."""
     if (q_weight is None) != (k_weight is None):
         raise ValueError("q_weight and k_weight come in pairs")
     wq = wk = cos = sin = None
     rows = 0
     if q_weight is not None:
-        _require_vector("q_weight", q_weight, D, torch.float32)
-        _require_vector("k_weight", k_weight, D, torch.float32)
-        wq, wk = q_weight.data_ptr(), k_weight.data_ptr()
+        wq = _require_vector("q_weight", q_weight, D, torch.float32, dev)
+        wk = _require_vector("k_weight", k_weight, D, torch.float32, dev)
     if rope is not None:
         cos_t, sin_t = rope
         for name, t in (("cos", cos_t), ("sin", sin_t)):
-            _require_cuda(name, t, torch.float32)
-            if t.dim() != 2 or t.shape[1] * 2 != D or not t.is_contiguous():
-                raise ValueError(f"rope {name} must be a contiguous fp32 (rows, {D // 2}) table, "
-                                 f"got {tuple(t.shape)}")
-        if cos_t.shape != sin_t.shape:
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or \
+                    t.get_device() != dev or t.dim() != 2 or t.shape[1] * 2 != D or \
+                    not t.is_contiguous():
+                raise ValueError(f"rope {name} must be a contiguous fp32 (rows, {D // 2}) table on "
+                                 f"cuda:{dev}, got {_describe(t)}")
+        rows = cos_t.shape[0]
+        if sin_t.shape[0] != rows:
             raise ValueError("rope tables must have one shape")
-        cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
+        cos, sin = cos_t.data_ptr(), sin_t.data_ptr()
     return wq, wk, cos, sin, rows
 
 
-def _page_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, B: int,
-               Hkv: int, D: int, dtype: torch.dtype) -> None:
-    """Checks of a paged cache's pools and block table."""
+def _require_pool(k_pages, v_pages, block_table, B: int, Hkv, D: int, dtype: torch.dtype,
+                  dev: int):
+    """(shape, strides) of a paged cache's pools after their checks."""
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.dim() != 4 \
-                or t.stride(-1) != 1:
-            got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
-            raise ValueError(f"{name} must be a {dtype} (num_pages, {Hkv}, page_size, {D}) CUDA "
-                             f"tensor with a contiguous head dimension, got {got}")
-    _, h, _, d = k_pages.shape
-    if h != Hkv or d != D or k_pages.shape != v_pages.shape or \
-            k_pages.stride() != v_pages.stride():
-        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must "
-                         f"share shape (num_pages, {Hkv}, page_size, {D}) and strides")
-    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or \
-            not block_table.is_cuda or block_table.dim() != 2 or block_table.shape[0] != B or \
-            block_table.stride(1) != 1:
-        raise ValueError(f"block_table must be an int32 ({B}, max_pages) CUDA tensor with "
-                         "contiguous rows")
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev or \
+                t.dim() != 4:
+            raise ValueError(f"{name} must be a {dtype} (num_pages, kv_heads, page_size, {D}) "
+                             f"tensor on cuda:{dev}, got {_describe(t)}")
+    shape, st = k_pages.shape, k_pages.stride()
+    if shape[3] != D or (Hkv is not None and shape[1] != Hkv) or v_pages.shape != shape or \
+            v_pages.stride() != st or st[3] != 1:
+        raise ValueError(f"k_pages {tuple(shape)} and v_pages {tuple(v_pages.shape)} must share "
+                         f"shape (num_pages, {Hkv or 'kv_heads'}, page_size, {D}) and strides, "
+                         "with a contiguous head dimension")
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype is not torch.int32 or \
+            block_table.get_device() != dev or block_table.dim() != 2 or \
+            block_table.shape[0] != B or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be an int32 ({B}, max_pages) tensor with contiguous "
+                         f"rows on cuda:{dev}, got {_describe(block_table)}")
+    return shape, st
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
@@ -806,33 +827,32 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     (B,), None = 0). out=(q_out, k_out) writes into given views, which may be q
     and k themselves. Returns (q_out, k_out), in out_dtype (default: q's).
     """
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or not isinstance(k, torch.Tensor) or \
-            k.dim() != 4:
-        raise ValueError("q and k must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
-    B, S, H, D = q.shape
-    Hkv = k.shape[2]
+    dev = _device_of("q", q, "batch, seq, heads, head_dim")
+    B, S, H, D = qshape = q.shape
     dt = q.dtype
-    _heads4("q", q, (B, S, H, D))
-    _heads4("k", k, (B, S, Hkv, D), (dt,))
-    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError(f"k must be a (batch, seq, kv_heads, head_dim) tensor, got {_describe(k)}")
+    Hkv = k.shape[2]
+    kshape = (B, S, Hkv, D)
+    qs = _require_heads("q", q, qshape, dt, dev)
+    ks = _require_heads("k", k, kshape, dt, dev)
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     if out is None:
         out_dtype = out_dtype or dt
-        q_out = torch.empty((B, S, H, D), dtype=out_dtype, device=q.device)
-        k_out = torch.empty((B, S, Hkv, D), dtype=out_dtype, device=q.device)
+        q_out = q.new_empty(qshape, dtype=out_dtype)
+        k_out = q.new_empty(kshape, dtype=out_dtype)
     else:
         q_out, k_out = out
-    _heads4("q_out", q_out, (B, S, H, D))
-    _heads4("k_out", k_out, (B, S, Hkv, D), (q_out.dtype,))
-    if start is not None:
-        _require_vector("start", start, B, torch.int32)
-    _same_device(q, ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("start", start),
-                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]),
-                 ("q_out", q_out), ("k_out", k_out))
+    qos = _require_heads("q_out", q_out, qshape, None, dev)
+    kos = _require_heads("k_out", k_out, kshape, q_out.dtype, dev)
     a = nat.QkNormRopeArgs(
         q.data_ptr(), k.data_ptr(), None, q_out.data_ptr(), k_out.data_ptr(), B, S, H, Hkv, D,
-        *q.stride()[:3], *k.stride()[:3], 0, 0, 0, *q_out.stride()[:3], *k_out.stride()[:3],
-        _DTYPES[dt], _DTYPES[q_out.dtype], wq, wk, eps, cos, sin, rows, pos0, _ptr(start))
-    nat.check(nat.load().enl_qk_norm_rope(ctypes.byref(a), _stream()), "enl_qk_norm_rope")
+        *qs, *ks, 0, 0, 0, *qos, *kos, _DTYPES[dt], _DTYPES[q_out.dtype], wq, wk, float(eps),
+        cos, sin, rows, int(pos0),
+        None if start is None else _require_vector("start", start, B, torch.int32, dev))
+    status = nat.load().enl_qk_norm_rope(ctypes.byref(a), _raw_stream(dev))
+    if status:
+        nat.check(status, "enl_qk_norm_rope")
     return q_out, k_out
 
 
@@ -854,37 +874,32 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     per row; the others cache nothing and their queries come out zero. Weights and
     rope may be None (no norm / no rotation). Returns the queries (B, S, H, D).
     """
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or not isinstance(k, torch.Tensor) or \
-            k.dim() != 4:
-        raise ValueError("q and k must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
-    B, S, H, D = q.shape
-    Hkv = k.shape[2]
+    dev = _device_of("q", q, "batch, seq, heads, head_dim")
+    B, S, H, D = qshape = q.shape
     dt = q.dtype
-    _heads4("q", q, (B, S, H, D))
-    _heads4("k", k, (B, S, Hkv, D), (dt,))
-    _heads4("v", v, (B, S, Hkv, D), (dt,))
-    _page_pool(k_pages, v_pages, block_table, B, Hkv, D, dt)
-    _require_vector("start", start, B, torch.int32)
-    if n_new is not None:
-        _require_vector("n_new", n_new, B, torch.int32)
-    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError(f"k must be a (batch, seq, kv_heads, head_dim) tensor, got {_describe(k)}")
+    Hkv = k.shape[2]
+    kshape = (B, S, Hkv, D)
+    qs = _require_heads("q", q, qshape, dt, dev)
+    ks = _require_heads("k", k, kshape, dt, dev)
+    vs = _require_heads("v", v, kshape, dt, dev)
+    pool, ps = _require_pool(k_pages, v_pages, block_table, B, Hkv, D, dt, dev)
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     if out is None:
-        out = torch.empty((B, S, H, D), dtype=dt, device=q.device)
-    _heads4("out", out, (B, S, H, D), (dt,))
-    _same_device(q, ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages),
-                 ("block_table", block_table), ("start", start), ("n_new", n_new),
-                 ("q_weight", q_weight), ("k_weight", k_weight),
-                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]), ("out", out))
-    if B * S == 0:
-        return out
+        out = q.new_empty(qshape)
+    os_ = _require_heads("out", out, qshape, dt, dev)
+    code = _DTYPES[dt]
     a = nat.QkNormRopeArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, B, S, H, Hkv, D,
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], 0, 0, 0,
-        _DTYPES[dt], _DTYPES[dt], wq, wk, eps, cos, sin, rows, 0, start.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0],
-        k_pages.shape[2], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        _ptr(n_new))
-    nat.check(nat.load().enl_qk_norm_rope(ctypes.byref(a), _stream()), "enl_qk_norm_rope")
+        *qs, *ks, *vs, *os_, 0, 0, 0, code, code, wq, wk, float(eps), cos, sin, rows, 0,
+        _require_vector("start", start, B, torch.int32, dev),
+        k_pages.data_ptr(), v_pages.data_ptr(), ps[0], ps[1], ps[2], pool[0], pool[2],
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        None if n_new is None else _require_vector("n_new", n_new, B, torch.int32, dev))
+    status = nat.load().enl_qk_norm_rope(ctypes.byref(a), _raw_stream(dev))
+    if status:
+        nat.check(status, "enl_qk_norm_rope")
     return out
 
 
@@ -902,75 +917,68 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: Optiona
     out=(dq, dk); the weight gradients fp32 (D,), summed over every token and
     head in a fixed order, None without weights.
     """
-    if not isinstance(dq_out, torch.Tensor) or dq_out.dim() != 4 or \
-            not isinstance(dk_out, torch.Tensor) or dk_out.dim() != 4:
-        raise ValueError("dq_out and dk_out must be 4-D CUDA tensors (batch, seq, heads, head_dim)")
-    B, S, H, D = dq_out.shape
-    Hkv = dk_out.shape[2]
+    dev = _device_of("dq_out", dq_out, "batch, seq, heads, head_dim")
+    B, S, H, D = qshape = dq_out.shape
     gdt = dq_out.dtype
-    _heads4("dq_out", dq_out, (B, S, H, D))
-    _heads4("dk_out", dk_out, (B, S, Hkv, D), (gdt,))
-    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope)
+    if not isinstance(dk_out, torch.Tensor) or dk_out.dim() != 4:
+        raise ValueError("dk_out must be a (batch, seq, kv_heads, head_dim) tensor, got "
+                         f"{_describe(dk_out)}")
+    Hkv = dk_out.shape[2]
+    kshape = (B, S, Hkv, D)
+    gqs = _require_heads("dq_out", dq_out, qshape, gdt, dev)
+    gks = _require_heads("dk_out", dk_out, kshape, gdt, dev)
+    wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     norm = wq is not None
-    in_dt = gdt
+    in_dt = q.dtype if isinstance(q, torch.Tensor) else gdt
+    qs = ks = (0, 0, 0)
     if norm:
-        _heads4("q", q, (B, S, H, D))
-        in_dt = q.dtype
-        _heads4("k", k, (B, S, Hkv, D), (in_dt,))
-    elif q is not None:
-        in_dt = q.dtype
-    dev = dq_out.device
+        qs = _require_heads("q", q, qshape, None, dev)
+        ks = _require_heads("k", k, kshape, in_dt, dev)
     if out is None:
         out_dtype = out_dtype or in_dt
-        dq = torch.empty((B, S, H, D), dtype=out_dtype, device=dev)
-        dk = torch.empty((B, S, Hkv, D), dtype=out_dtype, device=dev)
+        dq = dq_out.new_empty(qshape, dtype=out_dtype)
+        dk = dq_out.new_empty(kshape, dtype=out_dtype)
     else:
         dq, dk = out
-    _heads4("dq", dq, (B, S, H, D))
-    _heads4("dk", dk, (B, S, Hkv, D), (dq.dtype,))
-    if start is not None:
-        _require_vector("start", start, B, torch.int32)
-    x_q, x_k = (q, k) if norm else (None, None)
-    _same_device(dq_out, ("dk_out", dk_out), ("q", x_q), ("k", x_k), ("q_weight", q_weight),
-                 ("k_weight", k_weight), ("start", start), ("dq", dq), ("dk", dk),
-                 ("rope cos", rope and rope[0]), ("rope sin", rope and rope[1]))
+    dqs = _require_heads("dq", dq, qshape, None, dev)
+    dks = _require_heads("dk", dk, kshape, dq.dtype, dev)
     dwq = dwk = None
     if norm:
-        dwq = torch.empty((D,), dtype=torch.float32, device=dev)
-        dwk = torch.empty((D,), dtype=torch.float32, device=dev)
+        dwq = dq_out.new_empty((D,), dtype=torch.float32)
+        dwk = torch.empty_like(dwq)
     if B * S == 0:
         if norm:
             dwq.zero_()
             dwk.zero_()
         return dq, dk, dwq, dwk
-    none3 = (0, 0, 0)
     a = nat.QkNormRopeBackwardArgs(
-        dq_out.data_ptr(), dk_out.data_ptr(), _ptr(x_q), _ptr(x_k), dq.data_ptr(), dk.data_ptr(),
-        _ptr(dwq), _ptr(dwk), B, S, H, Hkv, D, *dq_out.stride()[:3], *dk_out.stride()[:3],
-        *(q.stride()[:3] if norm else none3), *(k.stride()[:3] if norm else none3),
-        *dq.stride()[:3], *dk.stride()[:3], _DTYPES[in_dt], _DTYPES[gdt], _DTYPES[dq.dtype],
-        wq, wk, eps, cos, sin, rows, pos0, _ptr(start))
+        dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr() if norm else None,
+        k.data_ptr() if norm else None, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk),
+        B, S, H, Hkv, D, *gqs, *gks, *qs, *ks, *dqs, *dks,
+        _DTYPES[in_dt], _DTYPES[gdt], _DTYPES[dq.dtype], wq, wk, float(eps), cos, sin, rows,
+        int(pos0), None if start is None else _require_vector("start", start, B, torch.int32, dev))
     lib = nat.load()
-    need = lib.enl_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
-    if need:
-        ws = _workspace(dev, need)
+    if norm:
+        need = lib.enl_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
+        ws = dq_out.new_empty((need,), dtype=torch.uint8)  # stream-ordered, freed after the launch
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    nat.check(lib.enl_qk_norm_rope_backward(ctypes.byref(a), _stream()),
-              "enl_qk_norm_rope_backward")
+    status = lib.enl_qk_norm_rope_backward(ctypes.byref(a), _raw_stream(dev))
+    if status:
+        nat.check(status, "enl_qk_norm_rope_backward")
     return dq, dk, dwq, dwk
 
 
 _zeroed: dict = {}
 
 
-def _zeroed_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+def _zeroed_workspace(dev: int, nbytes: int) -> torch.Tensor:
     """Scratch of attention_decode_paged, one per (device, stream) like
     _workspace, zeroed when it is made: its kernels leave the counters in it at
     zero for the next call."""
-    key = (device.index, _stream())
+    key = (dev, _raw_stream(dev))
     ws = _zeroed.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
         _zeroed[key] = ws
     return ws
 
@@ -1003,58 +1011,54 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     CUDA graph that replays beside other calls needs its own).
     Returns out (B, H, D) in out_dtype (default: q's) [and lse (B, H) fp32].
     """
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES or \
-            not q.is_cuda or q.stride(2) != 1:
-        raise ValueError("q must be a bf16/fp32 (batch, heads, head_dim) CUDA tensor with a "
-                         "contiguous head dimension")
-    B, H, D = q.shape
-    dt, dev = q.dtype, q.device
-    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
-        raise ValueError("k_pages must be a 4-D CUDA tensor (num_pages, kv_heads, page_size, "
-                         "head_dim)")
-    Hkv = k_pages.shape[1]
-    _page_pool(k_pages, v_pages, block_table, B, Hkv, D, dt)
-    _require_vector("seq_lens", seq_lens, B, torch.int32)
-    if window is not None and window < 0:
+    dev = _device_of("q", q, "batch, heads, head_dim")
+    B, H, D = shape = q.shape
+    dt = q.dtype
+    qs = _require_heads("q", q, shape, dt, dev)
+    pool, ps = _require_pool(k_pages, v_pages, block_table, B, None, D, dt, dev)
+    lens = _require_vector("seq_lens", seq_lens, B, torch.int32, dev)
+    if window is None:
+        window = -1
+    elif window < 0:
         raise ValueError(f"window must be >= 0 or None, got {window}")
-    if sinks < 0 or (sinks > 0 and window is None):
+    if sinks and (sinks < 0 or window < 0):
         raise ValueError(f"sinks={sinks} must be >= 0, and needs a window")
+    slopes = None
     if alibi_slopes is not None:
-        _require_vector("alibi_slopes", alibi_slopes, H, torch.float32)
+        slopes = _require_vector("alibi_slopes", alibi_slopes, H, torch.float32, dev)
     if out is None:
-        out = torch.empty((B, H, D), device=dev, dtype=out_dtype or dt)
-    elif out.dim() != 3 or out.shape != q.shape or out.dtype not in _DTYPES or \
-            out.stride(2) != 1:
-        raise ValueError(f"out must be ({B}, {H}, {D}) bf16/fp32 with a contiguous head dimension")
-    lse = torch.empty((B, H), device=dev, dtype=torch.float32) if return_lse else None
-    _same_device(q, ("k_pages", k_pages), ("v_pages", v_pages), ("block_table", block_table),
-                 ("seq_lens", seq_lens), ("alibi_slopes", alibi_slopes), ("out", out),
-                 ("workspace", workspace))
+        out = torch.empty_like(q) if out_dtype is None or out_dtype is dt else \
+            q.new_empty(shape, dtype=out_dtype)
+    os_ = _require_heads("out", out, shape, None, dev)
+    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     if B > 0:
         a = nat.PagedDecodeArgs(
-            q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
-            *k_pages.stride()[:3], k_pages.shape[0], k_pages.shape[2], block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), out.data_ptr(),
-            out.stride(0), out.stride(1), _ptr(lse), B, H, Hkv, D,
-            -1 if window is None else window, sinks, _ptr(alibi_slopes),
-            1.0 / math.sqrt(D) if scale is None else scale, _DTYPES[dt], _DTYPES[out.dtype])
+            q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(), v_pages.data_ptr(), ps[0], ps[1],
+            ps[2], pool[0], pool[2], block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], lens, out.data_ptr(), os_[0], os_[1],
+            None if lse is None else lse.data_ptr(), B, H, pool[1], D, int(window), int(sinks),
+            slopes, 1.0 / math.sqrt(D) if scale is None else float(scale), _DTYPES[dt],
+            _DTYPES[out.dtype])
         lib = nat.load()
         if workspace is None:
             workspace = _zeroed_workspace(
                 dev, lib.enl_paged_decode_workspace_bytes(ctypes.byref(a)))
-        a.workspace = workspace.data_ptr()
-        a.workspace_bytes = workspace.numel() * workspace.element_size()
-        nat.check(lib.enl_attn_decode_paged(ctypes.byref(a), _stream()), "enl_attn_decode_paged")
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}, got "
+                             f"{_describe(workspace)}")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
+        status = lib.enl_attn_decode_paged(ctypes.byref(a), _raw_stream(dev))
+        if status:
+            nat.check(status, "enl_attn_decode_paged")
     return (out, lse) if return_lse else out
 
 
-def _per_row(name: str, value, B: int, dtype: torch.dtype, off):
-    """(device pointer or None, scalar) of a setting given per row or for all."""
+def _per_row(name: str, value, B: int, dtype: torch.dtype, off, dev: int):
+    """(address or None, scalar) of a setting given per row or for all."""
     if value is None:
         return None, off
     if isinstance(value, torch.Tensor):
-        _require_vector(name, value, B, dtype)
-        return value.data_ptr(), off
+        return _require_vector(name, value, B, dtype, dev), off
     return None, value
 
 
@@ -1074,30 +1078,28 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     token does not depend on the rest of the batch. NaN logits count as -inf; a
     row without a logit above -inf gives -1. Returns int64 (B,).
     """
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or \
-            logits.dtype not in _DTYPES or not logits.is_cuda or \
-            (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be a bf16/fp32 (batch, vocab) CUDA tensor with contiguous "
-                         "rows")
+    dev = _device_of("logits", logits, "batch, vocab")
     B, V = logits.shape
-    _require_vector("u", u, B, torch.float32)
-    t_ptr, t_all = _per_row("temperature", temperature, B, torch.float32, 1.0)
-    k_ptr, k_all = _per_row("top_k", top_k, B, torch.int32, 0)
-    p_ptr, p_all = _per_row("top_p", top_p, B, torch.float32, 1.0)
-    m_ptr, m_all = _per_row("min_p", min_p, B, torch.float32, 0.0)
+    st = logits.stride()
+    if V > 1 and st[1] != 1:
+        raise ValueError("logits must have contiguous rows")
+    u_ptr = _require_vector("u", u, B, torch.float32, dev)
+    t_ptr, t_all = _per_row("temperature", temperature, B, torch.float32, 1.0, dev)
+    k_ptr, k_all = _per_row("top_k", top_k, B, torch.int32, 0, dev)
+    p_ptr, p_all = _per_row("top_p", top_p, B, torch.float32, 1.0, dev)
+    m_ptr, m_all = _per_row("min_p", min_p, B, torch.float32, 0.0, dev)
     if not (t_all >= 0.0 and k_all >= 0 and p_all >= 0.0 and 0.0 <= m_all <= 1.0):
         raise ValueError(f"temperature={t_all} top_k={k_all} top_p={p_all} must be >= 0 and "
                          f"min_p={m_all} within [0, 1]")
     if out is None:
-        out = torch.empty((B,), dtype=torch.int64, device=logits.device)
+        out = u.new_empty((B,), dtype=torch.int64)
+        o_ptr = out.data_ptr()
     else:
-        _require_vector("out", out, B, torch.int64)
-    _same_device(logits, ("u", u), ("out", out),
-                 *((n, t) for n, t in (("temperature", temperature), ("top_k", top_k),
-                                       ("top_p", top_p), ("min_p", min_p))
-                   if isinstance(t, torch.Tensor)))
-    a = nat.SampleArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], B, V,
-                       u.data_ptr(), t_ptr, k_ptr, p_ptr, m_ptr, t_all, k_all, p_all, m_all,
-                       out.data_ptr())
-    nat.check(nat.load().enl_sample_tokens(ctypes.byref(a), _stream()), "enl_sample_tokens")
+        o_ptr = _require_vector("out", out, B, torch.int64, dev)
+    a = nat.SampleArgs(logits.data_ptr(), st[0], _DTYPES[logits.dtype], B, V, u_ptr, t_ptr, k_ptr,
+                       p_ptr, m_ptr, float(t_all), min(int(k_all), 0x7fffffff), float(p_all),
+                       float(m_all), o_ptr)
+    status = nat.load().enl_sample_tokens(ctypes.byref(a), _raw_stream(dev))
+    if status:
+        nat.check(status, "enl_sample_tokens")
     return out
