@@ -48,6 +48,14 @@ int check_pool(const char* fn, const void* k, const void* v, int64_t sp, int64_t
   return ENL_OK;
 }
 
+// (token, head) pairs are numbered with 32 bits.
+int check_units(const char* fn, int32_t batch, int32_t seq, int32_t num_heads) {
+  if ((long long)batch * seq * num_heads > 0x7fffffffll)
+    return fail(ENL_ERR_UNSUPPORTED, "%s: batch * seq * num_heads = %lld exceeds 2^31 - 1", fn,
+                (long long)batch * seq * num_heads);
+  return ENL_OK;
+}
+
 // The norm weights and rotation tables that forward and backward share.
 int check_norm_rope(const char* fn, const float* wq, const float* wk, const float* cos_t,
                     const float* sin_t, int64_t rows) {
@@ -83,6 +91,7 @@ int enl_qk_norm_rope(const enl_qk_norm_rope_args* a, void* stream) {
     return fail(ENL_ERR_INVALID, "%s: needs norm weights, rotation tables or both", fn);
   if (!paged && a->n_new) return fail(ENL_ERR_INVALID, "%s: n_new needs k_pages", fn);
   if (a->batch == 0 || a->seq == 0) return ENL_OK;
+  if ((st = check_units(fn, a->batch, a->seq, a->num_heads))) return st;
   if ((st = check_operand(fn, "q", a->q, a->q_stride_b, a->q_stride_s, a->q_stride_h, a->in_dtype)))
     return st;
   if ((st = check_operand(fn, "k", a->k, a->k_stride_b, a->k_stride_s, a->k_stride_h, a->in_dtype)))
@@ -141,7 +150,7 @@ size_t enl_qk_norm_rope_backward_workspace_bytes(const enl_qk_norm_rope_backward
   int sms = 0;
   if (sm_count(&sms)) return 0;
   return (size_t)qk_rope_bwd_blocks(a->batch, a->seq, a->num_heads, a->num_kv_heads, a->head_dim,
-                                    sms) * 2 * a->head_dim * sizeof(float);
+                                    sms) * a->head_dim * sizeof(float);
 }
 
 int enl_qk_norm_rope_backward(const enl_qk_norm_rope_backward_args* a, void* stream) {
@@ -158,6 +167,7 @@ int enl_qk_norm_rope_backward(const enl_qk_norm_rope_backward_args* a, void* str
     return st;
   if (!a->q_weight && !a->rope_cos)
     return fail(ENL_ERR_INVALID, "%s: needs norm weights, rotation tables or both", fn);
+  if ((st = check_units(fn, a->batch, a->seq, a->num_heads))) return st;
   if ((st = check_operand(fn, "dq_out", a->dq_out, a->dqo_stride_b, a->dqo_stride_s,
                           a->dqo_stride_h, a->grad_dtype)))
     return st;
@@ -184,7 +194,7 @@ int enl_qk_norm_rope_backward(const enl_qk_norm_rope_backward_args* a, void* str
     if (!a->dq_weight || !a->dk_weight)
       return fail(ENL_ERR_INVALID, "%s: dq_weight and dk_weight must be non-NULL with norm weights",
                   fn);
-    const size_t need = (size_t)blocks * 2 * a->head_dim * sizeof(float);
+    const size_t need = (size_t)blocks * a->head_dim * sizeof(float);
     if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
       return fail(ENL_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)",
                   fn, need, a->workspace ? a->workspace_bytes : (size_t)0);

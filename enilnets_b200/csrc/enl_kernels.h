@@ -337,7 +337,7 @@ struct QkRopeBwdParams {
   const float* sin_t;
   long long rows, pos0;
   const int* start;
-  float* partial;  // (n_blocks, 2, D)
+  float* partial;  // (n_blocks, D)
   int n_blocks;
 };
 // Blocks of the backward's grid (they bound the partial sums' size).

@@ -8,12 +8,12 @@
 //   dx = rstd (g - xh mean(g xh)),  dw = sum dz xh
 //
 // All three move each element once and compute about ten operations on it, so
-// HBM bounds them. A group of D / 8 lanes (rounded up to a power of two) owns
-// one head of one token: lane j holds elements 4j .. 4j+3 of the first half and
-// their partners of the second half, so the rotation needs no exchange and the
-// norm one reduction over the group. A group takes up to kHeads heads of a
-// token at a time: their loads are all in flight together, and the token's
-// angles are read once for them.
+// HBM bounds them. A group of lanes owns one head of one token: a lane holds E
+// consecutive elements of the first half and their E partners of the second,
+// so the rotation needs no exchange and the norm one reduction over the group.
+// E is 8 where 16-bit values and the head dim allow it (16-byte loads), else 4.
+// A group takes several heads of a token at a time: their loads are in flight
+// together, kept packed until their turn, and the token's angles are read once.
 #include <algorithm>
 
 #include "enl_common.cuh"
@@ -24,44 +24,58 @@ namespace enl {
 namespace qkr {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;
+constexpr int kHeads = 4;     // heads of a token that a group takes, forward
+constexpr int kBwdHeads = 2;  // backward (gradients and inputs: more bytes each)
 
-struct Quad {
-  float v[4];
+// E elements as loaded: words of two bf16 or one fp32.
+template <bool kF32, int E>
+struct Raw {
+  static constexpr int kWords = kF32 ? E : E / 2;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const void* base, long long elem) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(
+        reinterpret_cast<const uint8_t*>(base) + elem * (kF32 ? 4 : 2));
+    if constexpr (kWords == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p + i);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (kF32) return __uint_as_float(w[e]);
+    return e % 2 ? bf16hi_to_f32(w[e / 2]) : bf16lo_to_f32(w[e / 2]);
+  }
 };
 
-template <bool kF32>
-__device__ __forceinline__ Quad load4(const void* base, long long elem) {
-  Quad q;
+template <bool kF32, int E>
+__device__ __forceinline__ void store(void* base, long long elem, const float (&x)[E]) {
   if constexpr (kF32) {
-    const float4 f = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + elem);
-    q.v[0] = f.x, q.v[1] = f.y, q.v[2] = f.z, q.v[3] = f.w;
+    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + elem);
+#pragma unroll
+    for (int i = 0; i < E; i += 4) p[i / 4] = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
   } else {
-    const uint2 w =
-        *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(base) + elem);
-    q.v[0] = bf16lo_to_f32(w.x), q.v[1] = bf16hi_to_f32(w.x);
-    q.v[2] = bf16lo_to_f32(w.y), q.v[3] = bf16hi_to_f32(w.y);
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<uint32_t*>(&v);
+    }
+    uint8_t* p = reinterpret_cast<uint8_t*>(base) + elem * 2;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  return q;
-}
-
-template <bool kF32>
-__device__ __forceinline__ void store4(void* base, long long elem, const Quad& q) {
-  if constexpr (kF32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + elem) =
-        make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
-  } else {
-    __nv_bfloat162 lo = __floats2bfloat162_rn(q.v[0], q.v[1]);
-    __nv_bfloat162 hi = __floats2bfloat162_rn(q.v[2], q.v[3]);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(base) + elem) =
-        make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
-  }
-}
-
-__device__ __forceinline__ Quad quad(float x) {
-  Quad q;
-  q.v[0] = q.v[1] = q.v[2] = q.v[3] = x;
-  return q;
 }
 
 template <int LG>
@@ -71,253 +85,247 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// One unit: heads [h0, h0 + n) of operand `op` at one token.
-struct Unit {
-  int op, b, s, h0, n;
-};
-
-__device__ __forceinline__ Unit unit_of(long long u, int S, int H, int Hkv, int nq, int nk, int nch,
-                                        int hc) {
-  Unit t;
-  const long long token = u / nch;
-  int c = (int)(u - token * nch);
-  t.b = (int)(token / S);
-  t.s = (int)(token - (long long)t.b * S);
-  t.op = c < nq ? 0 : c < nq + nk ? 1 : 2;
-  c -= t.op == 0 ? 0 : t.op == 1 ? nq : nq + nk;
-  const int heads = t.op == 0 ? H : Hkv;
-  t.h0 = c * hc;
-  t.n = min(hc, heads - t.h0);
-  return t;
-}
-
-template <bool kIn32, bool kOut32, int LG>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopeParams p, int hc,
-                                                                int nq, int nk, int nch,
-                                                                long long n_units) {
-  const long long u = ((long long)blockIdx.x * kThreads + threadIdx.x) / LG;
+// grid: (blocks over the tokens, head chunks of q, then k, then v).
+template <bool kIn32, bool kOut32, int E, int LG>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopeParams p, int nq,
+                                                                int nk) {
+  const int token = blockIdx.x * (kThreads / LG) + threadIdx.x / LG;
   const int j = threadIdx.x % LG;
   const int half = p.D / 2;
-  const bool real_unit = u < n_units;
-  const Unit t = unit_of(real_unit ? u : 0, p.S, p.H, p.Hkv, nq, nk, nch, hc);
-  const bool live = real_unit && j * 4 < half;
+  const int chunk = blockIdx.y;
+  const int op = chunk < nq ? 0 : chunk < nq + nk ? 1 : 2;
+  const int h0 = (chunk - (op == 0 ? 0 : op == 1 ? nq : nq + nk)) * kHeads;
+  const int n = min(kHeads, (op == 0 ? p.H : p.Hkv) - h0);
+  const bool live = token < p.B * p.S && j * E < half;
+  const int b = live ? token / p.S : 0, s = live ? token % p.S : 0;
+
+  const long long xe = b * p.x_sb[op] + s * p.x_ss[op] + h0 * p.x_sh[op] + j * E;
+  Raw<kIn32, E> ra[kHeads], rb[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    if (live && i < n) {
+      ra[i].load(p.x[op], xe + i * p.x_sh[op]);
+      rb[i].load(p.x[op], xe + i * p.x_sh[op] + half);
+    } else {
+      ra[i].zero();
+      rb[i].zero();
+    }
+  }
 
   // Where the token goes, and whether it is one.
-  const long long at = (p.start ? p.start[t.b] : 0) + (long long)t.s;  // cache position
-  bool keep = !p.n_new || t.s < p.n_new[t.b];
+  const long long at = (p.start ? p.start[b] : 0) + (long long)s;  // cache position
+  bool keep = !p.n_new || s < p.n_new[b];
   const long long row = p.pos0 + at;
   if (keep && p.cos_t && (row < 0 || row >= p.rows)) {
-    if (live && j == 0) report_error(kDevBadIndex, t.s);
+    if (live && j == 0) report_error(kDevBadIndex, s);
     keep = false;
   }
   long long slot = 0;  // element offset of the token's row in the pools, kv head 0
   if (p.pages[0] && keep) {
-    const long long col = at / p.page_size;
-    int page = -1;
-    if (at >= 0 && col < p.max_pages) page = p.table[t.b * p.t_sb + col];
+    int page = -1, off = 0;
+    if (at >= 0 && at < (long long)p.max_pages * p.page_size) {
+      const int col = (int)at / p.page_size;
+      off = (int)at - col * p.page_size;
+      page = p.table[b * p.t_sb + col];
+    }
     if (page < 0 || page >= p.n_pages) {
-      if (live && j == 0) report_error(kDevBadIndex, t.s);
+      if (live && j == 0) report_error(kDevBadIndex, s);
       keep = false;
     } else {
-      slot = page * p.p_sp + (at - col * p.page_size) * p.p_ss;
+      slot = page * p.p_sp + off * p.p_ss;
     }
   }
+  const bool to_pages = op > 0 && p.pages[0];
+  void* y = to_pages ? p.pages[op - 1] : p.y[op];
+  const long long ys = to_pages ? p.p_sh : p.y_sh[op];
+  const long long ye = (to_pages ? slot : b * p.y_sb[op] + s * p.y_ss[op]) + h0 * ys + j * E;
 
-  const int op = t.op;
-  const long long xb = t.b * p.x_sb[op] + t.s * p.x_ss[op];
-  Quad a[kHeads], b[kHeads];
+  float c[E], sn[E], w1[E], w2[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) c[e] = w1[e] = w2[e] = 1.0f, sn[e] = 0.0f;
+  if (op < 2 && live && keep) {
+    if (p.cos_t) {
+      Raw<true, E> t;
+      t.load(p.cos_t, row * half + j * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) c[e] = t.at(e);
+      t.load(p.sin_t, row * half + j * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sn[e] = t.at(e);
+    }
+    if (p.w[op]) {
+      Raw<true, E> t;
+      t.load(p.w[op], j * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) w1[e] = t.at(e);
+      t.load(p.w[op], half + j * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) w2[e] = t.at(e);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    a[i] = b[i] = quad(0.0f);
-    if (live && keep && i < t.n) {
-      const long long e = xb + (t.h0 + i) * p.x_sh[op] + j * 4;
-      a[i] = load4<kIn32>(p.x[op], e);
-      b[i] = load4<kIn32>(p.x[op], e + half);
-    }
-  }
-  float r[kHeads];
-  if (p.w[0]) {
-    // Every group of the warp takes part in the reduction, values (op 2) too.
+    float x1[E], x2[E];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      float ss = 0.0f;
+    for (int e = 0; e < E; ++e) x1[e] = ra[i].at(e), x2[e] = rb[i].at(e);
+    if (op < 2) {  // the same for the whole block, which the reduction needs
+      float rstd = 1.0f;
+      if (p.w[0]) {
+        float ss = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ss = fmaf(a[i].v[e], a[i].v[e], fmaf(b[i].v[e], b[i].v[e], ss));
-      r[i] = group_sum<LG>(ss);
-    }
-  }
-  if (op < 2) {
-    Quad c = quad(1.0f), s = quad(0.0f), w1 = quad(1.0f), w2 = quad(1.0f);
-    if (p.cos_t && live && keep) {
-      c = load4<true>(p.cos_t, row * half + j * 4);
-      s = load4<true>(p.sin_t, row * half + j * 4);
-    }
-    const float* w = p.w[op];
-    if (w && live) {
-      w1 = load4<true>(w, j * 4);
-      w2 = load4<true>(w, half + j * 4);
-    }
+        for (int e = 0; e < E; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
+        rstd = rsqrtf(group_sum<LG>(ss) / (float)p.D + p.eps);
+      }
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const float rstd = w ? rsqrtf(r[i] / (float)p.D + p.eps) : 1.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float z1 = a[i].v[e] * rstd * w1.v[e];
-        const float z2 = b[i].v[e] * rstd * w2.v[e];
-        a[i].v[e] = z1 * c.v[e] - z2 * s.v[e];
-        b[i].v[e] = z2 * c.v[e] + z1 * s.v[e];
+      for (int e = 0; e < E; ++e) {
+        const float z1 = x1[e] * rstd * w1[e], z2 = x2[e] * rstd * w2[e];
+        x1[e] = z1 * c[e] - z2 * sn[e];
+        x2[e] = z2 * c[e] + z1 * sn[e];
       }
     }
-  }
-  if (!live) return;
-  if (op == 0 || !p.pages[0]) {
-    if (!keep) {
+    if (live && i < n && (keep || !to_pages)) {
+      if (!keep) {
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i) a[i] = b[i] = quad(0.0f);
-    }
-    const long long yb = t.b * p.y_sb[op] + t.s * p.y_ss[op];
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      if (i >= t.n) break;
-      const long long e = yb + (t.h0 + i) * p.y_sh[op] + j * 4;
-      store4<kOut32>(p.y[op], e, a[i]);
-      store4<kOut32>(p.y[op], e + half, b[i]);
-    }
-  } else if (keep) {
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      if (i >= t.n) break;
-      const long long e = slot + (t.h0 + i) * p.p_sh + j * 4;
-      store4<kOut32>(p.pages[op - 1], e, a[i]);
-      store4<kOut32>(p.pages[op - 1], e + half, b[i]);
+        for (int e = 0; e < E; ++e) x1[e] = x2[e] = 0.0f;
+      }
+      store<kOut32, E>(y, ye + i * ys, x1);
+      store<kOut32, E>(y, ye + i * ys + half, x2);
     }
   }
 }
 
 // ---------------------------------------------------------------- backward
-template <bool kIn32, bool kGrad32, bool kOut32, int LG>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_bwd_kernel(const QkRopeBwdParams p,
-                                                                    int nq, int nk,
-                                                                    long long n_units) {
+// Blocks [0, n_q) walk the units (token, kBwdHeads heads) of q, the others
+// those of k, and keep their sums of dw in registers.
+template <bool kIn32, bool kGrad32, bool kOut32, int E, int LG>
+__global__ void __launch_bounds__(kThreads, 2)
+    qk_norm_rope_bwd_kernel(const QkRopeBwdParams p, int n_q) {
   constexpr int kGroups = kThreads / LG;
+  const int op = blockIdx.x < n_q ? 0 : 1;
+  const int block = blockIdx.x - (op ? n_q : 0), blocks = op ? gridDim.x - n_q : n_q;
+  const int heads = op ? p.Hkv : p.H;
+  const int nch = (heads + kBwdHeads - 1) / kBwdHeads;
+  const int n_units = p.B * p.S * nch;
   const int j = threadIdx.x % LG;
   const int half = p.D / 2;
-  const bool lane_live = j * 4 < half;
+  const bool lane_live = j * E < half;
   const bool norm = p.w[0] != nullptr;
-  float dw[2][8];
+  float dw1[E], dw2[E], w1[E], w2[E];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.0f;
+  for (int e = 0; e < E; ++e) dw1[e] = dw2[e] = 0.0f, w1[e] = w2[e] = 1.0f;
+  if (norm && lane_live) {
+    Raw<true, E> t;
+    t.load(p.w[op], j * E);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w1[e] = t.at(e);
+    t.load(p.w[op], half + j * E);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w2[e] = t.at(e);
+  }
 
-  const long long first = (long long)blockIdx.x * kGroups + threadIdx.x / LG;
+  const int step = blocks * kGroups;
   // The bound is the same for every lane of a warp, which the reductions need.
-  const long long warp_first = (long long)blockIdx.x * kGroups + threadIdx.x / 32 * (32 / LG);
-  const long long step = (long long)gridDim.x * kGroups;
-  for (long long uw = warp_first, u = first; uw < n_units; uw += step, u += step) {
-    const bool live = lane_live && u < n_units;
-    const Unit t = unit_of(u < n_units ? u : 0, p.S, p.H, p.Hkv, nq, nk, nq + nk, kHeads);
-    const int op = t.op;
-    const long long row = p.pos0 + (p.start ? p.start[t.b] : 0) + (long long)t.s;
+  const int warp_first = block * kGroups + threadIdx.x / 32 * (32 / LG);
+  const int mine = threadIdx.x % 32 / LG;
+  for (long long uw = warp_first; uw < n_units; uw += step) {
+    const bool live = lane_live && uw + mine < n_units;
+    const int u = live ? (int)uw + mine : 0;
+    const int token = u / nch, h0 = (u - token * nch) * kBwdHeads;
+    const int b = token / p.S, s = token - b * p.S;
+    const int n = min(kBwdHeads, heads - h0);
+    const long long row = p.pos0 + (p.start ? p.start[b] : 0) + (long long)s;
     const bool keep = !p.cos_t || (row >= 0 && row < p.rows);
-    if (!keep && live && j == 0) report_error(kDevBadIndex, t.s);
-    const long long gb = t.b * p.dy_sb[op] + t.s * p.dy_ss[op];
-    const long long xb = t.b * p.x_sb[op] + t.s * p.x_ss[op];
-    Quad ga[kHeads], gbq[kHeads], a[kHeads], b[kHeads];
+    if (!keep && live && j == 0) report_error(kDevBadIndex, s);
+    const long long ge = b * p.dy_sb[op] + s * p.dy_ss[op] + h0 * p.dy_sh[op] + j * E;
+    const long long xe = b * p.x_sb[op] + s * p.x_ss[op] + h0 * p.x_sh[op] + j * E;
+    Raw<kGrad32, E> ga[kBwdHeads], gb[kBwdHeads];
+    Raw<kIn32, E> xa[kBwdHeads], xb[kBwdHeads];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      ga[i] = gbq[i] = a[i] = b[i] = quad(0.0f);
-      if (live && keep && i < t.n) {
-        const long long eg = gb + (t.h0 + i) * p.dy_sh[op] + j * 4;
-        ga[i] = load4<kGrad32>(p.dy[op], eg);
-        gbq[i] = load4<kGrad32>(p.dy[op], eg + half);
+    for (int i = 0; i < kBwdHeads; ++i) {
+      ga[i].zero(), gb[i].zero(), xa[i].zero(), xb[i].zero();
+      if (live && keep && i < n) {
+        ga[i].load(p.dy[op], ge + i * p.dy_sh[op]);
+        gb[i].load(p.dy[op], ge + i * p.dy_sh[op] + half);
         if (norm) {
-          const long long ex = xb + (t.h0 + i) * p.x_sh[op] + j * 4;
-          a[i] = load4<kIn32>(p.x[op], ex);
-          b[i] = load4<kIn32>(p.x[op], ex + half);
+          xa[i].load(p.x[op], xe + i * p.x_sh[op]);
+          xb[i].load(p.x[op], xe + i * p.x_sh[op] + half);
         }
       }
     }
-    Quad c = quad(1.0f), s = quad(0.0f), w1 = quad(1.0f), w2 = quad(1.0f);
+    Raw<true, E> c, sn;
+    c.zero(), sn.zero();
     if (p.cos_t && live && keep) {
-      c = load4<true>(p.cos_t, row * half + j * 4);
-      s = load4<true>(p.sin_t, row * half + j * 4);
+      c.load(p.cos_t, row * half + j * E);
+      sn.load(p.sin_t, row * half + j * E);
     }
-    if (norm && live) {
-      w1 = load4<true>(p.w[op], j * 4);
-      w2 = load4<true>(p.w[op], half + j * 4);
-    }
+    const long long ye = b * p.dx_sb[op] + s * p.dx_ss[op] + h0 * p.dx_sh[op] + j * E;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      float ss = 0.0f, gx = 0.0f;
+    for (int i = 0; i < kBwdHeads; ++i) {
+      float d1[E], d2[E];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float d1 = ga[i].v[e] * c.v[e] + gbq[i].v[e] * s.v[e];
-        const float d2 = gbq[i].v[e] * c.v[e] - ga[i].v[e] * s.v[e];
-        ga[i].v[e] = d1;
-        gbq[i].v[e] = d2;
-        ss = fmaf(a[i].v[e], a[i].v[e], fmaf(b[i].v[e], b[i].v[e], ss));
-        gx = fmaf(d1 * w1.v[e], a[i].v[e], fmaf(d2 * w2.v[e], b[i].v[e], gx));
+      for (int e = 0; e < E; ++e) {
+        const float a = ga[i].at(e), g = gb[i].at(e);
+        d1[e] = p.cos_t ? a * c.at(e) + g * sn.at(e) : a;
+        d2[e] = p.cos_t ? g * c.at(e) - a * sn.at(e) : g;
       }
-      if (!norm) continue;
-      ss = group_sum<LG>(ss);
-      gx = group_sum<LG>(gx);
-      const float r = rsqrtf(ss / (float)p.D + p.eps);
-      const float m = gx * r * r / (float)p.D;  // mean(g xh) / |x| scale: xh m' = x m
+      if (norm) {
+        float ss = 0.0f, gx = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x1 = a[i].v[e], x2 = b[i].v[e];
-        const float t1 = ga[i].v[e] * x1 * r, t2 = gbq[i].v[e] * x2 * r;
-        if (op == 0) {
-          dw[0][e] += t1, dw[0][4 + e] += t2;
-        } else {
-          dw[1][e] += t1, dw[1][4 + e] += t2;
+        for (int e = 0; e < E; ++e) {
+          const float x1 = xa[i].at(e), x2 = xb[i].at(e);
+          ss = fmaf(x1, x1, fmaf(x2, x2, ss));
+          gx = fmaf(d1[e] * w1[e], x1, fmaf(d2[e] * w2[e], x2, gx));
         }
-        ga[i].v[e] = r * (ga[i].v[e] * w1.v[e] - x1 * m);
-        gbq[i].v[e] = r * (gbq[i].v[e] * w2.v[e] - x2 * m);
-      }
-    }
-    if (live) {
-      const long long yb = t.b * p.dx_sb[op] + t.s * p.dx_ss[op];
+        ss = group_sum<LG>(ss);
+        gx = group_sum<LG>(gx);
+        const float r = rsqrtf(ss / (float)p.D + p.eps);
+        const float m = gx * r * r / (float)p.D;  // mean(g xh) rstd
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i) {
-        if (i >= t.n) break;
-        const long long e = yb + (t.h0 + i) * p.dx_sh[op] + j * 4;
-        store4<kOut32>(p.dx[op], e, ga[i]);
-        store4<kOut32>(p.dx[op], e + half, gbq[i]);
+        for (int e = 0; e < E; ++e) {
+          const float x1 = xa[i].at(e), x2 = xb[i].at(e);
+          dw1[e] = fmaf(d1[e], x1 * r, dw1[e]);
+          dw2[e] = fmaf(d2[e], x2 * r, dw2[e]);
+          d1[e] = r * (d1[e] * w1[e] - x1 * m);
+          d2[e] = r * (d2[e] * w2[e] - x2 * m);
+        }
+      }
+      if (live && i < n) {
+        store<kOut32, E>(p.dx[op], ye + i * p.dx_sh[op], d1);
+        store<kOut32, E>(p.dx[op], ye + i * p.dx_sh[op] + half, d2);
       }
     }
   }
   if (!norm) return;
   // The block's sums, lane groups added in order.
-  __shared__ float sm[kGroups][LG * 8];
+  __shared__ float sm[kGroups][2 * LG * E];
 #pragma unroll
-  for (int op = 0; op < 2; ++op) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sm[threadIdx.x / LG][j * 4 + e] = dw[op][e];
-      sm[threadIdx.x / LG][LG * 4 + j * 4 + e] = dw[op][4 + e];
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < p.D; d += kThreads) {
-      const int col = d < half ? d : LG * 4 + (d - half);
-      float sum = 0.0f;
-      for (int g = 0; g < kGroups; ++g) sum += sm[g][col];
-      p.partial[((long long)blockIdx.x * 2 + op) * p.D + d] = sum;
-    }
+  for (int e = 0; e < E; ++e) {
+    sm[threadIdx.x / LG][j * E + e] = dw1[e];
+    sm[threadIdx.x / LG][LG * E + j * E + e] = dw2[e];
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.D; d += kThreads) {
+    const int col = d < half ? d : LG * E + (d - half);
+    float sum = 0.0f;
+    for (int g = 0; g < kGroups; ++g) sum += sm[g][col];
+    p.partial[(long long)blockIdx.x * p.D + d] = sum;
   }
 }
 
-// dw[op][d] = sum over blocks of partial[block][op][d]: 32 columns a block,
-// eight slices of the blocks each, added in a fixed order.
+// dw[op][d] = sum of the partial sums of op's blocks: 32 columns a block, eight
+// slices of the blocks each, added in a fixed order.
 __global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ partial,
-                                                         int n_blocks, int D, float* dwq,
+                                                         int n_q, int n_blocks, int D, float* dwq,
                                                          float* dwk) {
   __shared__ float sm[8][32];
   const int op = blockIdx.y, col = threadIdx.x % 32, slice = threadIdx.x / 32;
   const int d = blockIdx.x * 32 + col;
+  const int first = op ? n_q : 0, end = op ? n_blocks : n_q;
   float sum = 0.0f;
-  if (d < D)
-    for (int i = slice; i < n_blocks; i += 8) sum += partial[((long long)i * 2 + op) * D + d];
+  if (d < D) {
+#pragma unroll 8
+    for (int i = first + slice; i < end; i += 8) sum += partial[(long long)i * D + d];
+  }
   sm[slice][col] = sum;
   __syncthreads();
   if (slice == 0 && d < D) {
@@ -326,45 +334,72 @@ __global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict
   }
 }
 
-int lanes_for(int D) { return D > 64 ? 16 : D > 32 ? 8 : 4; }
+// Lanes of a group: the power of two that holds half a head of E elements each.
+int lanes_for(int D, int E) {
+  int lg = 4;
+  while (lg * E * 2 < D) lg *= 2;
+  return lg;
+}
 
+template <bool kIn32, bool kOut32, int E>
+cudaError_t launch_fwd_e(const QkRopeParams& p, cudaStream_t stream) {
+  const int nq = (p.H + kHeads - 1) / kHeads, nk = (p.Hkv + kHeads - 1) / kHeads;
+  const int LG = lanes_for(p.D, E);
+  const int groups = kThreads / LG;
+  const dim3 grid((p.B * p.S + groups - 1) / groups, nq + nk + (p.pages[0] ? nk : 0));
+  if constexpr (E == 4) {
+    if (LG == 16)
+      qk_norm_rope_kernel<kIn32, kOut32, E, 16><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+  }
+  if (LG == 8)
+    qk_norm_rope_kernel<kIn32, kOut32, E, 8><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+  else if (LG == 4)
+    qk_norm_rope_kernel<kIn32, kOut32, E, 4><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+  return cudaGetLastError();
+}
+
+// 16-byte loads of bf16 need halves of a multiple of eight elements.
 template <bool kIn32, bool kOut32>
 cudaError_t launch_fwd(const QkRopeParams& p, cudaStream_t stream) {
-  const int hc = kHeads;
-  const int nq = (p.H + hc - 1) / hc, nk = (p.Hkv + hc - 1) / hc;
-  const int nch = nq + nk + (p.pages[0] ? nk : 0);
-  const long long n_units = (long long)p.B * p.S * nch;
-  if (n_units == 0) return cudaSuccess;
-  const int LG = lanes_for(p.D);
-  const long long blocks = (n_units * LG + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks);
-  if (LG == 16)
-    qk_norm_rope_kernel<kIn32, kOut32, 16><<<grid, kThreads, 0, stream>>>(p, hc, nq, nk, nch, n_units);
-  else if (LG == 8)
-    qk_norm_rope_kernel<kIn32, kOut32, 8><<<grid, kThreads, 0, stream>>>(p, hc, nq, nk, nch, n_units);
-  else
-    qk_norm_rope_kernel<kIn32, kOut32, 4><<<grid, kThreads, 0, stream>>>(p, hc, nq, nk, nch, n_units);
+  if constexpr (!kIn32) {
+    if (p.D % 16 == 0) return launch_fwd_e<kIn32, kOut32, 8>(p, stream);
+  }
+  return launch_fwd_e<kIn32, kOut32, 4>(p, stream);
+}
+
+bool bwd_wide(int D, bool in32, bool grad32) { return D % 16 == 0 && !(in32 && grad32); }
+
+// q's share of the backward's blocks, in proportion to the heads.
+int bwd_q_blocks(int n_blocks, int H, int Hkv) {
+  return std::max(1, std::min(n_blocks - 1, (int)((long long)n_blocks * H / (H + Hkv))));
+}
+
+template <bool kIn32, bool kGrad32, bool kOut32, int E>
+cudaError_t launch_bwd_e(const QkRopeBwdParams& p, cudaStream_t stream) {
+  const int LG = lanes_for(p.D, E), blocks = p.n_blocks;
+  const int n_q = bwd_q_blocks(blocks, p.H, p.Hkv);
+  if constexpr (E == 4) {
+    if (LG == 16)
+      qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 16><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  }
+  if (LG == 8)
+    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 8><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  else if (LG == 4)
+    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 4><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !p.w[0]) return e;
+  qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, stream>>>(p.partial, n_q, blocks, p.D,
+                                                                 p.dw[0], p.dw[1]);
   return cudaGetLastError();
 }
 
 template <bool kIn32, bool kGrad32, bool kOut32>
 cudaError_t launch_bwd(const QkRopeBwdParams& p, cudaStream_t stream) {
-  const int nq = (p.H + kHeads - 1) / kHeads, nk = (p.Hkv + kHeads - 1) / kHeads;
-  const long long n_units = (long long)p.B * p.S * (nq + nk);
-  const int LG = lanes_for(p.D);
-  const int blocks = p.n_blocks;
-  if (LG == 16)
-    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 16><<<blocks, kThreads, 0, stream>>>(p, nq, nk, n_units);
-  else if (LG == 8)
-    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 8><<<blocks, kThreads, 0, stream>>>(p, nq, nk, n_units);
-  else
-    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 4><<<blocks, kThreads, 0, stream>>>(p, nq, nk, n_units);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !p.w[0]) return e;
-  qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, stream>>>(p.partial, blocks, p.D, p.dw[0],
-                                                                 p.dw[1]);
-  return cudaGetLastError();
+  if constexpr (!(kIn32 && kGrad32)) {
+    if (bwd_wide(p.D, kIn32, kGrad32))
+      return launch_bwd_e<kIn32, kGrad32, kOut32, 8>(p, stream);
+  }
+  return launch_bwd_e<kIn32, kGrad32, kOut32, 4>(p, stream);
 }
 
 }  // namespace qkr
@@ -377,12 +412,14 @@ cudaError_t launch_qk_norm_rope(const QkRopeParams& p, cudaStream_t stream) {
                     : qkr::launch_fwd<false, false>(p, stream);
 }
 
+// Two blocks a SM, or one for every group of units when there are fewer; two
+// at least, since q and k have their own.
 int qk_rope_bwd_blocks(int B, int S, int H, int Hkv, int D, int n_sms) {
-  const long long units = (long long)B * S * ((H + qkr::kHeads - 1) / qkr::kHeads +
-                                              (Hkv + qkr::kHeads - 1) / qkr::kHeads);
-  const long long per_block = qkr::kThreads / qkr::lanes_for(D);
+  const long long units = (long long)B * S * ((H + qkr::kBwdHeads - 1) / qkr::kBwdHeads +
+                                              (Hkv + qkr::kBwdHeads - 1) / qkr::kBwdHeads);
+  const long long per_block = qkr::kThreads / qkr::lanes_for(D, 4);
   const long long blocks = (units + per_block - 1) / per_block;
-  return (int)std::max(1ll, std::min(blocks, (long long)n_sms * 4));
+  return (int)std::max(2ll, std::min(blocks, (long long)n_sms * 2));
 }
 
 cudaError_t launch_qk_norm_rope_backward(const QkRopeBwdParams& p, cudaStream_t stream) {
