@@ -55,10 +55,24 @@ struct Raw {
     if constexpr (kF32) return __uint_as_float(w[e]);
     return e % 2 ? bf16hi_to_f32(w[e / 2]) : bf16lo_to_f32(w[e / 2]);
   }
+  // Elements 2i and 2i + 1 as one operand of the packed fp32 instructions.
+  __device__ __forceinline__ uint64_t pair(int i) const {
+    return f2_pack(at(2 * i), at(2 * i + 1));
+  }
 };
 
+__device__ __forceinline__ uint64_t both(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
 template <bool kF32, int E>
-__device__ __forceinline__ void store(void* base, long long elem, const float (&x)[E]) {
+__device__ __forceinline__ void store(void* base, long long elem, const uint64_t (&pairs)[E / 2]) {
+  float x[E];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) f2_unpack(pairs[i], x[2 * i], x[2 * i + 1]);
   if constexpr (kF32) {
     float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + elem);
 #pragma unroll
@@ -85,14 +99,16 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// grid: (blocks over the tokens, head chunks of q, then k, then v).
+// One block: kThreads / LG tokens of one head chunk. The chunks of q, then k,
+// then v run fastest over the grid, so that blocks that run together read whole
+// rows of a fused projection.
 template <bool kIn32, bool kOut32, int E, int LG>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopeParams p, int nq,
-                                                                int nk) {
-  const int token = blockIdx.x * (kThreads / LG) + threadIdx.x / LG;
+                                                                int nk, int nch) {
+  const int chunk = blockIdx.x % nch;
+  const int token = blockIdx.x / nch * (kThreads / LG) + threadIdx.x / LG;
   const int j = threadIdx.x % LG;
   const int half = p.D / 2;
-  const int chunk = blockIdx.y;
   const int op = chunk < nq ? 0 : chunk < nq + nk ? 1 : 2;
   const int h0 = (chunk - (op == 0 ? 0 : op == 1 ? nq : nq + nk)) * kHeads;
   const int n = min(kHeads, (op == 0 ? p.H : p.Hkv) - h0);
@@ -140,53 +156,60 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopePara
   const long long ys = to_pages ? p.p_sh : p.y_sh[op];
   const long long ye = (to_pages ? slot : b * p.y_sb[op] + s * p.y_ss[op]) + h0 * ys + j * E;
 
-  float c[E], sn[E], w1[E], w2[E];
+  // The token's turn with the norm's weights in it: y1 = r (x1 c1 - x2 s2),
+  // y2 = r (x2 c2 + x1 s1) with c1 = w1 c, s2 = w2 s and so on.
+  constexpr int P = E / 2;
+  uint64_t c1[P], c2[P], s1[P], s2[P];
 #pragma unroll
-  for (int e = 0; e < E; ++e) c[e] = w1[e] = w2[e] = 1.0f, sn[e] = 0.0f;
+  for (int i = 0; i < P; ++i) c1[i] = c2[i] = both(1.0f), s1[i] = s2[i] = both(0.0f);
   if (op < 2 && live && keep) {
     if (p.cos_t) {
       Raw<true, E> t;
       t.load(p.cos_t, row * half + j * E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) c[e] = t.at(e);
+      for (int i = 0; i < P; ++i) c1[i] = c2[i] = t.pair(i);
       t.load(p.sin_t, row * half + j * E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) sn[e] = t.at(e);
+      for (int i = 0; i < P; ++i) s1[i] = t.pair(i), s2[i] = f2_mul(t.pair(i), both(-1.0f));
     }
     if (p.w[op]) {
       Raw<true, E> t;
       t.load(p.w[op], j * E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) w1[e] = t.at(e);
+      for (int i = 0; i < P; ++i) c1[i] = f2_mul(c1[i], t.pair(i)), s1[i] = f2_mul(s1[i], t.pair(i));
       t.load(p.w[op], half + j * E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) w2[e] = t.at(e);
+      for (int i = 0; i < P; ++i) c2[i] = f2_mul(c2[i], t.pair(i)), s2[i] = f2_mul(s2[i], t.pair(i));
     }
   }
+  const float inv_d = 1.0f / (float)p.D;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    float x1[E], x2[E];
+    uint64_t x1[P], x2[P];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x1[e] = ra[i].at(e), x2[e] = rb[i].at(e);
+    for (int e = 0; e < P; ++e) x1[e] = ra[i].pair(e), x2[e] = rb[i].pair(e);
     if (op < 2) {  // the same for the whole block, which the reduction needs
-      float rstd = 1.0f;
       if (p.w[0]) {
-        float ss = 0.0f;
+        uint64_t ss = both(0.0f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-        rstd = rsqrtf(group_sum<LG>(ss) / (float)p.D + p.eps);
+        for (int e = 0; e < P; ++e) ss = f2_fma(x1[e], x1[e], f2_fma(x2[e], x2[e], ss));
+        const uint64_t r = both(rsqrtf(fmaf(group_sum<LG>(pair_sum(ss)), inv_d, p.eps)));
+#pragma unroll
+        for (int e = 0; e < P; ++e) x1[e] = f2_mul(x1[e], r), x2[e] = f2_mul(x2[e], r);
       }
+      if (p.w[0] || p.cos_t) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float z1 = x1[e] * rstd * w1[e], z2 = x2[e] * rstd * w2[e];
-        x1[e] = z1 * c[e] - z2 * sn[e];
-        x2[e] = z2 * c[e] + z1 * sn[e];
+        for (int e = 0; e < P; ++e) {
+          const uint64_t y1 = f2_fma(x1[e], c1[e], f2_mul(x2[e], s2[e]));
+          x2[e] = f2_fma(x2[e], c2[e], f2_mul(x1[e], s1[e]));
+          x1[e] = y1;
+        }
       }
     }
     if (live && i < n && (keep || !to_pages)) {
       if (!keep) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x1[e] = x2[e] = 0.0f;
+        for (int e = 0; e < P; ++e) x1[e] = x2[e] = both(0.0f);
       }
       store<kOut32, E>(y, ye + i * ys, x1);
       store<kOut32, E>(y, ye + i * ys + half, x2);
@@ -210,18 +233,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int half = p.D / 2;
   const bool lane_live = j * E < half;
   const bool norm = p.w[0] != nullptr;
-  float dw1[E], dw2[E], w1[E], w2[E];
+  constexpr int P = E / 2;
+  uint64_t dw1[P], dw2[P];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dw1[e] = dw2[e] = 0.0f, w1[e] = w2[e] = 1.0f;
+  for (int i = 0; i < P; ++i) dw1[i] = dw2[i] = both(0.0f);
+  Raw<true, E> w1, w2;
+  w1.zero(), w2.zero();
   if (norm && lane_live) {
-    Raw<true, E> t;
-    t.load(p.w[op], j * E);
-#pragma unroll
-    for (int e = 0; e < E; ++e) w1[e] = t.at(e);
-    t.load(p.w[op], half + j * E);
-#pragma unroll
-    for (int e = 0; e < E; ++e) w2[e] = t.at(e);
+    w1.load(p.w[op], j * E);
+    w2.load(p.w[op], half + j * E);
   }
+  const float inv_d = 1.0f / (float)p.D;
 
   const int step = blocks * kGroups;
   // The bound is the same for every lane of a warp, which the reductions need.
@@ -261,32 +283,34 @@ __global__ void __launch_bounds__(kThreads, 2)
     const long long ye = b * p.dx_sb[op] + s * p.dx_ss[op] + h0 * p.dx_sh[op] + j * E;
 #pragma unroll
     for (int i = 0; i < kBwdHeads; ++i) {
-      float d1[E], d2[E];
+      uint64_t d1[P], d2[P];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float a = ga[i].at(e), g = gb[i].at(e);
-        d1[e] = p.cos_t ? a * c.at(e) + g * sn.at(e) : a;
-        d2[e] = p.cos_t ? g * c.at(e) - a * sn.at(e) : g;
+      for (int e = 0; e < P; ++e) {
+        d1[e] = ga[i].pair(e), d2[e] = gb[i].pair(e);
+        if (p.cos_t) {
+          const uint64_t t = f2_mul(d1[e], f2_mul(sn.pair(e), both(-1.0f)));
+          d1[e] = f2_fma(d1[e], c.pair(e), f2_mul(d2[e], sn.pair(e)));
+          d2[e] = f2_fma(d2[e], c.pair(e), t);
+        }
       }
       if (norm) {
-        float ss = 0.0f, gx = 0.0f;
+        uint64_t ss = both(0.0f), gx = both(0.0f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float x1 = xa[i].at(e), x2 = xb[i].at(e);
-          ss = fmaf(x1, x1, fmaf(x2, x2, ss));
-          gx = fmaf(d1[e] * w1[e], x1, fmaf(d2[e] * w2[e], x2, gx));
+        for (int e = 0; e < P; ++e) {
+          const uint64_t x1 = xa[i].pair(e), x2 = xb[i].pair(e);
+          ss = f2_fma(x1, x1, f2_fma(x2, x2, ss));
+          gx = f2_fma(f2_mul(d1[e], w1.pair(e)), x1, f2_fma(f2_mul(d2[e], w2.pair(e)), x2, gx));
         }
-        ss = group_sum<LG>(ss);
-        gx = group_sum<LG>(gx);
-        const float r = rsqrtf(ss / (float)p.D + p.eps);
-        const float m = gx * r * r / (float)p.D;  // mean(g xh) rstd
+        const float r = rsqrtf(fmaf(group_sum<LG>(pair_sum(ss)), inv_d, p.eps));
+        const float m = group_sum<LG>(pair_sum(gx)) * inv_d * r * r;  // mean(g xh) rstd
+        const uint64_t rr = both(r), nm = both(-m);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float x1 = xa[i].at(e), x2 = xb[i].at(e);
-          dw1[e] = fmaf(d1[e], x1 * r, dw1[e]);
-          dw2[e] = fmaf(d2[e], x2 * r, dw2[e]);
-          d1[e] = r * (d1[e] * w1[e] - x1 * m);
-          d2[e] = r * (d2[e] * w2[e] - x2 * m);
+        for (int e = 0; e < P; ++e) {
+          const uint64_t x1 = xa[i].pair(e), x2 = xb[i].pair(e);
+          dw1[e] = f2_fma(d1[e], f2_mul(x1, rr), dw1[e]);
+          dw2[e] = f2_fma(d2[e], f2_mul(x2, rr), dw2[e]);
+          d1[e] = f2_mul(rr, f2_fma(x1, nm, f2_mul(d1[e], w1.pair(e))));
+          d2[e] = f2_mul(rr, f2_fma(x2, nm, f2_mul(d2[e], w2.pair(e))));
         }
       }
       if (live && i < n) {
@@ -299,9 +323,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   // The block's sums, lane groups added in order.
   __shared__ float sm[kGroups][2 * LG * E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    sm[threadIdx.x / LG][j * E + e] = dw1[e];
-    sm[threadIdx.x / LG][LG * E + j * E + e] = dw2[e];
+  for (int i = 0; i < P; ++i) {
+    float* at = &sm[threadIdx.x / LG][j * E + 2 * i];
+    f2_unpack(dw1[i], at[0], at[1]);
+    f2_unpack(dw2[i], at[LG * E], at[LG * E + 1]);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < p.D; d += kThreads) {
@@ -346,15 +371,16 @@ cudaError_t launch_fwd_e(const QkRopeParams& p, cudaStream_t stream) {
   const int nq = (p.H + kHeads - 1) / kHeads, nk = (p.Hkv + kHeads - 1) / kHeads;
   const int LG = lanes_for(p.D, E);
   const int groups = kThreads / LG;
-  const dim3 grid((p.B * p.S + groups - 1) / groups, nq + nk + (p.pages[0] ? nk : 0));
+  const int nch = nq + nk + (p.pages[0] ? nk : 0);
+  const int grid = (p.B * p.S + groups - 1) / groups * nch;
   if constexpr (E == 4) {
     if (LG == 16)
-      qk_norm_rope_kernel<kIn32, kOut32, E, 16><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+      qk_norm_rope_kernel<kIn32, kOut32, E, 16><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   }
   if (LG == 8)
-    qk_norm_rope_kernel<kIn32, kOut32, E, 8><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+    qk_norm_rope_kernel<kIn32, kOut32, E, 8><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   else if (LG == 4)
-    qk_norm_rope_kernel<kIn32, kOut32, E, 4><<<grid, kThreads, 0, stream>>>(p, nq, nk);
+    qk_norm_rope_kernel<kIn32, kOut32, E, 4><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   return cudaGetLastError();
 }
 
