@@ -11,9 +11,14 @@
 // HBM bounds them. A group of lanes owns one head of one token: a lane holds E
 // consecutive elements of the first half and their E partners of the second,
 // so the rotation needs no exchange and the norm one reduction over the group.
-// E is 8 where 16-bit values and the head dim allow it (16-byte loads), else 4.
 // A group takes several heads of a token at a time: their loads are in flight
 // together, kept packed until their turn, and the token's angles are read once.
+// How many, and how many blocks share an SM, is a choice between loads in
+// flight and registers; measured (bf16, 8 x 4096 tokens, 16 + 16 heads of 128,
+// floor 82 us): E = 8 with 8 heads and 2 blocks 86 us, 4 heads and 3 blocks
+// 91 us, 2 heads and 4 blocks 102 us. The backward (4 x 4095, 16 + 4 heads,
+// fp32 gradients, floor 51 us): E = 4 with 4 heads and 2 blocks 65 us, 2 heads
+// and 3 blocks 66 us, E = 8 with 2 heads 68 us, 1 head and 3 blocks 99 us.
 #include <algorithm>
 
 #include "enl_common.cuh"
@@ -24,8 +29,7 @@ namespace enl {
 namespace qkr {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;     // heads of a token that a group takes, forward
-constexpr int kBwdHeads = 2;  // backward (gradients and inputs: more bytes each)
+constexpr int kBwdHeads = 4;  // heads of a token that a group takes, backward
 
 // E elements as loaded: words of two bf16 or one fp32.
 template <bool kF32, int E>
@@ -102,8 +106,8 @@ __device__ __forceinline__ float group_sum(float x) {
 // One block: kThreads / LG tokens of one head chunk. The chunks of q, then k,
 // then v run fastest over the grid, so that blocks that run together read whole
 // rows of a fused projection.
-template <bool kIn32, bool kOut32, int E, int LG>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const QkRopeParams p, int nq,
+template <bool kIn32, bool kOut32, int E, int LG, int kHeads>
+__global__ void __launch_bounds__(kThreads, kHeads > 4 ? 2 : 3) qk_norm_rope_kernel(const QkRopeParams p, int nq,
                                                                 int nk, int nch) {
   const int chunk = blockIdx.x % nch;
   const int token = blockIdx.x / nch * (kThreads / LG) + threadIdx.x / LG;
@@ -366,8 +370,8 @@ int lanes_for(int D, int E) {
   return lg;
 }
 
-template <bool kIn32, bool kOut32, int E>
-cudaError_t launch_fwd_e(const QkRopeParams& p, cudaStream_t stream) {
+template <bool kIn32, bool kOut32, int E, int kHeads>
+cudaError_t launch_fwd_h(const QkRopeParams& p, cudaStream_t stream) {
   const int nq = (p.H + kHeads - 1) / kHeads, nk = (p.Hkv + kHeads - 1) / kHeads;
   const int LG = lanes_for(p.D, E);
   const int groups = kThreads / LG;
@@ -375,57 +379,52 @@ cudaError_t launch_fwd_e(const QkRopeParams& p, cudaStream_t stream) {
   const int grid = (p.B * p.S + groups - 1) / groups * nch;
   if constexpr (E == 4) {
     if (LG == 16)
-      qk_norm_rope_kernel<kIn32, kOut32, E, 16><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
+      qk_norm_rope_kernel<kIn32, kOut32, E, 16, kHeads><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   }
   if (LG == 8)
-    qk_norm_rope_kernel<kIn32, kOut32, E, 8><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
+    qk_norm_rope_kernel<kIn32, kOut32, E, 8, kHeads><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   else if (LG == 4)
-    qk_norm_rope_kernel<kIn32, kOut32, E, 4><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
+    qk_norm_rope_kernel<kIn32, kOut32, E, 4, kHeads><<<grid, kThreads, 0, stream>>>(p, nq, nk, nch);
   return cudaGetLastError();
 }
 
-// 16-byte loads of bf16 need halves of a multiple of eight elements.
+// 16-byte loads of bf16 need halves of a multiple of eight elements. Eight
+// heads a group where they leave none over and the blocks still fill the card
+// (8 x 4096 tokens, 16 + 16 heads: 86 us against 91 with four; 16 + 4 heads: 34
+// against 32).
 template <bool kIn32, bool kOut32>
 cudaError_t launch_fwd(const QkRopeParams& p, cudaStream_t stream) {
   if constexpr (!kIn32) {
-    if (p.D % 16 == 0) return launch_fwd_e<kIn32, kOut32, 8>(p, stream);
+    if (p.D % 16 == 0) {
+      const long long groups8 = (long long)p.B * p.S * ((p.H + p.Hkv) / 8);
+      if (p.H % 8 == 0 && p.Hkv % 8 == 0 && groups8 >= 1 << 15)
+        return launch_fwd_h<kIn32, kOut32, 8, 8>(p, stream);
+      return launch_fwd_h<kIn32, kOut32, 8, 4>(p, stream);
+    }
   }
-  return launch_fwd_e<kIn32, kOut32, 4>(p, stream);
+  return launch_fwd_h<kIn32, kOut32, 4, 4>(p, stream);
 }
-
-bool bwd_wide(int D, bool in32, bool grad32) { return D % 16 == 0 && !(in32 && grad32); }
 
 // q's share of the backward's blocks, in proportion to the heads.
 int bwd_q_blocks(int n_blocks, int H, int Hkv) {
   return std::max(1, std::min(n_blocks - 1, (int)((long long)n_blocks * H / (H + Hkv))));
 }
 
-template <bool kIn32, bool kGrad32, bool kOut32, int E>
-cudaError_t launch_bwd_e(const QkRopeBwdParams& p, cudaStream_t stream) {
-  const int LG = lanes_for(p.D, E), blocks = p.n_blocks;
+template <bool kIn32, bool kGrad32, bool kOut32>
+cudaError_t launch_bwd(const QkRopeBwdParams& p, cudaStream_t stream) {
+  const int LG = lanes_for(p.D, 4), blocks = p.n_blocks;
   const int n_q = bwd_q_blocks(blocks, p.H, p.Hkv);
-  if constexpr (E == 4) {
-    if (LG == 16)
-      qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 16><<<blocks, kThreads, 0, stream>>>(p, n_q);
-  }
-  if (LG == 8)
-    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 8><<<blocks, kThreads, 0, stream>>>(p, n_q);
-  else if (LG == 4)
-    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, E, 4><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  if (LG == 16)
+    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 4, 16><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  else if (LG == 8)
+    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 4, 8><<<blocks, kThreads, 0, stream>>>(p, n_q);
+  else
+    qk_norm_rope_bwd_kernel<kIn32, kGrad32, kOut32, 4, 4><<<blocks, kThreads, 0, stream>>>(p, n_q);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !p.w[0]) return e;
   qk_norm_dw_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, stream>>>(p.partial, n_q, blocks, p.D,
                                                                  p.dw[0], p.dw[1]);
   return cudaGetLastError();
-}
-
-template <bool kIn32, bool kGrad32, bool kOut32>
-cudaError_t launch_bwd(const QkRopeBwdParams& p, cudaStream_t stream) {
-  if constexpr (!(kIn32 && kGrad32)) {
-    if (bwd_wide(p.D, kIn32, kGrad32))
-      return launch_bwd_e<kIn32, kGrad32, kOut32, 8>(p, stream);
-  }
-  return launch_bwd_e<kIn32, kGrad32, kOut32, 4>(p, stream);
 }
 
 }  // namespace qkr
