@@ -16,14 +16,18 @@
 // probabilities in shared or tensor memory for no gain.
 //
 // Work: a sequence's visible positions are cut into tiles of 16 keys a warp;
-// tiles are numbered sequence by sequence, kv head by kv head, and every block
-// takes an equal run of them (the lengths are read on the device). A block
-// walks its run with the loads of the next tiles in flight (cp.async, row
-// addresses from the block table one tile further ahead), whatever sequence
-// they belong to. Where a (sequence, head group) ends inside its run and began
-// there too, the block writes the output; a part of one goes to the workspace
-// and the last block to finish joins all parts in a fixed order, so the result
-// does not depend on timing.
+// tiles are numbered sequence by sequence, head group by head group, and every
+// block takes an equal run of them (the lengths are read on the device). One
+// or two warps of a block only load: they walk the run through a ring of stages
+// with cp.async, which takes pages of any size, alignment and order, and leave
+// with each tile a note of whose it is and which keys exist. The other warps
+// wait for a stage, compute and hand it back, each at its own pace. (With the
+// loads issued by the computing warps and a block barrier a tile, every
+// instruction of the address work added to the time: 286 us against 250 for 64
+// sequences of up to 8192.) Where a (sequence, head group) ends inside its run
+// and began there too, the block writes the output; a part of one goes to the
+// workspace and the last block to finish joins all parts in a fixed order, so
+// the result does not depend on timing.
 //
 // Precision: scores, softmax and sums in fp32. bf16: products of bf16 inputs
 // are exact; the probabilities are split into two bf16 parts (16 bits of
@@ -42,6 +46,7 @@ namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kSite = 70;  // of this file's waits in the device error word
 
 // The visible positions of a sequence of length L as one index range:
 // index i < n_sink is position i, the others lie `gap` further.
@@ -58,27 +63,34 @@ __device__ __forceinline__ Visible visible_of(int L, int window, int sinks) {
   return v;
 }
 
+constexpr int kLens = 256;  // sequence lengths kept in shared memory
+
 // Kernel shapes: D is the padded head dim, NT column tiles of 8 heads per item,
-// NW warps. Stages are filled while the block works on one.
-template <int D_, bool kF32_, int NT_, int NW_>
+// NW computing warps, S stages.
+template <int D_, bool kF32_, int NT_, int NW_, int S_>
 struct Cfg {
-  static constexpr int D = D_, NT = NT_, NW = NW_;
+  static constexpr int D = D_, NT = NT_, NW = NW_, S = S_;
   static constexpr bool kF32 = kF32_;
-  static constexpr int kThreads = NW * 32;
   static constexpr int kKeys = NW * 16;  // keys of a tile
+  static constexpr int NP = kKeys / 32;  // loading warps, a key a lane
+  static constexpr int kThreads = (NW + NP) * 32;
   static constexpr int kEsz = kF32 ? 4 : 2;
   static constexpr int kRow = D * kEsz;  // bytes of a row in shared memory
   static constexpr int kTile = kKeys * kRow;
   static constexpr int kStage = 2 * kTile;  // K, then V
-  static constexpr int kStages = kStage > 16384 ? 3 : 4;
-  static constexpr int kRing = kStages + 1;  // row-address slots
   static constexpr int kMerge = (NW - 1) * 8 * D * 4;
-  static constexpr int kOffMerge = kStages * kStage;
-  static constexpr int kOffRows = kOffMerge + kMerge;
-  static constexpr int kSmem = kOffRows + kRing * kKeys * 8;
-  static constexpr int kPerSm = (227 * 1024) / (kSmem + 2048);  // blocks a SM
-  static constexpr int kSlot = NT * 8 * D + NT * 16;            // floats of one part
-  static constexpr int kRegs = D / 16 * 4;                      // accumulators of a column tile
+  static constexpr int kSmem = S * kStage + kMerge;
+  static constexpr int kStatic = kLens * 4 + S * 64 + 768;           // at most
+  static constexpr int kFit = 228 * 1024 / (kSmem + kStatic + 1024);
+  static constexpr int kPerSm = NT > 1 && kFit > 2 ? 2 : kFit;  // blocks a SM (registers)
+  static constexpr int kSlot = NT * 8 * D + NT * 16;                 // floats of one part
+  static constexpr int kRegs = D / 16 * 4;  // accumulators of a column tile
+};
+
+// What the loading warps say about a stage's tile.
+struct Note {
+  uint32_t ok[2];  // bit k: key k exists
+  int b, sub, t, nt, L, n_sink, gap, n_keys;
 };
 
 // Partial results never take more than this per SM (the counters follow them
@@ -90,10 +102,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
                "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on the barrier when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -138,18 +150,18 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
   return f;
 }
 
-// x = hi + lo with hi of tf32's 11 bits; lo's own tail past them is dropped by
-// the product.
+// x = hi + lo with hi the upper 11 bits (tf32); lo's own tail past 11 bits is
+// dropped by the product. Cutting takes one logic instruction where rounding
+// takes a conversion at a quarter of the rate.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  hi = __float_as_uint(x) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // x = hi + lo + rest, exact: a probability of one returns its value unchanged.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo, uint32_t& rest) {
-  float left;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  left = x - __uint_as_float(hi);
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(left));
+  hi = __float_as_uint(x) & 0xffffe000u;
+  const float left = x - __uint_as_float(hi);
+  lo = __float_as_uint(left) & 0xffffe000u;
   rest = __float_as_uint(left - __uint_as_float(lo));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -173,13 +185,26 @@ struct Walker {
   Visible vis;
 };
 
+struct Block {  // shared by a block's warps
+  int lens[kLens];  // lengths of sequences [lens_b, lens_b + kLens)
+  uint64_t full[4], empty[4];
+  Note note[4];
+  long long scan[8];
+  int b, rest;  // where the run starts
+  int last;
+  int abort;  // a wait ran out: the others stop waiting
+  float m[4][16], l[4][16];
+};
+
 template <class C>
 struct Decoder {
   const PagedDecodeParams& p;
+  Block& sh;
   uint8_t* smem;
   uint32_t sbase;
-  int G, HB, SUB;
+  int G, HB, SUB;  // heads a group, head blocks a group, head blocks in all
   int lane, warp, r, q;
+  int lens_b;
 
   // Softmax state of the warp: heads 8 nt + 2q (+1) of the item, this lane's
   // share of the sums; O^T fragments (rows: dims, columns: heads).
@@ -187,14 +212,19 @@ struct Decoder {
   // Q^T fragments.
   uint32_t qf[C::NT][C::D / 16][C::kF32 ? 8 : 2];
 
-  __device__ int length(int b) const {
+  __device__ int read_length(int b) const {
     int L = p.lens[b];
     const long long most = (long long)p.max_pages * p.page_size;
     if (L > most) L = (int)most;
     return max(L, 0);
   }
+  __device__ int length(int b) const {
+    const int at = b - lens_b;
+    return at >= 0 && at < kLens ? sh.lens[at] : read_length(b);
+  }
   __device__ __forceinline__ int tiles_of(int n) const { return (n + C::kKeys - 1) / C::kKeys; }
 
+  // ------------------------------------------------------- loading warps
   __device__ void enter(Walker& w, int b) const {
     w.b = b;
     w.L = length(b);
@@ -211,63 +241,101 @@ struct Decoder {
     if (b < p.B) enter(w, b);
   }
 
-  // Element offset of key `key` of the walker's tile in the pools, or -1 for
-  // none (past the end, or a page outside the pool).
-  __device__ long long row_offset(const Walker& w, int key) const {
+  // A key's row in the pools: the page number as read (whose latency passes
+  // while the tile before is loaded), then the address.
+  struct Key {
+    int page, slot;  // slot < 0: past the end
+  };
+  __device__ __forceinline__ Key find_key(const Walker& w, int key) const {
+    Key k{0, -1};
     const int i = w.t * C::kKeys + key;
-    if (i >= w.vis.n) return -1;
-    const int j = i < w.vis.n_sink ? i : i + w.vis.gap;
-    const int col = j / p.page_size;
-    const int page = p.table[w.b * p.t_sb + col];
-    if (page < 0 || page >= p.n_pages) {
-      report_error(kDevBadIndex, w.b);
-      return -1;
+    if (i < w.vis.n) {
+      const int j = i < w.vis.n_sink ? i : i + w.vis.gap;
+      const int col = j / p.page_size;
+      k.slot = j - col * p.page_size;
+      k.page = p.table[w.b * p.t_sb + col];
     }
-    return page * p.p_sp + (w.sub / HB) * p.p_sh + (j - col * p.page_size) * p.p_ss;
-  }
-  __device__ __forceinline__ long long* rows(int slot) const {
-    return reinterpret_cast<long long*>(smem + C::kOffRows) + slot * C::kKeys;
+    return k;
   }
 
-  // Starts the loads of one tile.
-  __device__ __forceinline__ void load_tile(int stage, int slot) const {
-    constexpr int kChunks = C::kRow / 16;
-    constexpr int kRows = C::kThreads / kChunks;  // rows a pass
-    const int chunk = threadIdx.x % kChunks;
+  __device__ void load_run(const Walker& start, int n) {
+    constexpr int kChunks = C::kRow / 16, kRows = 32 / kChunks;  // rows a pass
+    const int pw = warp - C::NW;
+    const int chunk = lane % kChunks, sub_row = lane / kChunks;
     const bool real = chunk * 16 < p.D * C::kEsz;
-    const uint32_t dst = sbase + stage * C::kStage;
-    const uint8_t* k = reinterpret_cast<const uint8_t*>(p.k);
-    const uint8_t* v = reinterpret_cast<const uint8_t*>(p.v);
-#pragma unroll
-    for (int i = 0; i < C::kKeys / kRows; ++i) {
-      const int row = threadIdx.x / kChunks + i * kRows;
-      const long long off = rows(slot)[row];
-      const int bytes = real && off >= 0 ? 16 : 0;
-      const long long e = bytes ? off * C::kEsz + chunk * 16 : 0;
-      const uint32_t at = dst + place<C>(row, chunk);
-      cp_async16(at, k + e, bytes);
-      cp_async16(at + C::kTile, v + e, bytes);
+    const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k) + chunk * 16;
+    const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + chunk * 16;
+    Walker w = start;
+    Key next = find_key(w, pw * 32 + lane);
+    for (int i = 0; i < n; ++i) {
+      const Walker now = w;
+      const Key key = next;
+      if (i + 1 < n) {
+        advance(w);
+        next = find_key(w, pw * 32 + lane);
+      }
+      const int stage = i % C::S;
+      if (i >= C::S) mbar_wait(&sh.empty[stage], (i / C::S - 1) & 1, &sh.abort, kSite);
+      // Byte offset of this lane's key, or -1 for none or a page outside the
+      // pool (which counts as masked).
+      long long off = -1;
+      if (key.slot >= 0) {
+        if (key.page < 0 || key.page >= p.n_pages)
+          report_error(kDevBadIndex, now.b);
+        else
+          off = (key.page * p.p_sp + (now.sub / HB) * p.p_sh + key.slot * p.p_ss) * C::kEsz;
+      }
+      const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+      const int n_keys = min(C::kKeys, now.vis.n - now.t * C::kKeys);
+      const uint32_t dst = sbase + stage * C::kStage;
+      // Rows of warps without keys stay as they are: those skip the tile.
+      const int passes = min(32, (n_keys + 15) / 16 * 16 - pw * 32) / kRows;
+#pragma unroll 4
+      for (int s = 0; s < passes; ++s) {
+        const int row = s * kRows + sub_row;
+        const long long o = __shfl_sync(0xffffffffu, off, row);
+        const int bytes = real && o >= 0 ? 16 : 0;
+        const long long e = bytes ? o : -chunk * 16;
+        const uint32_t at = dst + place<C>(pw * 32 + row, chunk);
+        cp_async16(at, kb + e, bytes);
+        cp_async16(at + C::kTile, vb + e, bytes);
+      }
+      cp_arrive(&sh.full[stage]);
+      if (lane == 0) {
+        Note& note = sh.note[stage];
+        note.ok[pw] = ok;
+        if (pw == 0) {
+          note.b = now.b, note.sub = now.sub, note.t = now.t, note.nt = now.nt;
+          note.L = now.L, note.n_sink = now.vis.n_sink, note.gap = now.vis.gap;
+          note.n_keys = n_keys;
+        }
+        mbar_arrive(&sh.full[stage]);
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
-  __device__ int heads_of(const Walker& w) const {  // real heads of the item
+  // ----------------------------------------------------- computing warps
+  __device__ __forceinline__ void sync_warps() const { named_bar_sync(1, C::NW * 32); }
+
+  __device__ int heads_of(const Note& w) const {  // real heads of the item
     return min(C::NT * 8, G - (w.sub % HB) * (C::NT * 8));
   }
-  __device__ int first_head(const Walker& w) const {
+  __device__ int first_head(const Note& w) const {
     return (w.sub / HB) * G + (w.sub % HB) * (C::NT * 8);
   }
 
-  __device__ void begin_item(const Walker& w) {
+  __device__ void begin_item(const Note& w) {
     const int n = heads_of(w);
+    const long long q0 = w.b * p.q_sb + first_head(w) * p.q_sh;
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < C::kRegs / 4; ++i)
-        o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+      for (int i = 0; i < C::kRegs; ++i) o[nt][i / 4][i % 4] = 0.0f;
       const int h = nt * 8 + r;  // this lane's column
-      const long long e = w.b * p.q_sb + (first_head(w) + h) * p.q_sh;
+      const long long e = q0 + h * p.q_sh;
 #pragma unroll
       for (int ks = 0; ks < C::D / 16; ++ks) {
         if constexpr (C::kF32) {
@@ -431,12 +499,12 @@ struct Decoder {
     }
   }
 
-  __device__ __forceinline__ void tile(const Walker& w, int stage, int slot) {
+  __device__ __forceinline__ void tile(const Note& w, int stage) {
     const uint32_t kbase = sbase + stage * C::kStage;
     float s[C::NT][4];
     scores(kbase, s);
-    const int key = warp * 16 + r;
-    const bool ok0 = rows(slot)[key] >= 0, ok1 = rows(slot)[key + 8] >= 0;
+    const int key = warp * 16 + r;  // this lane's keys: key and key + 8
+    const uint32_t ok = w.ok[C::NP > 1 ? warp / 2 : 0] >> (key & 31);
     float mx[C::NT][2];
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
@@ -448,12 +516,12 @@ struct Decoder {
         for (int i = 0; i < 4; ++i) {
           const int h = nt * 8 + 2 * q + i % 2;
           const int idx = w.t * C::kKeys + key + i / 2 * 8;
-          const int j = idx < w.vis.n_sink ? idx : idx + w.vis.gap;
+          const int j = idx < w.n_sink ? idx : idx + w.gap;
           if (h < n) s[nt][i] -= p.alibi[h0 + h] * kLog2e * (float)(w.L - 1 - j);
         }
       }
-      if (!ok0) s[nt][0] = s[nt][1] = -INFINITY;
-      if (!ok1) s[nt][2] = s[nt][3] = -INFINITY;
+      if (!(ok & 1)) s[nt][0] = s[nt][1] = -INFINITY;
+      if (!(ok & 256)) s[nt][2] = s[nt][3] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float x = fmaxf(s[nt][i], s[nt][i + 2]);
@@ -474,54 +542,58 @@ struct Decoder {
     accumulate(kbase + C::kTile, s);
   }
 
-  // Sums the lanes' shares of l, then joins the warps' states into warp 0's.
-  __device__ void join_warps() {
-    float* buf = reinterpret_cast<float*>(smem + C::kOffMerge);
-    __shared__ float sm[C::NW][C::NT * 8], sl[C::NW][C::NT * 8];
-#pragma unroll
-    for (int nt = 0; nt < C::NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1)
-          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], off);
-        if (r == 0) sm[warp][nt * 8 + 2 * q + i] = m[nt][i], sl[warp][nt * 8 + 2 * q + i] = l[nt][i];
-      }
-    __syncthreads();
-    float top[C::NT][2];
-#pragma unroll
-    for (int nt = 0; nt < C::NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[nt][i] = m[nt][i];
-#pragma unroll
-        for (int w = 0; w < C::NW; ++w)
-          top[nt][i] = fmaxf(top[nt][i], sm[w][nt * 8 + 2 * q + i]);
-      }
-    raise(top);
-    if (warp == 0) {
+  // Sums the lanes' shares of l, then joins the states of the first n warps,
+  // the others having none, into warp 0's.
+  __device__ void join_warps(int n) {
+    float* buf = reinterpret_cast<float*>(smem + C::S * C::kStage);
+    if (warp < n) {
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int w = 1; w < C::NW; ++w) {
-            const int h = nt * 8 + 2 * q + i;
-            if (sm[w][h] > -INFINITY) l[nt][i] += sl[w][h] * fast_exp2(sm[w][h] - m[nt][i]);
+          for (int off = 4; off < 32; off <<= 1)
+            l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], off);
+          if (r == 0) {
+            sh.m[warp][nt * 8 + 2 * q + i] = m[nt][i];
+            sh.l[warp][nt * 8 + 2 * q + i] = l[nt][i];
           }
+        }
+    }
+    if (n == 1) return;
+    sync_warps();
+    if (warp < n) {
+      float top[C::NT][2];
+#pragma unroll
+      for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[nt][i] = m[nt][i];
+          for (int w = 0; w < n; ++w) top[nt][i] = fmaxf(top[nt][i], sh.m[w][nt * 8 + 2 * q + i]);
+        }
+      raise(top);
+      if (warp == 0) {
+#pragma unroll
+        for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            for (int w = 1; w < n; ++w) {
+              const int h = nt * 8 + 2 * q + i;
+              if (sh.m[w][h] > -INFINITY) l[nt][i] += sh.l[w][h] * fast_exp2(sh.m[w][h] - m[nt][i]);
+            }
+      }
     }
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
-      if (nt > 0) __syncthreads();
-      if (warp > 0) {
+      if (nt > 0) sync_warps();
+      if (warp > 0 && warp < n) {
 #pragma unroll
         for (int i = 0; i < C::kRegs; ++i)
           buf[((warp - 1) * C::kRegs + i) * 32 + lane] = o[nt][i / 4][i % 4];
       }
-      __syncthreads();
+      sync_warps();
       if (warp == 0) {
-#pragma unroll
-        for (int w = 0; w < C::NW - 1; ++w)
+        for (int w = 0; w < n - 1; ++w)
 #pragma unroll
           for (int i = 0; i < C::kRegs; ++i)
             o[nt][i / 4][i % 4] += buf[(w * C::kRegs + i) * 32 + lane];
@@ -535,7 +607,7 @@ struct Decoder {
     return C::kF32 ? tile / 2 * 32 + r * 4 + tile % 2 * 2 + second : tile * 16 + second * 8 + r;
   }
 
-  __device__ void write_output(const Walker& w) const {  // warp 0
+  __device__ void write_output(const Note& w) const {  // warp 0
     const int n = heads_of(w);
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt)
@@ -609,13 +681,13 @@ struct Decoder {
     }
   }
 
-  // The walker's item ends with this tile, or the block's run does. g: the
-  // tile's number among all T; the block's run starts at `first`.
-  // Block c of n takes tiles [c T / n, (c + 1) T / n).
-  __device__ void end_segment(const Walker& w, long long g, long long first, long long T,
+  // The note's item ends with this tile, or the block's run does. g: the
+  // tile's number among all T; block c of n takes tiles [c T / n, (c + 1) T / n)
+  // and this one's run starts at `first`.
+  __device__ void end_segment(const Note& w, long long g, long long first, long long T,
                               long long n) {
-    __shared__ int last;
-    join_warps();
+    // A segment of one tile may leave warps without keys.
+    join_warps(w.t > 0 && g > first ? C::NW : min(C::NW, (w.n_keys + 15) / 16));
     const long long a = g - w.t, z = a + w.nt;  // the item's tiles
     if (first <= a && g == z - 1) {
       if (warp == 0) write_output(w);
@@ -630,13 +702,17 @@ struct Decoder {
       __threadfence();
       __syncwarp();
       if (lane == 0) {
-        last = atomicAdd(count, 1) == (int)(c1 - c0);
+        const bool last = atomicAdd(count, 1) == (int)(c1 - c0);
         if (last) *count = 0;  // for the next call
         __threadfence();
+        sh.last = last;
       }
     }
-    __syncthreads();
-    if (!last) return;
+    sync_warps();
+    if (!sh.last) {
+      sync_warps();  // read by all before the next one is written
+      return;
+    }
     // The warps share the parts, each in ascending order.
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
@@ -647,21 +723,41 @@ struct Decoder {
     }
     for (long long c = c0 + warp; c <= c1; c += C::NW)
       add_part(slot_of(c, c * T / n >= a ? 0 : 1));
-    join_warps();
+    join_warps((int)min((long long)C::NW, c1 - c0 + 1));
     if (warp == 0) write_output(w);
   }
 
+  __device__ void compute_run(long long first, int n, long long T, long long blocks) {
+    for (int i = 0; i < n; ++i) {
+      const int stage = i % C::S;
+      mbar_wait(&sh.full[stage], (i / C::S) & 1, &sh.abort, kSite + 1);
+      const Note w = sh.note[stage];
+      if (i == 0 || w.t == 0) begin_item(w);
+      if (warp * 16 < w.n_keys) tile(w, stage);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+      if (w.t == w.nt - 1 || i == n - 1) end_segment(w, first + i, first, T, blocks);
+    }
+  }
+
   __device__ void run() {
-    constexpr int S = C::kStages;
     const int tid = threadIdx.x;
+    constexpr int kWarps = C::NW + C::NP;
+    if (tid == 0) {
+      for (int s = 0; s < C::S; ++s) {
+        mbar_init(&sh.full[s], C::NP * 33);  // each loading lane's copies, and its warp's note
+        mbar_init(&sh.empty[s], C::NW);
+      }
+      sh.abort = 0;
+      fence_barrier_init();
+    }
     // Every sequence's tiles: this thread's stretch of sequences, then a scan.
-    __shared__ long long scan[C::NW];
-    __shared__ int s_b, s_rest;
     const int per = (p.B + C::kThreads - 1) / C::kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     long long mine = 0;
     for (int b = b0; b < b1; ++b) {
-      const int L = length(b);
+      const int L = read_length(b);
+      if (b < kLens) sh.lens[b] = L;
       if (blockIdx.x == 0 && p.lens[b] > L) report_error(kDevBadIndex, b);
       mine += tiles_of(visible_of(L, p.window, p.sinks).n);
     }
@@ -671,13 +767,14 @@ struct Decoder {
       const long long y = __shfl_up_sync(0xffffffffu, inc, off);
       if (lane >= off) inc += y;
     }
-    if (lane == 31) scan[warp] = inc;
+    if (lane == 31) sh.scan[warp] = inc;
     __syncthreads();
+    lens_b = 0;
     long long before = 0, T = 0;
 #pragma unroll
-    for (int w = 0; w < C::NW; ++w) {
-      if (w < warp) before += scan[w];
-      T += scan[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.scan[w];
+      T += sh.scan[w];
     }
     before += inc - mine;
     // Sequences without a visible position: a zero output.
@@ -707,54 +804,34 @@ struct Decoder {
         if (first < (run + nt) * SUB) break;
         run += nt;
       }
-      s_b = b;
-      s_rest = (int)(first - run * SUB);
+      sh.b = b;
+      sh.rest = (int)(first - run * SUB);
     }
     __syncthreads();
-    Walker ahead, here;
-    enter(ahead, s_b);
-    ahead.sub = s_rest / ahead.nt;
-    ahead.t = s_rest % ahead.nt;
-    here = ahead;
-
-    // Row addresses of the first S tiles, loads of the first S - 1.
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-      if (i < n) {
-        if (tid < C::kKeys) rows(i)[tid] = row_offset(ahead, tid);
-        advance(ahead);
-      }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) {
-      if (i < n) load_tile(i, i);
-      cp_commit();
-    }
-    begin_item(here);
-    for (int i = 0; i < n; ++i) {
-      cp_wait<S - 2>();
+    if (p.B > kLens) {  // keep the lengths that this run meets first
+      const int b = sh.b;
+      for (int i = tid; i < kLens && b + i < p.B; i += C::kThreads)
+        sh.lens[i] = read_length(b + i);
+      lens_b = b;
       __syncthreads();
-      if (i + S - 1 < n) load_tile((i + S - 1) % S, (i + S - 1) % C::kRing);
-      cp_commit();
-      long long next = -1;
-      const bool more = i + S < n;
-      if (more && tid < C::kKeys) next = row_offset(ahead, tid);
-      tile(here, i % S, i % C::kRing);
-      if (more) {
-        if (tid < C::kKeys) rows((i + S) % C::kRing)[tid] = next;
-        advance(ahead);
-      }
-      if (here.t == here.nt - 1 || i == n - 1) end_segment(here, first + i, first, T, blocks);
-      advance(here);
-      if (here.t == 0 && i + 1 < n) begin_item(here);
+    }
+    if (warp >= C::NW) {
+      Walker w;
+      enter(w, sh.b);
+      w.sub = sh.rest / w.nt;
+      w.t = sh.rest % w.nt;
+      load_run(w, n);
+    } else {
+      compute_run(first, n, T, blocks);
     }
   }
 };
 
 template <class C>
-__global__ void __launch_bounds__(C::kThreads) paged_kernel(const PagedDecodeParams p) {
+__global__ void __launch_bounds__(C::kThreads, C::kPerSm) paged_kernel(const PagedDecodeParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  Decoder<C> d{p};
+  __shared__ Block sh;
+  Decoder<C> d{p, sh};
   d.smem = smem;
   d.sbase = smem_u32(smem);
   d.G = p.H / p.Hkv;
@@ -770,7 +847,7 @@ __global__ void __launch_bounds__(C::kThreads) paged_kernel(const PagedDecodePar
 template <class C>
 cudaError_t launch(const PagedDecodeParams& p, cudaStream_t stream) {
   static_assert(C::kPerSm * 2 * C::kSlot * 4 <= kPartBytesPerSm, "parts fit the workspace");
-  static_assert(C::kPerSm >= 1, "a block fits an SM");
+  static_assert(C::kPerSm >= 1 && sizeof(Block) <= C::kStatic && C::S <= 4, "a block fits an SM");
   const int G = p.H / p.Hkv;
   const long long most = std::min<long long>((long long)p.max_pages * p.page_size, 0x7fffffff);
   const long long tiles = (long long)p.B * p.Hkv * ((G + C::NT * 8 - 1) / (C::NT * 8)) *
@@ -803,12 +880,13 @@ cudaError_t launch_paged_decode(const PagedDecodeParams& p, cudaStream_t stream)
   using namespace paged;
   const bool wide = p.H / p.Hkv > 8;  // more than one column tile
   if (p.in_fp32)
-    return p.D > 64 ? launch<Cfg<128, true, 1, 2>>(p, stream)
-                    : launch<Cfg<64, true, 1, 4>>(p, stream);
+    return p.D > 64 ? launch<Cfg<128, true, 1, 2, 3>>(p, stream)
+                    : launch<Cfg<64, true, 1, 4, 3>>(p, stream);
   if (p.D > 64)
-    return wide ? launch<Cfg<128, false, 2, 4>>(p, stream)
-                : launch<Cfg<128, false, 1, 4>>(p, stream);
-  return wide ? launch<Cfg<64, false, 2, 4>>(p, stream) : launch<Cfg<64, false, 1, 4>>(p, stream);
+    return wide ? launch<Cfg<128, false, 2, 4, 3>>(p, stream)
+                : launch<Cfg<128, false, 1, 4, 3>>(p, stream);
+  return wide ? launch<Cfg<64, false, 2, 4, 4>>(p, stream)
+              : launch<Cfg<64, false, 1, 4, 4>>(p, stream);
 }
 
 }  // namespace enl
