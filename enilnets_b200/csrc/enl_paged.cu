@@ -23,11 +23,12 @@
 // with each tile a note of whose it is and which keys exist. The other warps
 // wait for a stage, compute and hand it back, each at its own pace. (With the
 // loads issued by the computing warps and a block barrier a tile, every
-// instruction of the address work added to the time: 286 us against 250 for 64
-// sequences of up to 8192.) Where a (sequence, head group) ends inside its run
+// instruction of the address work added to the time: 287 us against 244 for 64
+// sequences of 6144.) Where a (sequence, head group) ends inside its run
 // and began there too, the block writes the output; a part of one goes to the
 // workspace and the last block to finish joins all parts in a fixed order, so
-// the result does not depend on timing.
+// the result does not depend on timing. Short sequences (up to kWholeTiles
+// tiles) are not divided: joining two parts costs about four tiles' time.
 //
 // Precision: scores, softmax and sums in fp32. bf16: products of bf16 inputs
 // are exact; the probabilities are split into two bf16 parts (16 bits of
@@ -64,6 +65,7 @@ __device__ __forceinline__ Visible visible_of(int L, int window, int sinks) {
 }
 
 constexpr int kLens = 256;  // sequence lengths kept in shared memory
+constexpr int kWholeTiles = 6;
 
 // Kernel shapes: D is the padded head dim, NT column tiles of 8 heads per item,
 // NW computing warps, S stages.
@@ -190,6 +192,7 @@ struct Block {  // shared by a block's warps
   uint64_t full[4], empty[4];
   Note note[4];
   long long scan[8];
+  int longest[8];
   int b, rest;  // where the run starts
   int last;
   int abort;  // a wait ran out: the others stop waiting
@@ -681,24 +684,38 @@ struct Decoder {
     }
   }
 
-  // The note's item ends with this tile, or the block's run does. g: the
-  // tile's number among all T; block c of n takes tiles [c T / n, (c + 1) T / n)
-  // and this one's run starts at `first`.
-  __device__ void end_segment(const Note& w, long long g, long long first, long long T,
-                              long long n) {
+  // How the tiles are shared out: block c of n takes tiles [c T / n, (c + 1) T / n);
+  // this one's run starts at `first`. Whole: runs of whole items instead.
+  struct Share {
+    long long first, T, n;
+    bool whole;
+
+    // x / y of values whose product fits: 32-bit where possible, since parts are
+    // joined by few threads at the end of a call.
+    static __device__ __forceinline__ long long quot(long long x, long long y) {
+      return x >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
+    }
+    __device__ __forceinline__ long long begin(long long c) const { return quot(c * T, n); }
+    __device__ __forceinline__ long long block_of(long long t) const {
+      return quot((t + 1) * n - 1, T);
+    }
+  };
+
+  // The note's item ends with this tile, or the block's run does. g: the tile's
+  // number among all.
+  __device__ void end_segment(const Note& w, long long g, const Share& share) {
     // A segment of one tile may leave warps without keys.
-    join_warps(w.t > 0 && g > first ? C::NW : min(C::NW, (w.n_keys + 15) / 16));
+    join_warps(w.t > 0 && g > share.first ? C::NW : min(C::NW, (w.n_keys + 15) / 16));
     const long long a = g - w.t, z = a + w.nt;  // the item's tiles
-    if (first <= a && g == z - 1) {
+    if (share.whole || (share.first <= a && g == z - 1)) {
       if (warp == 0) write_output(w);
       return;
     }
-    auto block_of = [&](long long t) { return ((t + 1) * n - 1) / T; };
-    const long long c0 = block_of(a), c1 = block_of(z - 1);
+    const long long c0 = share.block_of(a), c1 = share.block_of(z - 1);
     int* count = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(p.workspace) +
                                         p.n_sms * kPartBytesPerSm) + (w.b * SUB + w.sub);
     if (warp == 0) {
-      write_part(slot_of(blockIdx.x, first >= a ? 0 : 1));
+      write_part(slot_of(blockIdx.x, share.first >= a ? 0 : 1));
       __threadfence();
       __syncwarp();
       if (lane == 0) {
@@ -722,12 +739,12 @@ struct Decoder {
       for (int i = 0; i < C::kRegs; ++i) o[nt][i / 4][i % 4] = 0.0f;
     }
     for (long long c = c0 + warp; c <= c1; c += C::NW)
-      add_part(slot_of(c, c * T / n >= a ? 0 : 1));
+      add_part(slot_of(c, share.begin(c) >= a ? 0 : 1));
     join_warps((int)min((long long)C::NW, c1 - c0 + 1));
     if (warp == 0) write_output(w);
   }
 
-  __device__ void compute_run(long long first, int n, long long T, long long blocks) {
+  __device__ void compute_run(const Share& share, int n) {
     for (int i = 0; i < n; ++i) {
       const int stage = i % C::S;
       mbar_wait(&sh.full[stage], (i / C::S) & 1, &sh.abort, kSite + 1);
@@ -736,7 +753,7 @@ struct Decoder {
       if (warp * 16 < w.n_keys) tile(w, stage);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.empty[stage]);
-      if (w.t == w.nt - 1 || i == n - 1) end_segment(w, first + i, first, T, blocks);
+      if (w.t == w.nt - 1 || i == n - 1) end_segment(w, share.first + i, share);
     }
   }
 
@@ -754,12 +771,17 @@ struct Decoder {
     // Every sequence's tiles: this thread's stretch of sequences, then a scan.
     const int per = (p.B + C::kThreads - 1) / C::kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+    // (tiles, and in the upper half sequences that have some)
+    constexpr long long kSeq = 1ll << 40;
     long long mine = 0;
+    int longest = 0;
     for (int b = b0; b < b1; ++b) {
       const int L = read_length(b);
       if (b < kLens) sh.lens[b] = L;
       if (blockIdx.x == 0 && p.lens[b] > L) report_error(kDevBadIndex, b);
-      mine += tiles_of(visible_of(L, p.window, p.sinks).n);
+      const int nt = tiles_of(visible_of(L, p.window, p.sinks).n);
+      mine += nt > 0 ? nt + kSeq : 0;
+      longest = max(longest, nt);
     }
     long long inc = mine;
 #pragma unroll
@@ -767,14 +789,16 @@ struct Decoder {
       const long long y = __shfl_up_sync(0xffffffffu, inc, off);
       if (lane >= off) inc += y;
     }
-    if (lane == 31) sh.scan[warp] = inc;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 31) sh.scan[warp] = inc, sh.longest[warp] = longest;
     __syncthreads();
     lens_b = 0;
-    long long before = 0, T = 0;
+    long long before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += sh.scan[w];
-      T += sh.scan[w];
+      all += sh.scan[w];
+      longest = max(longest, sh.longest[w]);
     }
     before += inc - mine;
     // Sequences without a visible position: a zero output.
@@ -789,23 +813,29 @@ struct Decoder {
             reinterpret_cast<__nv_bfloat16*>(p.o)[e] = __float2bfloat16_rn(0.0f);
           if (d == 0 && p.lse) p.lse[(long long)b * p.H + h] = -INFINITY;
         }
-    // No more blocks than tiles take part, so none of those has an empty run.
-    T *= SUB;
-    const long long blocks = min((long long)gridDim.x, T);
-    if (blockIdx.x >= blocks) return;
-    const long long first = blockIdx.x * T / blocks, end = (blockIdx.x + 1ll) * T / blocks;
-    const int n = (int)(end - first);
-    // The sequence that holds the run's first tile.
-    if (before * SUB <= first && first < (before + mine) * SUB) {
-      long long run = before;
+    // Units shared out: whole items, or tiles. No more blocks than units take
+    // part, so none of those has an empty run.
+    Share share;
+    const long long items = (all >> 40) * SUB;
+    share.whole = longest <= kWholeTiles && items <= 16ll * gridDim.x;
+    auto units = [&](long long x) { return (share.whole ? x >> 40 : x & (kSeq - 1)) * SUB; };
+    share.T = units(all);
+    share.n = min((long long)gridDim.x, share.T);
+    if (blockIdx.x >= share.n) return;
+    const long long first = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1ll);
+    share.first = share.whole ? 0 : first;
+    // The sequence that holds the run's first unit.
+    if (units(before) <= first && first < units(before + mine)) {
+      long long run = units(before);
       int b = b0;
       for (;; ++b) {
         const int nt = tiles_of(visible_of(length(b), p.window, p.sinks).n);
-        if (first < (run + nt) * SUB) break;
-        run += nt;
+        const long long u = (long long)(share.whole ? min(nt, 1) : nt) * SUB;
+        if (first < run + u) break;
+        run += u;
       }
       sh.b = b;
-      sh.rest = (int)(first - run * SUB);
+      sh.rest = (int)(first - run);
     }
     __syncthreads();
     if (p.B > kLens) {  // keep the lengths that this run meets first
@@ -815,15 +845,25 @@ struct Decoder {
       lens_b = b;
       __syncthreads();
     }
-    if (warp >= C::NW) {
-      Walker w;
-      enter(w, sh.b);
-      w.sub = sh.rest / w.nt;
-      w.t = sh.rest % w.nt;
-      load_run(w, n);
-    } else {
-      compute_run(first, n, T, blocks);
+    Walker w;
+    enter(w, sh.b);
+    w.sub = share.whole ? sh.rest : sh.rest / w.nt;
+    w.t = share.whole ? 0 : sh.rest % w.nt;
+    int n = (int)(end - first);  // tiles of the run
+    if (share.whole) {
+      Walker x = w;
+      int tiles = 0;
+      for (int i = 0; i < n; ++i) {
+        tiles += x.nt;
+        x.t = x.nt - 1;
+        advance(x);
+      }
+      n = tiles;
     }
+    if (warp >= C::NW)
+      load_run(w, n);
+    else
+      compute_run(share, n);
   }
 };
 
@@ -878,10 +918,16 @@ size_t paged_decode_workspace(int B, int H, int Hkv, int D, int n_sms) {
 
 cudaError_t launch_paged_decode(const PagedDecodeParams& p, cudaStream_t stream) {
   using namespace paged;
+  // Stages and warps, measured (us): fp32 spends longer on a tile, so more and
+  // smaller blocks serve it better. Heads of 128 (16 x 6144 keys, 8 kv heads,
+  // floor 123): 2 warps with 2 stages, 3 blocks a SM, 166; 3 stages, 2 blocks
+  // 182; 4 warps, 1 block 177. Heads of 64: 2 warps with 3 stages, 4 blocks, 142;
+  // 4 warps with 2 or 3 stages 145. bf16, heads of 128 (64 x 6144 keys, floor
+  // 246): 4 warps with 3 stages, 2 blocks, 244; with 2 stages, 3 blocks 259.
   const bool wide = p.H / p.Hkv > 8;  // more than one column tile
   if (p.in_fp32)
-    return p.D > 64 ? launch<Cfg<128, true, 1, 2, 3>>(p, stream)
-                    : launch<Cfg<64, true, 1, 4, 3>>(p, stream);
+    return p.D > 64 ? launch<Cfg<128, true, 1, 2, 2>>(p, stream)
+                    : launch<Cfg<64, true, 1, 2, 3>>(p, stream);
   if (p.D > 64)
     return wide ? launch<Cfg<128, false, 2, 4, 3>>(p, stream)
                 : launch<Cfg<128, false, 1, 4, 3>>(p, stream);
