@@ -19,11 +19,13 @@
 //    again. Their few candidates go to one list in shared memory, where they
 //    are ranked, and the rest of the row is never touched.
 //  * min-p alone: the same with the groups whose maximum weighs min_p or more.
-//  * top-p alone: one more pass for the exact total, then the same with about
-//    kNucleus groups, provided that their candidates carry the wanted mass.
-//  * larger top-k, flatter nuclei: a histogram of the logits finds the bin that
-//    the cut falls into, one pass sums what lies above it and collects the bin's
-//    tokens, which are sorted.
+//  * top-p alone: the groups whose maxima carry the wanted share of a total
+//    estimated from the maxima and one vector a thread, one more pass for the
+//    exact total, and the same list, provided that it carries the exact share.
+//  * larger top-k, flatter nuclei: a histogram of the logits (made together with
+//    the exact total) finds the bins around the cut; one pass sums what lies
+//    above them and lists their tokens. The cut and the draw follow from the list
+//    and the warps' sums.
 //  * rows that defeat the bins (thousands of equal logits at the cut): bisection
 //    over the composite, one pass per bit.
 // With temperature alone one pass sums the row in ranges and the range that
@@ -42,14 +44,15 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kGroups = 4;       // group maxima per thread
-constexpr int kCap = 2048;       // candidates that fit the shared-memory sort
+constexpr int kCap = 2048;       // candidates that fit the list
 constexpr int kSmallK = 1024;    // largest top-k of the group path
-constexpr int kNucleus = 512;    // groups asked for when only top-p cuts
-constexpr int kRank = 256;       // candidates that are ranked by counting, not sorted
+constexpr int kNucleus = 1200;   // most groups that a top-p list is made of
+constexpr int kRank = 256;       // entries that are ranked by counting
 constexpr int kMaxCluster = 8;
 constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
 constexpr float kOne = 1099511627776.0f;  // 2^40
+constexpr uint32_t kNoCut = ~0u;  // in place of a top-p share
 constexpr float kLive = 28.0f;   // weights below exp(-28) < 2^-40 are zero
 
 // Order-preserving bits of a float: a < b as floats iff key(a) < key(b).
@@ -191,6 +194,16 @@ struct Pair {
   u64 a, b;
 };
 
+// What a block knows about its row, for the paths that are functions of their
+// own: inlined they would take the common path's registers.
+struct Case {
+  const void* row;
+  int V, n_blocks, turn;
+  uint32_t rank;
+  float top, inv_t, min_p, least, u;
+  long long* token;
+};
+
 struct Shared {
   union {
     u64 list[kCap];  // candidates (composites)
@@ -199,18 +212,20 @@ struct Shared {
       float heavy[kBins];    // those above 2^-10 of the largest
     };
   };
-  union {
-    u64 order[kCap];  // kept candidates by index
-    u64 q[kCap];      // whole weights of the list's entries
-    u64 mass[kGroupBins];
-  };
+  u64 q[kRank];           // whole weights of entries that are ranked
+  u64 mass[kGroupBins];   // of the entries in select()'s bins
   u64 part[kWarps];
+  u64 wsum[kWarps * kMaxCluster];  // rank 0: kept weight of every warp's range
   float fpart[kWarps];
   Pair swap[2][kMaxCluster];  // what the cluster's blocks tell each other
-  uint32_t gbins[kGroupBins], gsum[kGroupBins];
-  int groups[kThreads * kGroups];  // first vectors of the groups to read again
-  u64 cut;  // composite found by rank 0
-  int count, found, n_groups;
+  uint32_t gbins[kGroupBins], gmass[kGroupBins];  // groups, and their maxima's weight
+  union {
+    int groups[kThreads * kGroups];  // first vectors of the groups to read again
+    u64 few[kRank];                  // entries that select() ranks
+  };
+  u64 cut, rest;  // composite and draw found by rank 0
+  Case row;
+  int count, found, n_groups, pick;
 };
 
 // ------------------------------------------------------- block and cluster
@@ -283,27 +298,24 @@ __device__ u64 block_scan(u64 x, u64& total, Shared& sm) {
   return before + inc - x;
 }
 
-// Bitonic sort of a[0 .. n), n a power of two.
-template <bool kDescending>
-__device__ void block_sort(u64* a, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-        const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-        const u64 x = a[i], y = a[j];
-        const bool up = ((i & size) == 0) != kDescending;
-        if ((x > y) == up) a[i] = y, a[j] = x;
-      }
-    }
-  __syncthreads();
-}
-
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
 __device__ __forceinline__ uint32_t draw_part(float u) {
   return (uint32_t)(fminf(fmaxf(u, 0.0f), 0.99999994f) * 16777216.0f);
 }
+
+struct Groups {  // maxima of a thread's groups
+  float m[kGroups];
+};
+template <bool kF32>
+__device__ __noinline__ void draw_by_bins(Shared& sm, Groups gm, int k, uint32_t part, u64 total);
+template <bool kF32>
+__device__ __noinline__ void draw_by_weight(Shared& sm, Groups gm, u64 C);
+template <bool kF32>
+__device__ __noinline__ void draw_from_row(Shared& sm, u64 C);
+template <bool kF32>
+__device__ __noinline__ void draw_long_list(Shared& sm, int n, int n_k, bool use_p, u64 bound,
+                                            uint32_t part);
 
 // ------------------------------------------------------------------- sampler
 template <bool kF32>
@@ -317,12 +329,25 @@ struct Sampler {
   float top = 0.0f, inv_t = 1.0f, min_p = 0.0f;
   int per_warp;   // vectors of a warp's contiguous range, a multiple of 32
   int per_group;  // steps of 32 vectors of a group (the last may have fewer)
+  Groups gm;      // maxima of this thread's groups
 
   __device__ Sampler(const void* p, int V, Shared& s, int blocks, uint32_t r)
       : row(p, V), sm(s), n_blocks(blocks), rank(r) {
     const int ranges = blocks * kWarps * 32;
     per_warp = (row.n_vec + ranges - 1) / ranges * 32;
     per_group = (per_warp / 32 + kGroups - 1) / kGroups;
+  }
+  // The block's row again, in another function.
+  __device__ explicit Sampler(Shared& s) : Sampler(s.row.row, s.row.V, s, s.row.n_blocks, s.row.rank) {
+    turn = s.row.turn;
+    top = s.row.top, inv_t = s.row.inv_t, min_p = s.row.min_p;
+  }
+  // ... for which this leaves it (every thread calls it, after its last
+  // exchange here).
+  __device__ void leave(const void* p, float least, float u, long long* token) const {
+    if (threadIdx.x == 0)
+      sm.row = Case{p, row.V, n_blocks, turn, rank, top, inv_t, min_p, least, u, token};
+    __syncthreads();
   }
   __device__ __forceinline__ int warp_begin() const {
     return ((int)rank * kWarps + threadIdx.x / 32) * per_warp;
@@ -449,26 +474,6 @@ struct Sampler {
     return n_blocks == 1 ? sm.count : (int)remote_load(remote(&sm.count, 0));
   }
 
-  // Sorts the list (n entries) with the largest composite first.
-  __device__ void sort_list(int n) const {
-    const int N = pow2_at_least(n);
-    for (int t = n + threadIdx.x; t < N; t += kThreads) sm.list[t] = 0;
-    block_sort<true>(sm.list, N);
-  }
-
-  // Whole weights of this thread's four list entries, their sum's place among
-  // the threads (exclusive) and the total.
-  __device__ u64 list_scan(int n, u64 (&q)[4], u64& total) const {
-    u64 mine = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = threadIdx.x * 4 + e;
-      q[e] = r < n ? whole(sm.list[r]) : 0;
-      mine += q[e];
-    }
-    return block_scan(mine, total, sm);
-  }
-
   // ------------------------------------------------------ rank 0: the list
   // Draws from the list's n entries: the first n_k by rank, of those the
   // leading run that reaches `bound` (part of the n_k's total when bound is 0
@@ -505,100 +510,178 @@ struct Sampler {
     if (keep && sub == 0 && run <= target && target < run + q) *token = index_of(mine);
   }
 
-  // The same for a long list, by sorting.
-  __device__ void draw_sorted(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
-                              long long* token) const {
-    sort_list(n);
-    u64 q[4], total;
-    u64 run = list_scan(n_k, q, total);
-    if (use_p && bound == 0) bound = max(share_of(total, part), (u64)1);
-    u64 keep = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = threadIdx.x * 4 + e;
-      keep += r < n_k && (!use_p || run < bound) && q[e] &&
-              weight(logit_of(sm.list[r])) >= min_p;
-      run += q[e];
-    }
-    n = (int)block_sum(keep, sm);
-    const int N = pow2_at_least(n);
-    for (int t = threadIdx.x; t < N; t += kThreads)
-      sm.order[t] = t < n ? ((u64)index_of(sm.list[t]) << 32) | (sm.list[t] >> 32) : ~0ull;
-    block_sort<false>(sm.order, N);
-    u64 mine = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = threadIdx.x * 4 + e;
-      q[e] = r < n ? whole_of(weight(of_key((uint32_t)sm.order[r]))) : 0;
-      mine += q[e];
-    }
-    run = block_scan(mine, total, sm);
-    const u64 target = share_of(total, draw_part(u));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (q[e] && run <= target && target < run + q[e])
-        *token = (long long)(sm.order[threadIdx.x * 4 + e] >> 32);
-      run += q[e];
-    }
-  }
+  enum Order { kCount, kMass, kIndex };
 
-  // Keeps the list's entries in the bins (linear in the logit) up to the one
-  // where their weight reaches `bound`; returns their number. The list carries
-  // at least `bound`.
-  __device__ int shorten(int n, u64 bound, float low) const {
+  // The entry of the list (n of them) at which the running sum reaches `need`:
+  // of ones or whole weights from the largest composite down, or (kIndex) of
+  // the kept weights in index order, kept being at or above C with w >= min_p.
+  // Entries are narrowed to one of 256 bins of the order's value at a time (equal
+  // logits by their indices), and the last few ranked by counting.
+  template <Order kOrder>
+  __device__ u64 select(int n, u64 need, u64 C) const {
     const int tid = threadIdx.x;
-    const float range = fminf(top - low, 3.0e38f);
-    const float scale = range > 0.0f ? (float)kGroupBins / range : 0.0f;
-    auto bin_of = [&](float x) { return min(kGroupBins - 1, (int)((top - x) * scale)); };
-    if (tid < kGroupBins) sm.mass[tid] = 0;
-    if (tid == 0) sm.found = kGroupBins - 1;
-    __syncthreads();
-    u64 c[4];
+    auto weight_in = [&](u64 c) -> u64 {
+      if constexpr (kOrder == kCount) return 1;
+      if (kOrder == kIndex && (c < C || weight(logit_of(c)) < min_p)) return 0;
+      return whole(c);
+    };
+    u64 c[4], q[4];
+    int alive = 0;  // bits
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = tid + e * kThreads;
       c[e] = r < n ? sm.list[r] : 0;
-      if (r < n) atomicAdd(&sm.mass[bin_of(logit_of(c[e]))], whole(c[e]));
+      q[e] = r < n ? weight_in(c[e]) : 0;
+      if (q[e]) alive |= 1 << e;
+    }
+    u64 base = 0;  // weight before the entries that are left
+    bool by_index = kOrder == kIndex;
+    auto place = [&](u64 x) { return by_index ? (float)index_of(x) : top - logit_of(x); };
+    int left = (int)block_sum(__popc(alive), sm);
+    while (left > kRank) {
+      float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (alive >> e & 1) lo = fminf(lo, place(c[e])), hi = fmaxf(hi, place(c[e]));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+      }
+      __syncthreads();
+      if (tid % 32 == 0)
+        sm.part[tid / 32] = ((u64)__float_as_uint(lo) << 32) | __float_as_uint(hi);
+      if (tid < kGroupBins) sm.mass[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        lo = fminf(lo, __uint_as_float((uint32_t)(sm.part[w] >> 32)));
+        hi = fmaxf(hi, __uint_as_float((uint32_t)sm.part[w]));
+      }
+      if (!(hi > lo)) {  // equal logits follow each other by index
+        by_index = true;
+        continue;
+      }
+      const float scale = (float)kGroupBins / fminf(hi - lo, 3.0e38f);
+      auto bin_of = [&](u64 x) { return min(kGroupBins - 1, (int)((place(x) - lo) * scale)); };
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (alive >> e & 1) atomicAdd(&sm.mass[bin_of(c[e])], q[e]);
+      __syncthreads();
+      u64 all;
+      const u64 mine = tid < kGroupBins ? sm.mass[tid] : 0;
+      const u64 before = base + block_scan(mine, all, sm);
+      if (before < need && need <= before + mine) sm.found = tid, sm.rest = before;
+      __syncthreads();
+      base = sm.rest;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((alive >> e & 1) && bin_of(c[e]) != sm.found) alive &= ~(1 << e);
+      left = (int)block_sum(__popc(alive), sm);
     }
     __syncthreads();
-    u64 all;
-    const u64 mine = tid < kGroupBins ? sm.mass[tid] : 0;
-    const u64 before = block_scan(mine, all, sm);
-    if (tid == 0) sm.count = 0;
-    if (before < bound && bound <= before + mine) sm.found = tid;
+    if (tid == 0) sm.found = 0;
     __syncthreads();
-    const int cut = sm.found;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (c[e] && bin_of(logit_of(c[e])) <= cut) sm.list[atomicAdd(&sm.count, 1)] = c[e];
+      if (alive >> e & 1) {
+        const int at = atomicAdd(&sm.found, 1);
+        sm.few[at] = c[e];
+        sm.q[at] = q[e];
+      }
     __syncthreads();
-    return sm.count;
+    const int each_of = kThreads / max(16, pow2_at_least(left));
+    const int i = tid / each_of, sub = tid % each_of;
+    const bool live = i < left;
+    const u64 mine = live ? sm.few[i] : 0;
+    u64 before = 0;
+    for (int j = sub; j < left; j += each_of) {
+      const u64 other = sm.few[j];
+      const bool ahead = kOrder == kIndex ? index_of(other) < index_of(mine) : other > mine;
+      before += ahead ? sm.q[j] : 0;
+    }
+    for (int off = each_of / 2; off > 0; off >>= 1)
+      before += __shfl_xor_sync(0xffffffffu, before, off);
+    before += base;
+    if (live && sub == 0 && before < need && need <= before + sm.q[i]) sm.cut = mine;
+    __syncthreads();
+    return sm.cut;
   }
 
+  // Whole weight of the list's entries at or above C (with w >= min_p where
+  // `kept` asks for it).
+  __device__ u64 list_mass(int n, u64 C, bool kept) const {
+    u64 s = 0;
+    for (int r = threadIdx.x; r < n; r += kThreads) {
+      const u64 c = sm.list[r];
+      if (c >= C && (!kept || weight(logit_of(c)) >= min_p)) s += whole(c);
+    }
+    return block_sum(s, sm);
+  }
+
+  __device__ void long_list(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+                            long long* token) const {
+    u64 C = n_k < n ? select<kCount>(n, (u64)n_k, 0) : 0;
+    if (use_p) {
+      if (bound == 0) bound = max(share_of(list_mass(n, C, false), part), (u64)1);
+      C = select<kMass>(n, bound, 0);
+    }
+    const u64 target = share_of(list_mass(n, C, true), draw_part(u));
+    const u64 c = select<kIndex>(n, target + 1, C);
+    if (threadIdx.x == 0) *token = index_of(c);
+  }
   __device__ void draw_from_list(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
                                  long long* token) const {
     if (n <= kRank)
       draw_ranked(n, n_k, use_p, bound, part, u, token);
     else
-      draw_sorted(n, n_k, use_p, bound, part, u, token);
+      draw_long_list<kF32>(sm, n, n_k, use_p, bound, part);
   }
 
   // -------------------------------------------------------- whole-row draws
-  // Draw among the tokens at or above the composite C with w >= min_p: sums of
-  // the blocks' and warps' ranges, then of the range that holds the draw.
-  __device__ void draw_from_row(u64 C, float u, long long* token) {
-    auto mass_of = [&](float x, int i) -> u64 {
-      if (!(x > -INFINITY)) return 0;  // NaN too
-      const float w = weight(x);
-      return w >= min_p && (C == 0 || composite(x, i) >= C) ? whole_of(w) : 0;
-    };
+  // Whole weight of a token if it is kept: at or above C, w >= min_p.
+  __device__ __forceinline__ u64 kept_mass(float x, int i, u64 C) const {
+    if (!(x > -INFINITY)) return 0;  // NaN too
+    const float w = weight(x);
+    return w >= min_p && (C == 0 || composite(x, i) >= C) ? whole_of(w) : 0;
+  }
+
+  // The draw falls into warp range w of the row, `target` into its kept weight:
+  // the range in contiguous pieces, one per thread.
+  __device__ void draw_from_range(int w, u64 target, u64 C, long long* token) const {
+    const int begin = w * per_warp, end = min(row.n_vec, begin + per_warp);
+    const int piece = (per_warp + kThreads - 1) / kThreads;
+    const int j0 = begin + threadIdx.x * piece, j1 = min(end, j0 + piece);
+    u64 mine = 0, all;
+    for (int j = j0; j < j1; ++j) {
+      const Vec<kF32> x = row.get(j);
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine += kept_mass(x.at(e), j * E - row.mis + e, C);
+    }
+    u64 run = block_scan(mine, all, sm);
+    if (run <= target && target < run + mine) {
+      for (int j = j0; j < j1; ++j) {
+        const Vec<kF32> x = row.get(j);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = j * E - row.mis + e;
+          const u64 q = kept_mass(x.at(e), i, C);
+          if (q && run <= target && target < run + q) *token = i;
+          run += q;
+        }
+      }
+    }
+  }
+
+  // Draw among the kept tokens by sums of the blocks' and warps' ranges.
+  __device__ void by_row(u64 C, float u, long long* token) {
     u64 mine = 0;
     if (C == 0 && min_p <= 0.0f) {
       mine = mass();
     } else {
       const float least = C == 0 ? -INFINITY : logit_of(C);
       each([&](float x, int i) {
-        if (x >= least) mine += mass_of(x, i);
+        if (x >= least) mine += kept_mass(x, i, C);
       });
     }
     mine = warp_sum(mine);
@@ -617,30 +700,7 @@ struct Sampler {
     if (target < before || target >= before + ours) return;  // another block's
     int w = 0;
     while (w < kWarps - 1 && before + sm.part[w] <= target) before += sm.part[w++];
-    // The range in contiguous pieces, one per thread.
-    const int begin = ((int)rank * kWarps + w) * per_warp, end = min(row.n_vec, begin + per_warp);
-    const int piece = (per_warp + kThreads - 1) / kThreads;
-    const int j0 = begin + threadIdx.x * piece, j1 = min(end, j0 + piece);
-    mine = 0;
-    for (int j = j0; j < j1; ++j) {
-      const Vec<kF32> x = row.get(j);
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine += mass_of(x.at(e), j * E - row.mis + e);
-    }
-    u64 all;
-    u64 run = before + block_scan(mine, all, sm);
-    if (run <= target && target < run + mine) {
-      for (int j = j0; j < j1; ++j) {
-        const Vec<kF32> x = row.get(j);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = j * E - row.mis + e;
-          const u64 q = mass_of(x.at(e), i);
-          if (q && run <= target && target < run + q) *token = i;
-          run += q;
-        }
-      }
-    }
+    draw_from_range((int)rank * kWarps + w, target - before, C, token);
   }
 
   // Composite of the last token of the smallest leading run of the tokens at
@@ -667,25 +727,141 @@ struct Sampler {
     return n_blocks == 1 ? sm.cut : remote_load64(remote(&sm.cut, 0));
   }
 
-  // The cuts by histogram (see the head of the file): the composite at or
-  // above which a token is kept. k <= 0: no top-k; `total`: the row's weight
-  // where it is known (else 0); least: the row's smallest logit.
-  __device__ u64 cut_by_bins(int k, bool use_p, uint32_t part, u64 total, float least) {
-    const int tid = threadIdx.x;
-    // Bins are linear in the logit over the live range [low, top].
-    const float low = fmaxf(least, cutoff());
-    const float range = fminf(top - low, 3.0e38f);
-    const float scale = range > 0.0f ? (float)kBins / range : 0.0f;
-    auto bin_of = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };
-    const int light = bin_of(top - 7.0f / inv_t);  // bins from here: by their centre
-    for (int t = tid; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
+  // ------------------------------------------------------------ histograms
+  // Bins are linear in the logit over the live range [low, top].
+  struct Bins {
+    float top, low, scale, width;
+    int light;  // bins from here on weigh by their centre
+
+    __device__ __forceinline__ int of(float x) const {
+      const float t = fminf((top - x) * scale, (float)(kBins - 1));  // NaN: the last
+      return __float_as_uint(__fadd_rd(t, 8388608.0f)) & (kBins - 1);
+    }
+    __device__ __forceinline__ float upper(int b) const {  // value where bin b begins
+      return b <= 0 ? INFINITY : top - (float)b * width;
+    }
+    __device__ __forceinline__ float lower(int b) const {
+      return b >= kBins - 1 ? low : top - (float)(b + 1) * width;
+    }
+  };
+  __device__ Bins bins_over(float least) const {
+    Bins b;
+    b.top = top;
+    b.low = fmaxf(least, cutoff());
+    const float range = fminf(top - b.low, 3.0e38f);
+    b.scale = range > 0.0f ? (float)kBins / range : 0.0f;
+    b.width = range / kBins;
+    b.light = 0;
+    b.light = b.of(top - 7.0f / inv_t);
+    return b;
+  }
+  __device__ __forceinline__ void count_in(const Bins& bins, float x, bool weigh) const {
+    if (!(x >= bins.low)) return;
+    const int b = bins.of(x);
+    atomicAdd(&sm.bins[b], 1u);
+    if (b < bins.light && weigh) atomicAdd(&sm.heavy[b], __expf((x - top) * inv_t));
+  }
+  __device__ void clear_bins() const {
+    for (int t = threadIdx.x; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
     __syncthreads();
-    each([&](float x, int) {
-      if (!(x >= low)) return;
-      const int b = bin_of(x);
-      atomicAdd(&sm.bins[b], 1u);
-      if (b < light && use_p) atomicAdd(&sm.heavy[b], __expf((x - top) * inv_t));
-    });
+  }
+  // mass() and the histogram in one pass.
+  __device__ u64 mass_and_bins(const Bins& bins) const {
+    clear_bins();
+    u64 s = 0;
+    const int end = end_vec();
+    for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
+      WholeSum w;
+      const int stop = min(end, j0 + 32 * 128);
+      for (int j = j0; j < stop; j += 32) {
+        const Vec<kF32> x = row.get(j);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          w.add(x.at(e) > -INFINITY ? weight(x.at(e)) : 0.0f);
+          count_in(bins, x.at(e), true);
+        }
+      }
+      s += w.total();
+    }
+    return s;
+  }
+
+  // One pass that divides the row by value: this thread's sum of the whole
+  // weights above `hi` (where weigh is set) and their number; the tokens of
+  // [lo, hi] at or above C go to the list.
+  __device__ u64 split(float hi, float lo, u64 C, bool weigh, uint32_t& count) const {
+    u64 s = 0;
+    count = 0;
+    const int end = end_vec();
+    for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
+      WholeSum w;
+      const int stop = min(end, j0 + 32 * 128);
+#pragma unroll 2
+      for (int j = j0; j < stop; j += 32) {
+        const Vec<kF32> x = row.get(j);
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float v = x.at(e);
+          const int i = j * E - row.mis + e;
+          n += v > hi;
+          if (v >= lo && !(v > hi) && (C == 0 || composite(v, i) >= C)) push(v, i);
+        }
+        count += n;
+        if (n && weigh) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) w.add(x.at(e) > hi ? weight(x.at(e)) : 0.0f);
+        }
+      }
+      s += w.total();
+    }
+    return s;
+  }
+
+  // The draw among the tokens at or above C: `mine` is this thread's weight
+  // above the list's range; rank 0's list (n entries) has the other kept ones.
+  __device__ void draw_from_split(u64 mine, int n, u64 C, float u, long long* token) {
+    mine = warp_sum(mine);
+    if (threadIdx.x % 32 == 0) {
+      const int at = (int)rank * kWarps + threadIdx.x / 32;
+      if (n_blocks == 1)
+        sm.wsum[at] = mine;
+      else
+        remote_store(remote(&sm.wsum[at], 0), mine);
+    }
+    sync();
+    if (rank == 0) {
+      for (int t = threadIdx.x; t < n; t += kThreads) {
+        const u64 c = sm.list[t];
+        if (c >= C) atomicAdd(&sm.wsum[((int)index_of(c) + row.mis) / E / per_warp], whole(c));
+      }
+      __syncthreads();
+      u64 all;
+      const int ranges = n_blocks * kWarps;
+      const u64 ours = threadIdx.x < ranges ? sm.wsum[threadIdx.x] : 0;
+      const u64 before = block_scan(ours, all, sm);
+      const u64 target = share_of(all, draw_part(u));
+      if (before <= target && target < before + ours)
+        sm.pick = threadIdx.x, sm.rest = target - before;
+    }
+    sync();
+    const int w = n_blocks == 1 ? sm.pick : (int)remote_load(remote(&sm.pick, 0));
+    const u64 target = n_blocks == 1 ? sm.rest : remote_load64(remote(&sm.rest, 0));
+    if (w / kWarps == (int)rank) draw_from_range(w, target, C, token);
+  }
+
+  // The draw where the cuts go by histogram (see the head of the file). k <= 0:
+  // no top-k, then `total` is the row's weight where it is known (else 0).
+  __device__ void by_bins(int k, bool use_p, uint32_t part, u64 total, float least, float u,
+                          long long* token) {
+    const int tid = threadIdx.x;
+    const Bins bins = bins_over(least);
+    if (k <= 0 && total == 0) {
+      total = cluster_sum(mass_and_bins(bins));
+    } else {
+      clear_bins();
+      each([&](float x, int) { count_in(bins, x, use_p); });
+    }
     sync();
     // This thread's four bins: tokens, and roughly their weight. The rough
     // weights only choose which bins are looked at; exact sums decide.
@@ -703,8 +879,8 @@ struct Sampler {
         heavy += n_blocks == 1 ? sm.heavy[b]
                                : __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
       }
-      m[e] = b < light ? heavy
-                       : (float)c[e] * __expf(-((float)b + 0.5f) * (range / kBins) * inv_t);
+      m[e] = b < bins.light ? heavy
+                            : (float)c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
       n_mine += c[e];
       m_mine += m[e];
     }
@@ -719,53 +895,60 @@ struct Sampler {
     if (k > 0 && (u64)k < n_all) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (n_before < (u64)k && (u64)k <= n_before + c[e]) {
-          sm.found = tid * 4 + e;
-          sm.n_groups = (int)((u64)k - n_before);  // wanted of that bin
-        }
+        if (n_before < (u64)k && (u64)k <= n_before + c[e]) sm.found = tid * 4 + e;
         n_before += c[e];
       }
       __syncthreads();
-      last_bin = sm.found;
-      const int need = sm.n_groups;
-      u64 above = 0;
-      each([&](float x, int i) {
-        if (!(x >= low)) return;
-        const int b = bin_of(x);
-        if (b < last_bin && use_p) above += whole_of(weight(x));
-        if (b == last_bin) push(x, i);
-      });
-      above = cluster_sum(above);
+      const int at = sm.found;
+      last_bin = min(kBins - 1, at + 1);
+      uint32_t count;
+      const u64 mine = split(bins.upper(at - 1), bins.lower(last_bin), 0, use_p || min_p <= 0.0f,
+                             count);
+      const Pair above = cluster_sum(mine, count);
       sync();
       const int n = list_size();
-      if (n > kCap) {
-        C = bisect((u64)k, true, 0);
-        if (use_p) {
-          u64 s = 0;
-          each([&](float x, int i) {
-            if (x > -INFINITY && composite(x, i) >= C) s += whole_of(weight(x));
-          });
-          mass_k = cluster_sum(s);
-        }
-      } else {
+      const int need = (int)((u64)k - above.b);
+      if (n <= kCap && above.b < (u64)k && need <= n) {
         u64 within = 0;
         if (rank == 0) {
-          sort_list(n);
-          if (tid == 0) sm.cut = sm.list[need - 1];
-          u64 q[4];
-          list_scan(need, q, within);
+          const u64 c = select<kCount>(n, (u64)need, 0);
+          within = list_mass(n, c, false);
         }
         C = shared_cut();
-        if (use_p) mass_k = above + exchange(within, 0)[0].a;
+        if (!use_p) {
+          if (min_p > 0.0f)
+            by_weight(C, u, token);
+          else
+            draw_from_split(mine, n, C, u, token);
+          return;
+        }
+        mass_k = above.a + exchange(within, 0)[0].a;
+      } else {
+        C = bisect((u64)k, true, 0);
+        if (!use_p) {
+          by_row(C, u, token);
+          return;
+        }
+        u64 s = 0;
+        each([&](float x, int i) {
+          if (x > -INFINITY && composite(x, i) >= C) s += whole_of(weight(x));
+        });
+        mass_k = cluster_sum(s);
       }
-    } else if (use_p && total == 0) {
+    } else if (!use_p) {  // fewer live tokens than k: all are kept
+      if (min_p > 0.0f)
+        by_weight(0, u, token);
+      else
+        by_row(0, u, token);
+      return;
+    } else if (total == 0) {
       mass_k = cluster_sum(mass());
     }
-    if (!use_p) return C;
 
     // The bin that the mass bound falls into, by the rough weights; it and its
     // neighbours are collected, and the exact sums decide or correct the guess.
     const u64 bound = max(share_of(mass_k, part), (u64)1);
+    const float most = C ? logit_of(C) : -INFINITY;
     float m_inc = m_mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -793,35 +976,23 @@ struct Sampler {
       }
       __syncthreads();
       const int b0 = max(0, sm.found - 1), b1 = min(last_bin, sm.found + 1);
-      u64 above = 0;
-      each([&](float x, int i) {
-        if (!(x >= low)) return;
-        const int b = bin_of(x);
-        if (b > b1 || (b == last_bin && C != 0 && composite(x, i) < C)) return;
-        if (b < b0)
-          above += whole_of(weight(x));
-        else
-          push(x, i);
-      });
-      above = cluster_sum(above);
+      uint32_t count;
+      const u64 mine = split(fmaxf(bins.upper(b0), most), bins.lower(b1), C, true, count);
+      const u64 above = cluster_sum(mine);
       sync();
       const int n = list_size();
       if (n > kCap) break;
-      u64 q[4], all = 0;
-      if (rank == 0) list_scan(n, q, all);
+      u64 all = 0;
+      if (rank == 0) all = list_mass(n, 0, false);
       all = exchange(all, 0)[0].a;
       if (above < bound && bound <= above + all) {
-        if (rank == 0) {
-          sort_list(n);
-          u64 before = above + list_scan(n, q, all);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (q[e] && before < bound && bound <= before + q[e])
-              sm.cut = sm.list[tid * 4 + e];
-            before += q[e];
-          }
-        }
-        return shared_cut();
+        if (rank == 0) select<kMass>(n, bound - above, 0);
+        C = shared_cut();
+        if (min_p > 0.0f)
+          by_weight(C, u, token);
+        else
+          draw_from_split(mine, n, C, u, token);
+        return;
       }
       // The rough sum at the start of bin b0 is off by what the exact one says.
       run = rough;
@@ -834,15 +1005,75 @@ struct Sampler {
       __syncthreads();
       want = sm.fpart[0] + ((float)bound - (float)above) / kOne;
     }
-    return bisect(bound, false, C);
+    by_row(bisect(bound, false, C), u, token);
+  }
+
+  // ------------------------------------------------------- group candidates
+  // Lists the tokens of the groups whose maximum is a candidate, those that are
+  // candidates themselves; returns this thread's whole weight among them. The
+  // list is complete after the next sync().
+  template <class F>
+  __device__ u64 list_candidates(F candidate) {
+    const int tid = threadIdx.x;
+    if (tid == 0) sm.n_groups = 0, sm.count = 0;
+    sync();
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if (candidate(gm.m[g], -1)) sm.groups[atomicAdd(&sm.n_groups, 1)] = group_first(g);
+    __syncthreads();
+    // Their vectors, shared among all threads.
+    const int items = sm.n_groups * per_group;
+    u64 listed = 0;
+    for (int it0 = tid; it0 < items; it0 += 4 * kThreads) {
+      Vec<kF32> x[4];
+      int at[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // Step s of a group, unless past the end of the group's warp range.
+        const int it = it0 + e * kThreads;
+        at[e] = -1;
+        if (it < items) {
+          const int f = sm.groups[it / per_group], j = f + it % per_group * 32;
+          if (j < min(row.n_vec, (f / per_warp + 1) * per_warp)) at[e] = j;
+        }
+        if (at[e] >= 0) x[e] = row.get(at[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at[e] >= 0) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const float v = x[e].at(i);
+            if (candidate(v, at[e] * E - row.mis + i)) {
+              push(v, at[e] * E - row.mis + i);
+              listed += whole_of(weight(v));
+            }
+          }
+        }
+    }
+    return listed;
+  }
+
+  // Draw among the tokens at or above C with w >= min_p, min_p > 0.
+  __device__ void by_weight(u64 C, float u, long long* token) {
+    sync();  // the list before has been read
+    list_candidates([&](float x, int i) {
+      return x > -INFINITY && weight(x) >= min_p && (C == 0 || i < 0 || composite(x, i) >= C);
+    });
+    sync();
+    const int n = list_size();
+    if (n > kCap) {
+      by_row(C, u, token);
+    } else if (rank == 0) {
+      draw_from_list(n, n, false, 0, 0, u, token);
+    }
   }
 
   // --------------------------------------------------------------- one row
-  __device__ void run(float T, int k, float top_p, float u, long long* token) {
+  __device__ void run(const void* p, float T, int k, float top_p, float u, long long* token) {
     const int tid = threadIdx.x, lane = tid % 32;
     // Maxima of the thread's groups, and the row's extremes.
     const int end = end_vec();
-    float gm[kGroups];
     Extremes<kF32> all;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -857,16 +1088,16 @@ struct Sampler {
         for (int i = 0; i < 8; ++i) m.add(x[i], all);
       }
       for (; j < stop; j += 32) m.add(row.get(j), all);
-      gm[g] = m.max();
+      gm.m[g] = m.max();
     }
-    if (tid < kGroupBins) sm.gbins[tid] = 0;
+    if (tid < kGroupBins) sm.gbins[tid] = sm.gmass[tid] = 0;
     if (tid == 0) sm.count = 0, sm.n_groups = 0, sm.found = 0x7fffffff;
     float low, least;  // smallest group maximum, smallest logit
     {
-      float hi = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3])), lo = INFINITY;
+      float hi = fmaxf(fmaxf(gm.m[0], gm.m[1]), fmaxf(gm.m[2], gm.m[3])), lo = INFINITY;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        if (gm[g] > -INFINITY) lo = fminf(lo, gm[g]);
+        if (gm.m[g] > -INFINITY) lo = fminf(lo, gm.m[g]);
       float mn = all.min();
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) {
@@ -904,7 +1135,7 @@ struct Sampler {
       // Greedy: the lowest index that holds the maximum.
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        if (gm[g] == top)
+        if (gm.m[g] == top)
           each_in(group_first(g), min(end, group_first(g) + 32 * per_group), [&](float x, int i) {
             if (x == top) atomicMin(&sm.found, i);
           });
@@ -919,124 +1150,171 @@ struct Sampler {
     }
     const bool use_k = k > 0 && k < row.V, use_p = top_p < 1.0f;
     const uint32_t part = (uint32_t)(fmaxf(top_p, 0.0f) * 16777216.0f);
-    const bool by_weight = !use_k && !use_p;
-    if (by_weight && min_p <= 0.0f) {
-      draw_from_row(0, u, token);
+    if (!use_k && !use_p) {
+      leave(p, least, u, token);
+      if (min_p > 0.0f)
+        draw_by_weight<kF32>(sm, gm, 0);
+      else
+        draw_from_row<kF32>(sm, 0);
       return;
     }
     u64 total = 0;
     if (!use_k || k <= kSmallK) {
-      // Which logits are candidates goes by bins over the group maxima, so that
-      // they are a leading run up to ties; with min-p alone by the weight.
+      // Bins over the group maxima; a bin also decides which logits are
+      // candidates, so that those are a leading run up to ties.
       const float live = cutoff();
       const float range = fminf(top - low, fminf(kLive / inv_t, 3.0e38f));
       const float scale = range > 0.0f ? (float)kGroupBins / range : 0.0f;
       auto bin_of = [&](float x) { return min(kGroupBins - 1, (int)((top - x) * scale)); };
-      int cut = 0;
-      if (!by_weight) {
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-          if (gm[g] > -INFINITY && gm[g] >= live) atomicAdd(&sm.gbins[bin_of(gm[g])], 1u);
-        sync();
-        const uint32_t* counts = sm.gbins;
-        if (n_blocks > 1) {
-          if (tid < kGroupBins) {
-            uint32_t c = 0;
-            for (int r = 0; r < n_blocks; ++r) c += remote_load(remote(&sm.gbins[tid], r));
-            sm.gsum[tid] = c;
-          }
-          __syncthreads();
-          counts = sm.gsum;
-        }
-        // The first bin up to which the groups suffice (the last if none does);
-        // every warp finds it for itself.
-        const uint32_t want = use_k ? (uint32_t)k : (uint32_t)kNucleus;
-        uint32_t c[kGroupBins / 32], mine = 0;
-#pragma unroll
-        for (int e = 0; e < kGroupBins / 32; ++e) mine += c[e] = counts[lane * (kGroupBins / 32) + e];
-        uint32_t inc = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
-          if (lane >= off) inc += y;
-        }
-        uint32_t run = inc - mine;
-        int at = kGroupBins - 1;
-#pragma unroll
-        for (int e = kGroupBins / 32 - 1; e >= 0; --e) {
-          uint32_t upto = run;
-#pragma unroll
-          for (int f = 0; f <= e; ++f) upto += c[f];
-          if (upto >= want) at = lane * (kGroupBins / 32) + e;
-        }
-        cut = __reduce_min_sync(0xffffffffu, at);
-      }
-      auto candidate = [&](float x) {
-        return x > -INFINITY && x >= live && (by_weight ? weight(x) >= min_p : bin_of(x) <= cut);
-      };
-      // The groups to read again, then their vectors shared among all threads.
+      float sure = 0.0f, sample = 0.0f;  // weight of the maxima, and of a vector's rest
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        if (candidate(gm[g])) sm.groups[atomicAdd(&sm.n_groups, 1)] = group_first(g);
-      __syncthreads();
-      const int items = sm.n_groups * per_group;
-      u64 listed = 0;
-      for (int it0 = tid; it0 < items; it0 += 4 * kThreads) {
-        Vec<kF32> x[4];
-        int at[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          // Step s of a group, unless past the end of the group's warp range.
-          const int it = it0 + e * kThreads;
-          at[e] = -1;
-          if (it < items) {
-            const int f = sm.groups[it / per_group], j = f + it % per_group * 32;
-            if (j < min(row.n_vec, (f / per_warp + 1) * per_warp)) at[e] = j;
+        if (gm.m[g] > -INFINITY && gm.m[g] >= live) {
+          const int b = bin_of(gm.m[g]);
+          atomicAdd(&sm.gbins[b], 1u);
+          if (!use_k) {
+            const float w = __expf((gm.m[g] - top) * inv_t);
+            sure += gm.m[g] == top ? 1.0f : w;
+            atomicAdd(&sm.gmass[b], (uint32_t)((gm.m[g] == top ? 1.0f : w) * 131072.0f));
           }
-          if (at[e] >= 0) x[e] = row.get(at[e]);
+        }
+      if (!use_k) {
+        const int j = first_vec();
+        if (j < end) {
+          const Vec<kF32> x = row.get(j);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (x.at(e) < gm.m[0]) sample += __expf((x.at(e) - top) * inv_t);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at[e] >= 0) {
+        for (int off = 16; off > 0; off >>= 1) {
+          sure += __shfl_xor_sync(0xffffffffu, sure, off);
+          sample += __shfl_xor_sync(0xffffffffu, sample, off);
+        }
+        if (lane == 0)
+          sm.part[tid / 32] = ((u64)__float_as_uint(sure) << 32) | __float_as_uint(sample);
+        __syncthreads();
+        sure = sample = 0.0f;
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-              if (candidate(x[e].at(i))) {
-                push(x[e].at(i), at[e] * E - row.mis + i);
-                listed += whole_of(weight(x[e].at(i)));
-              }
+        for (int w = 0; w < kWarps; ++w) {
+          sure += __uint_as_float((uint32_t)(sm.part[w] >> 32));
+          sample += __uint_as_float((uint32_t)sm.part[w]);
+        }
+        if (n_blocks > 1) {
+          const Pair* p = exchange(__float_as_uint(sure), __float_as_uint(sample));
+          sure = sample = 0.0f;
+          for (int r = 0; r < n_blocks; ++r) {
+            sure += __uint_as_float((uint32_t)p[r].a);
+            sample += __uint_as_float((uint32_t)p[r].b);
           }
+        }
       }
-      if (!use_k && use_p) {
-        const Pair s = cluster_sum(mass(), listed);
+      sync();
+      if (n_blocks > 1) {
+        uint32_t n = 0, w = 0;
+        if (tid < kGroupBins)
+          for (int r = 0; r < n_blocks; ++r) {
+            n += remote_load(remote(&sm.gbins[tid], r));
+            w += remote_load(remote(&sm.gmass[tid], r));
+          }
+        sync();  // read by all before it is overwritten
+        if (tid < kGroupBins) sm.gbins[tid] = n, sm.gmass[tid] = w;
+        __syncthreads();
+      }
+      // The first bin up to which the groups suffice (the last if none does), by
+      // number for top-k, by weight for top-p; every warp finds it for itself.
+      float want = (float)k;
+      if (!use_k) {
+        const int sampled = min(row.n_vec, n_blocks * kThreads);
+        const float est = sure + sample * ((float)row.n_vec / (float)sampled);
+        want = fminf(1.05f * est * (float)part * (131072.0f / 16777216.0f), 4.0e9f);
+      }
+      constexpr int kEach = kGroupBins / 32;
+      const uint32_t* goal = use_k ? sm.gbins : sm.gmass;
+      uint32_t mine = 0, mine_n = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        mine += goal[lane * kEach + e], mine_n += sm.gbins[lane * kEach + e];
+      uint32_t inc = mine, inc_n = mine_n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
+        const uint32_t z = __shfl_up_sync(0xffffffffu, inc_n, off);
+        if (lane >= off) inc += y, inc_n += z;
+      }
+      uint32_t run = inc - mine, run_n = inc_n - mine_n;
+      int at = kGroupBins;
+      uint32_t at_n = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        run += goal[lane * kEach + e], run_n += sm.gbins[lane * kEach + e];
+        if (at == kGroupBins && (float)run >= want) at = lane * kEach + e, at_n = run_n;
+      }
+      const int cut = __reduce_min_sync(0xffffffffu, at);
+      const uint32_t n_cut = __reduce_max_sync(0xffffffffu, at == cut ? at_n : 0u);
+      // A flat nucleus: its tokens are found by the row's histogram.
+      if (!use_k && (cut == kGroupBins || n_cut > kNucleus)) {
+        leave(p, least, u, token);
+        draw_by_bins<kF32>(sm, gm, 0, part, 0);
+        return;
+      }
+      const u64 listed_mine = list_candidates([&](float x, int) {
+        return x > -INFINITY && x >= live && bin_of(x) <= cut;
+      });
+      u64 listed = 0;
+      if (!use_k) {
+        const Pair s = cluster_sum(mass(), listed_mine);
         total = s.a;
         listed = s.b;
       }
       sync();
       const int n = list_size();
-      const u64 bound = !use_k && use_p ? max(share_of(total, part), (u64)1) : 0;
-      if (n <= kCap && (use_k || !use_p || listed >= bound)) {
-        if (rank == 0) {
-          const int m = bound && n > kRank ? shorten(n, bound, low) : n;
-          draw_from_list(m, use_k ? min(n, k) : m, use_p, bound, part, u, token);
-        }
+      const u64 bound = !use_k ? max(share_of(total, part), (u64)1) : 0;
+      if (n <= kCap && (use_k || listed >= bound)) {
+        if (n > kRank) leave(p, least, u, token);
+        if (rank == 0) draw_from_list(n, use_k ? min(n, k) : n, use_p, bound, part, u, token);
         return;
       }
     }
-    draw_from_row(cut_by_bins(use_k ? k : 0, use_p, part, total, least), u, token);
+    leave(p, least, u, token);
+    draw_by_bins<kF32>(sm, gm, use_k ? k : 0, use_p ? part : kNoCut, total);
   }
-
 };
+
+template <bool kF32>
+__device__ __noinline__ void draw_by_bins(Shared& sm, Groups gm, int k, uint32_t part, u64 total) {
+  Sampler<kF32> s(sm);
+  s.gm = gm;
+  s.by_bins(k, part != kNoCut, part, total, sm.row.least, sm.row.u, sm.row.token);
+}
+template <bool kF32>
+__device__ __noinline__ void draw_by_weight(Shared& sm, Groups gm, u64 C) {
+  Sampler<kF32> s(sm);
+  s.gm = gm;
+  s.by_weight(C, sm.row.u, sm.row.token);
+}
+template <bool kF32>
+__device__ __noinline__ void draw_from_row(Shared& sm, u64 C) {
+  Sampler<kF32> s(sm);
+  s.by_row(C, sm.row.u, sm.row.token);
+}
+template <bool kF32>
+__device__ __noinline__ void draw_long_list(Shared& sm, int n, int n_k, bool use_p, u64 bound,
+                                            uint32_t part) {
+  Sampler<kF32> s(sm);
+  s.long_list(n, n_k, use_p, bound, part, sm.row.u, sm.row.token);
+}
 
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p, int n_blocks) {
   __shared__ Shared sm;
   const int b = blockIdx.x / n_blocks;
-  Sampler<kF32> s(reinterpret_cast<const uint8_t*>(p.logits) + b * p.stride * (kF32 ? 4 : 2), p.V,
-                  sm, n_blocks, n_blocks > 1 ? cluster_rank() : 0);
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(p.logits) + b * p.stride * (kF32 ? 4 : 2);
+  Sampler<kF32> s(row, p.V, sm, n_blocks, n_blocks > 1 ? cluster_rank() : 0);
   const float T = p.temperature ? p.temperature[b] : p.temperature_all;
   s.inv_t = T > 0.0f ? 1.0f / fminf(T, 1.0e38f) : 1.0f;
   s.min_p = fminf(p.min_p ? p.min_p[b] : p.min_p_all, 1.0f);  // the best token stays
-  s.run(T, p.top_k ? p.top_k[b] : p.top_k_all, p.top_p ? p.top_p[b] : p.top_p_all, p.u[b],
+  s.run(row, T, p.top_k ? p.top_k[b] : p.top_k_all, p.top_p ? p.top_p[b] : p.top_p_all, p.u[b],
         p.tokens + b);
   if (n_blocks > 1) s.sync();  // no block's shared memory goes while another reads it
 }
