@@ -109,6 +109,13 @@ struct Vec {
     if constexpr (kF32) return __uint_as_float(w[e]);
     return e % 2 ? bf16hi_to_f32(w[e / 2]) : bf16lo_to_f32(w[e / 2]);
   }
+  __device__ __forceinline__ float pick(int e) const {  // any e, by selection
+    const int i = kF32 ? e : e >> 1;
+    const uint32_t lo = i & 1 ? w[1] : w[0], hi = i & 1 ? w[3] : w[2];
+    const uint32_t v = i & 2 ? hi : lo;
+    if constexpr (kF32) return __uint_as_float(v);
+    return e & 1 ? bf16hi_to_f32(v) : bf16lo_to_f32(v);
+  }
 };
 
 // Running maximum of a group's vectors, and (in `row`) the smallest logit of
@@ -253,13 +260,6 @@ __device__ __forceinline__ uint32_t remote_load(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ int remote_add(uint32_t addr, int v) {
-  int old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v)
-               : "memory");
-  return old;
-}
-
 __device__ __forceinline__ u64 warp_sum(u64 x) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
@@ -314,7 +314,7 @@ __device__ __noinline__ void draw_by_weight(Shared& sm, Groups gm, u64 C);
 template <bool kF32>
 __device__ __noinline__ void draw_from_row(Shared& sm, u64 C);
 template <bool kF32>
-__device__ __noinline__ void draw_long_list(Shared& sm, int n, int n_k, bool use_p, u64 bound,
+__device__ __noinline__ void draw_long_list(Shared& sm, int n, u64 C, int n_k, bool use_p, u64 bound,
                                             uint32_t part);
 
 // ------------------------------------------------------------------- sampler
@@ -458,27 +458,49 @@ struct Sampler {
     return s;
   }
 
-  // Adds a composite to rank 0's list; it may overflow (its count says so).
-  __device__ __forceinline__ void push(float x, int i) const {
-    const u64 c = composite(x, i);
-    if (n_blocks == 1) {
+  // Adds the tokens of vector j whose bits are set to the block's list, which
+  // may overflow (its count says so).
+  __device__ __forceinline__ void push(const Vec<kF32>& x, int j, uint32_t bits) const {
+    while (bits) {
+      const int e = __ffs(bits) - 1;
+      bits &= bits - 1;
       const int at = atomicAdd(&sm.count, 1);
-      if (at < kCap) sm.list[at] = c;
-    } else {
-      const int at = remote_add(remote(&sm.count, 0), 1);
-      if (at < kCap) remote_store(remote(&sm.list[at], 0), c);
+      if (at < kCap) sm.list[at] = composite(x.pick(e), j * E - row.mis + e);
     }
   }
-  // Entries pushed, for every block, once all have.
-  __device__ __forceinline__ int list_size() const {
-    return n_blocks == 1 ? sm.count : (int)remote_load(remote(&sm.count, 0));
+  // Empties the lists, before a pass that fills them.
+  __device__ __forceinline__ void clear_list() const {
+    sync();  // rank 0's has been read
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+  }
+  // Brings the blocks' lists together in rank 0's; returns its size (above kCap:
+  // too long, nothing was moved).
+  __device__ int collect_list() {
+    if (n_blocks == 1) {
+      __syncthreads();
+      return sm.count;
+    }
+    __syncthreads();
+    const int mine = sm.count;
+    const Pair* p = exchange((u64)mine, 0);
+    u64 total = 0, before = 0;
+    for (int r = 0; r < n_blocks; ++r) {
+      if (r < (int)rank) before += p[r].a;
+      total += p[r].a;
+    }
+    if (total <= kCap && rank > 0)
+      for (int t = threadIdx.x; t < mine; t += kThreads)
+        remote_store(remote(&sm.list[before + t], 0), sm.list[t]);
+    sync();
+    return (int)min(total, (u64)kCap + 1);
   }
 
   // ------------------------------------------------------ rank 0: the list
-  // Draws from the list's n entries: the first n_k by rank, of those the
+  // Draws from the list's n entries at or above C: the first n_k by rank, of those the
   // leading run that reaches `bound` (part of the n_k's total when bound is 0
   // and use_p is set), of those the ones with w >= min_p.
-  __device__ void draw_ranked(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+  __device__ void draw_ranked(int n, u64 C, int n_k, bool use_p, u64 bound, uint32_t part, float u,
                               long long* token) const {
     // Threads share each entry's count over the others.
     const int shared = kThreads / max(16, pow2_at_least(n));
@@ -496,7 +518,7 @@ struct Sampler {
       before_n += __shfl_xor_sync(0xffffffffu, before_n, off);
       before += __shfl_xor_sync(0xffffffffu, before, off);
     }
-    const bool in_k = live && before_n < n_k;
+    const bool in_k = live && mine >= C && before_n < n_k;
     if (use_p && bound == 0)
       bound = max(share_of(block_sum(in_k && sub == 0 ? q : 0, sm), part), (u64)1);
     const bool keep = in_k && (!use_p || before < bound) && weight(logit_of(mine)) >= min_p;
@@ -514,15 +536,16 @@ struct Sampler {
 
   // The entry of the list (n of them) at which the running sum reaches `need`:
   // of ones or whole weights from the largest composite down, or (kIndex) of
-  // the kept weights in index order, kept being at or above C with w >= min_p.
+  // those with w >= min_p in index order; only entries at or above C count.
   // Entries are narrowed to one of 256 bins of the order's value at a time (equal
   // logits by their indices), and the last few ranked by counting.
   template <Order kOrder>
   __device__ u64 select(int n, u64 need, u64 C) const {
     const int tid = threadIdx.x;
     auto weight_in = [&](u64 c) -> u64 {
+      if (c < C) return 0;
       if constexpr (kOrder == kCount) return 1;
-      if (kOrder == kIndex && (c < C || weight(logit_of(c)) < min_p)) return 0;
+      if (kOrder == kIndex && weight(logit_of(c)) < min_p) return 0;
       return whole(c);
     };
     u64 c[4], q[4];
@@ -619,23 +642,23 @@ struct Sampler {
     return block_sum(s, sm);
   }
 
-  __device__ void long_list(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
+  __device__ void long_list(int n, u64 C, int n_k, bool use_p, u64 bound, uint32_t part, float u,
                             long long* token) const {
-    u64 C = n_k < n ? select<kCount>(n, (u64)n_k, 0) : 0;
+    if (n_k < n) C = select<kCount>(n, (u64)n_k, C);
     if (use_p) {
       if (bound == 0) bound = max(share_of(list_mass(n, C, false), part), (u64)1);
-      C = select<kMass>(n, bound, 0);
+      C = select<kMass>(n, bound, C);
     }
     const u64 target = share_of(list_mass(n, C, true), draw_part(u));
     const u64 c = select<kIndex>(n, target + 1, C);
     if (threadIdx.x == 0) *token = index_of(c);
   }
-  __device__ void draw_from_list(int n, int n_k, bool use_p, u64 bound, uint32_t part, float u,
-                                 long long* token) const {
+  __device__ void draw_from_list(int n, u64 C, int n_k, bool use_p, u64 bound, uint32_t part,
+                                 float u, long long* token) const {
     if (n <= kRank)
-      draw_ranked(n, n_k, use_p, bound, part, u, token);
+      draw_ranked(n, C, n_k, use_p, bound, part, u, token);
     else
-      draw_long_list<kF32>(sm, n, n_k, use_p, bound, part);
+      draw_long_list<kF32>(sm, n, C, n_k, use_p, bound, part);
   }
 
   // -------------------------------------------------------- whole-row draws
@@ -788,10 +811,12 @@ struct Sampler {
 
   // One pass that divides the row by value: this thread's sum of the whole
   // weights above `hi` (where weigh is set) and their number; the tokens of
-  // [lo, hi] at or above C go to the list.
+  // [lo, hi] whose logit is not below C's go to the list (its users leave out
+  // those with C's logit and a higher index).
   __device__ u64 split(float hi, float lo, u64 C, bool weigh, uint32_t& count) const {
     u64 s = 0;
     count = 0;
+    const float least = C ? logit_of(C) : -INFINITY;
     const int end = end_vec();
     for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
       WholeSum w;
@@ -799,14 +824,14 @@ struct Sampler {
 #pragma unroll 2
       for (int j = j0; j < stop; j += 32) {
         const Vec<kF32> x = row.get(j);
-        uint32_t n = 0;
+        uint32_t n = 0, inside = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float v = x.at(e);
-          const int i = j * E - row.mis + e;
           n += v > hi;
-          if (v >= lo && !(v > hi) && (C == 0 || composite(v, i) >= C)) push(v, i);
+          inside |= v >= lo && !(v > hi) && v >= least ? 1u << e : 0u;
         }
+        push(x, j, inside);
         count += n;
         if (n && weigh) {
 #pragma unroll
@@ -863,50 +888,82 @@ struct Sampler {
       each([&](float x, int) { count_in(bins, x, use_p); });
     }
     sync();
-    // This thread's four bins: tokens, and roughly their weight. The rough
-    // weights only choose which bins are looked at; exact sums decide.
+    // Each block takes a run of the bins over the whole row, a thread up to four
+    // of them: tokens, and roughly their weight. The rough weights only choose
+    // which bins are looked at; exact sums decide.
+    const int per = kBins / n_blocks, each_of = (per + kThreads - 1) / kThreads;
+    const int first_bin = (int)rank * per + tid * each_of;
+    const int n_bins = tid * each_of < per ? each_of : 0;
     uint32_t c[4];
     float m[4];
     u64 n_mine = 0;
     float m_mine = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int b = tid * 4 + e;
+      const int b = first_bin + e;
       float heavy = 0.0f;
-      c[e] = 0;
-      for (int r = 0; r < n_blocks; ++r) {
-        c[e] += n_blocks == 1 ? sm.bins[b] : remote_load(remote(&sm.bins[b], r));
-        heavy += n_blocks == 1 ? sm.heavy[b]
-                               : __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+      c[e] = 0, m[e] = 0.0f;
+      if (e >= n_bins) continue;
+      if (n_blocks == 1) {
+        c[e] = sm.bins[b], heavy = sm.heavy[b];
+      } else {
+        for (int r = 0; r < n_blocks; ++r) {
+          c[e] += remote_load(remote(&sm.bins[b], r));
+          heavy += __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+        }
       }
       m[e] = b < bins.light ? heavy
                             : (float)c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
       n_mine += c[e];
       m_mine += m[e];
     }
-    if (tid == 0) sm.count = 0;
-    sync();  // the bins have been read: lists may be written over them
-    u64 n_all;
-    u64 n_before = block_scan(n_mine, n_all, sm);
+    // Tokens and rough weight before this thread's bins: in the block, then in
+    // the blocks before.
+    u64 n_ours;
+    u64 n_before = block_scan(n_mine, n_ours, sm);
+    float m_inc = m_mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, m_inc, off);
+      if (tid % 32 >= off) m_inc += y;
+    }
+    __syncthreads();
+    if (tid % 32 == 31) sm.fpart[tid / 32] = m_inc;
+    __syncthreads();
+    float rough = m_inc - m_mine, m_ours = 0.0f;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < tid / 32) rough += sm.fpart[w];
+      m_ours += sm.fpart[w];
+    }
+    const Pair* all_bins = exchange(n_ours, __float_as_uint(m_ours));
+    u64 n_all = 0;
+    for (int r = 0; r < n_blocks; ++r) {
+      if (r < (int)rank) n_before += all_bins[r].a, rough += __uint_as_float((uint32_t)all_bins[r].b);
+      n_all += all_bins[r].a;
+    }
+    clear_list();  // the bins have been read: lists may be written over them
 
     u64 C = 0;
     u64 mass_k = total;  // exact weight of the top-k, once known
     int last_bin = kBins - 1;
     if (k > 0 && (u64)k < n_all) {
+      if (tid == 0) sm.found = -1;
+      __syncthreads();
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (n_before < (u64)k && (u64)k <= n_before + c[e]) sm.found = tid * 4 + e;
+        if (n_before < (u64)k && (u64)k <= n_before + c[e]) sm.found = first_bin + e;
         n_before += c[e];
       }
       __syncthreads();
-      const int at = sm.found;
+      const Pair* p = exchange((u64)(sm.found + 1), 0);
+      int at = -1;  // one block has it
+      for (int r = 0; r < n_blocks; ++r) at = max(at, (int)p[r].a - 1);
       last_bin = min(kBins - 1, at + 1);
       uint32_t count;
       const u64 mine = split(bins.upper(at - 1), bins.lower(last_bin), 0, use_p || min_p <= 0.0f,
                              count);
       const Pair above = cluster_sum(mine, count);
-      sync();
-      const int n = list_size();
+      const int n = collect_list();
       const int need = (int)((u64)k - above.b);
       if (n <= kCap && above.b < (u64)k && need <= n) {
         u64 within = 0;
@@ -949,44 +1006,36 @@ struct Sampler {
     // neighbours are collected, and the exact sums decide or correct the guess.
     const u64 bound = max(share_of(mass_k, part), (u64)1);
     const float most = C ? logit_of(C) : -INFINITY;
-    float m_inc = m_mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const float y = __shfl_up_sync(0xffffffffu, m_inc, off);
-      if (tid % 32 >= off) m_inc += y;
-    }
-    __syncthreads();
-    if (tid % 32 == 31) sm.fpart[tid / 32] = m_inc;
-    __syncthreads();
-    float rough = m_inc - m_mine;  // before this thread's bins
-    for (int w = 0; w < (int)(tid / 32); ++w) rough += sm.fpart[w];
     float want = (float)bound / kOne;
     for (int tries = 0; tries < 4; ++tries) {
-      sync();
-      if (tid == 0) sm.found = last_bin, sm.count = 0;
-      sync();
+      if (tid == 0) sm.found = last_bin;
+      clear_list();
       float run = rough;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         run += m[e];
-        if (run >= want) {
-          atomicMin(&sm.found, tid * 4 + e);
+        if (e < n_bins && run >= want) {
+          atomicMin(&sm.found, first_bin + e);
           break;
         }
       }
       __syncthreads();
-      const int b0 = max(0, sm.found - 1), b1 = min(last_bin, sm.found + 1);
+      int at = last_bin;
+      {
+        const Pair* p = exchange((u64)sm.found, 0);
+        for (int r = 0; r < n_blocks; ++r) at = min(at, (int)p[r].a);
+      }
+      const int b0 = max(0, at - 1), b1 = min(last_bin, at + 1);
       uint32_t count;
       const u64 mine = split(fmaxf(bins.upper(b0), most), bins.lower(b1), C, true, count);
       const u64 above = cluster_sum(mine);
-      sync();
-      const int n = list_size();
+      const int n = collect_list();
       if (n > kCap) break;
       u64 all = 0;
-      if (rank == 0) all = list_mass(n, 0, false);
+      if (rank == 0) all = list_mass(n, C, false);
       all = exchange(all, 0)[0].a;
       if (above < bound && bound <= above + all) {
-        if (rank == 0) select<kMass>(n, bound - above, 0);
+        if (rank == 0) select<kMass>(n, bound - above, C);
         C = shared_cut();
         if (min_p > 0.0f)
           by_weight(C, u, token);
@@ -999,31 +1048,30 @@ struct Sampler {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (tid * 4 + e == b0) sm.fpart[0] = run;
+        if (e < n_bins && first_bin + e == b0) sm.fpart[0] = run;
         run += m[e];
       }
       __syncthreads();
-      want = sm.fpart[0] + ((float)bound - (float)above) / kOne;
+      const Pair* p = exchange(__float_as_uint(sm.fpart[0]), 0);
+      want = __uint_as_float((uint32_t)p[b0 / per].a) + ((float)bound - (float)above) / kOne;
     }
     by_row(bisect(bound, false, C), u, token);
   }
 
   // ------------------------------------------------------- group candidates
   // Lists the tokens of the groups whose maximum is a candidate, those that are
-  // candidates themselves; returns this thread's whole weight among them. The
-  // list is complete after the next sync().
+  // candidates themselves.
   template <class F>
-  __device__ u64 list_candidates(F candidate) {
+  __device__ void list_candidates(F candidate) {
     const int tid = threadIdx.x;
-    if (tid == 0) sm.n_groups = 0, sm.count = 0;
-    sync();
+    if (tid == 0) sm.n_groups = 0;
+    clear_list();
 #pragma unroll
     for (int g = 0; g < kGroups; ++g)
-      if (candidate(gm.m[g], -1)) sm.groups[atomicAdd(&sm.n_groups, 1)] = group_first(g);
+      if (candidate(gm.m[g])) sm.groups[atomicAdd(&sm.n_groups, 1)] = group_first(g);
     __syncthreads();
     // Their vectors, shared among all threads.
     const int items = sm.n_groups * per_group;
-    u64 listed = 0;
     for (int it0 = tid; it0 < items; it0 += 4 * kThreads) {
       Vec<kF32> x[4];
       int at[4];
@@ -1041,32 +1089,23 @@ struct Sampler {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (at[e] >= 0) {
+          uint32_t bits = 0;
 #pragma unroll
-          for (int i = 0; i < E; ++i) {
-            const float v = x[e].at(i);
-            if (candidate(v, at[e] * E - row.mis + i)) {
-              push(v, at[e] * E - row.mis + i);
-              listed += whole_of(weight(v));
-            }
-          }
+          for (int i = 0; i < E; ++i) bits |= candidate(x[e].at(i)) ? 1u << i : 0u;
+          push(x[e], at[e], bits);
         }
     }
-    return listed;
   }
 
   // Draw among the tokens at or above C with w >= min_p, min_p > 0.
   __device__ void by_weight(u64 C, float u, long long* token) {
-    sync();  // the list before has been read
-    list_candidates([&](float x, int i) {
-      return x > -INFINITY && weight(x) >= min_p && (C == 0 || i < 0 || composite(x, i) >= C);
-    });
-    sync();
-    const int n = list_size();
-    if (n > kCap) {
+    const float least = C ? logit_of(C) : -INFINITY;
+    list_candidates([&](float x) { return x > -INFINITY && x >= least && weight(x) >= min_p; });
+    const int n = collect_list();
+    if (n > kCap)
       by_row(C, u, token);
-    } else if (rank == 0) {
-      draw_from_list(n, n, false, 0, 0, u, token);
-    }
+    else if (rank == 0)
+      draw_from_list(n, C, n, false, 0, 0, u, token);
   }
 
   // --------------------------------------------------------------- one row
@@ -1258,21 +1297,22 @@ struct Sampler {
         draw_by_bins<kF32>(sm, gm, 0, part, 0);
         return;
       }
-      const u64 listed_mine = list_candidates([&](float x, int) {
-        return x > -INFINITY && x >= live && bin_of(x) <= cut;
-      });
-      u64 listed = 0;
+      list_candidates(
+          [&](float x) { return x > -INFINITY && x >= live && bin_of(x) <= cut; });
+      const int n = collect_list();
+      u64 bound = 0;
+      bool enough = n <= kCap;
       if (!use_k) {
-        const Pair s = cluster_sum(mass(), listed_mine);
+        // Rank 0 adds the list's weight, which the others need not know of.
+        const u64 listed = rank == 0 && n <= kCap ? list_mass(n, 0, false) : 0;
+        const Pair s = cluster_sum(mass(), threadIdx.x == 0 ? listed : 0);
         total = s.a;
-        listed = s.b;
+        bound = max(share_of(total, part), (u64)1);
+        enough = enough && s.b >= bound;
       }
-      sync();
-      const int n = list_size();
-      const u64 bound = !use_k ? max(share_of(total, part), (u64)1) : 0;
-      if (n <= kCap && (use_k || listed >= bound)) {
+      if (enough) {
         if (n > kRank) leave(p, least, u, token);
-        if (rank == 0) draw_from_list(n, use_k ? min(n, k) : n, use_p, bound, part, u, token);
+        if (rank == 0) draw_from_list(n, 0, use_k ? min(n, k) : n, use_p, bound, part, u, token);
         return;
       }
     }
@@ -1299,10 +1339,10 @@ __device__ __noinline__ void draw_from_row(Shared& sm, u64 C) {
   s.by_row(C, sm.row.u, sm.row.token);
 }
 template <bool kF32>
-__device__ __noinline__ void draw_long_list(Shared& sm, int n, int n_k, bool use_p, u64 bound,
+__device__ __noinline__ void draw_long_list(Shared& sm, int n, u64 C, int n_k, bool use_p, u64 bound,
                                             uint32_t part) {
   Sampler<kF32> s(sm);
-  s.long_list(n, n_k, use_p, bound, part, sm.row.u, sm.row.token);
+  s.long_list(n, C, n_k, use_p, bound, part, sm.row.u, sm.row.token);
 }
 
 template <bool kF32>
