@@ -22,10 +22,12 @@
 //  * top-p alone: the groups whose maxima carry the wanted share of a total
 //    estimated from the maxima and one vector a thread, one more pass for the
 //    exact total, and the same list, provided that it carries the exact share.
-//  * larger top-k, flatter nuclei: a histogram of the logits (made together with
-//    the exact total) finds the bins around the cut; one pass sums what lies
-//    above them and lists their tokens. The cut and the draw follow from the list
-//    and the warps' sums.
+//  * larger top-k, flatter nuclei: a histogram of a quarter of the logits guesses
+//    the bins around the cut (shared-memory atomics take 1.4 tokens a cycle, so
+//    one of all the logits cost 92 us of 256 rows of 131072); one pass sums what
+//    lies above them, and the total where it is not known, and lists their
+//    tokens. The exact sums confirm the guess or correct it for another pass.
+//    The cut and the draw follow from the list and the warps' sums.
 //  * rows that defeat the bins (thousands of equal logits at the cut): bisection
 //    over the composite, one pass per bit.
 // With temperature alone one pass sums the row in ranges and the range that
@@ -51,6 +53,8 @@ constexpr int kRank = 256;       // entries that are ranked by counting
 constexpr int kMaxCluster = 8;
 constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
+constexpr int kTries = 16;       // passes with guessed bins (the last halve what is left)
+constexpr int kWindow = 650;     // tokens listed to each side of a guessed cut
 constexpr float kOne = 1099511627776.0f;  // 2^40
 constexpr uint32_t kNoCut = ~0u;  // in place of a top-p share
 constexpr float kLive = 28.0f;   // weights below exp(-28) < 2^-40 are zero
@@ -219,6 +223,7 @@ struct Shared {
       float heavy[kBins];    // those above 2^-10 of the largest
     };
   };
+  float cum_n[kBins], cum_m[kBins];  // guessed tokens and weight before each bin
   u64 q[kRank];           // whole weights of entries that are ranked
   u64 mass[kGroupBins];   // of the entries in select()'s bins
   u64 part[kWarps];
@@ -249,6 +254,9 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
 }
 __device__ __forceinline__ void remote_store(uint32_t addr, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void remote_store32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ u64 remote_load64(uint32_t addr) {
   u64 v;
@@ -425,6 +433,20 @@ struct Sampler {
         }
     }
   }
+  // f(vector, its number) likewise, for the vectors from j0 to below end,
+  // `apart` apart.
+  template <class F>
+  __device__ __forceinline__ void each_vec(int j0, int end, int apart, F f) const {
+    for (int j = j0; j < end; j += 4 * apart) {
+      Vec<kF32> x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + apart * u < end) x[u] = row.get(j + apart * u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + apart * u < end) f(x[u], j + apart * u);
+    }
+  }
   // ... for every logit that this thread reads.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
@@ -441,10 +463,7 @@ struct Sampler {
     }
     for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {  // at most 1024 logits a stretch
       WholeSum w;
-      const int stop = min(end, j0 + 32 * 128);
-#pragma unroll 2
-      for (int j = j0; j < stop; j += 32) {
-        const Vec<kF32> x = row.get(j);
+      each_vec(j0, min(end, j0 + 32 * 128), 32, [&](const Vec<kF32>& x, int) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           // NaN and -inf take the bound, whose weight is zero; at the top the
@@ -452,7 +471,7 @@ struct Sampler {
           const float a = fmaxf((x.at(e) - top) * inv_t, -100.0f);
           w.add(expf(a));
         }
-      }
+      });
       s += w.total();
     }
     return s;
@@ -788,42 +807,19 @@ struct Sampler {
     for (int t = threadIdx.x; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
     __syncthreads();
   }
-  // mass() and the histogram in one pass.
-  __device__ u64 mass_and_bins(const Bins& bins) const {
-    clear_bins();
-    u64 s = 0;
-    const int end = end_vec();
-    for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
-      WholeSum w;
-      const int stop = min(end, j0 + 32 * 128);
-      for (int j = j0; j < stop; j += 32) {
-        const Vec<kF32> x = row.get(j);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          w.add(x.at(e) > -INFINITY ? weight(x.at(e)) : 0.0f);
-          count_in(bins, x.at(e), true);
-        }
-      }
-      s += w.total();
-    }
-    return s;
-  }
-
   // One pass that divides the row by value: this thread's sum of the whole
-  // weights above `hi` (where weigh is set) and their number; the tokens of
-  // [lo, hi] whose logit is not below C's go to the list (its users leave out
-  // those with C's logit and a higher index).
-  __device__ u64 split(float hi, float lo, u64 C, bool weigh, uint32_t& count) const {
+  // weights above `hi` (where weigh is set) and their number, and with kAll the
+  // sum of all; the tokens of [lo, hi] whose logit is not below C's go to the
+  // list (its users leave out those with C's logit and a higher index).
+  template <bool kAll>
+  __device__ u64 split(float hi, float lo, u64 C, bool weigh, uint32_t& count, u64& all) const {
     u64 s = 0;
     count = 0;
     const float least = C ? logit_of(C) : -INFINITY;
     const int end = end_vec();
     for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
-      WholeSum w;
-      const int stop = min(end, j0 + 32 * 128);
-#pragma unroll 2
-      for (int j = j0; j < stop; j += 32) {
-        const Vec<kF32> x = row.get(j);
+      WholeSum w, a;
+      each_vec(j0, min(end, j0 + 32 * 128), 32, [&](const Vec<kF32>& x, int j) {
         uint32_t n = 0, inside = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -833,12 +829,18 @@ struct Sampler {
         }
         push(x, j, inside);
         count += n;
-        if (n && weigh) {
+        if (kAll || (n && weigh)) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) w.add(x.at(e) > hi ? weight(x.at(e)) : 0.0f);
+          for (int e = 0; e < E; ++e) {
+            const float v = x.at(e);
+            const float f = kAll ? (v > -INFINITY ? weight(v) : 0.0f) : weight(v);
+            w.add(v > hi ? f : 0.0f);
+            if (kAll) a.add(f);
+          }
         }
-      }
+      });
       s += w.total();
+      if (kAll) all += a.total();
     }
     return s;
   }
@@ -875,112 +877,166 @@ struct Sampler {
     if (w / kWarps == (int)rank) draw_from_range(w, target, C, token);
   }
 
-  // The draw where the cuts go by histogram (see the head of the file). k <= 0:
-  // no top-k, then `total` is the row's weight where it is known (else 0).
-  __device__ void by_bins(int k, bool use_p, uint32_t part, u64 total, float least, float u,
-                          long long* token) {
+  // Fills cum_n and cum_m of every block from a sample of the row.
+  __device__ void guess_bins(const Bins& bins, bool weigh) {
     const int tid = threadIdx.x;
-    const Bins bins = bins_over(least);
-    if (k <= 0 && total == 0) {
-      total = cluster_sum(mass_and_bins(bins));
-    } else {
-      clear_bins();
-      each([&](float x, int) { count_in(bins, x, use_p); });
-    }
+    clear_bins();
+    const int every = per_warp / 32 > 8 ? 4 : 1;
+    const int end = end_vec();
+    each_vec(first_vec(), end, 32 * every, [&](const Vec<kF32>& x, int) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) count_in(bins, x.at(e), weigh);
+    });
     sync();
     // Each block takes a run of the bins over the whole row, a thread up to four
-    // of them: tokens, and roughly their weight. The rough weights only choose
-    // which bins are looked at; exact sums decide.
+    // of them: tokens, and roughly their weight.
     const int per = kBins / n_blocks, each_of = (per + kThreads - 1) / kThreads;
     const int first_bin = (int)rank * per + tid * each_of;
     const int n_bins = tid * each_of < per ? each_of : 0;
-    uint32_t c[4];
-    float m[4];
-    u64 n_mine = 0;
-    float m_mine = 0.0f;
+    float c[4], m[4], c_mine = 0.0f, m_mine = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int b = first_bin + e;
       float heavy = 0.0f;
-      c[e] = 0, m[e] = 0.0f;
-      if (e >= n_bins) continue;
-      if (n_blocks == 1) {
-        c[e] = sm.bins[b], heavy = sm.heavy[b];
-      } else {
-        for (int r = 0; r < n_blocks; ++r) {
-          c[e] += remote_load(remote(&sm.bins[b], r));
-          heavy += __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+      uint32_t n = 0;
+      if (e < n_bins) {
+        if (n_blocks == 1) {
+          n = sm.bins[b], heavy = sm.heavy[b];
+        } else {
+          for (int r = 0; r < n_blocks; ++r) {
+            n += remote_load(remote(&sm.bins[b], r));
+            heavy += __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+          }
         }
       }
-      m[e] = b < bins.light ? heavy
-                            : (float)c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
-      n_mine += c[e];
+      c[e] = (float)n * (float)every;
+      m[e] = b < bins.light ? heavy * (float)every
+                            : c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
+      c_mine += c[e];
       m_mine += m[e];
     }
-    // Tokens and rough weight before this thread's bins: in the block, then in
-    // the blocks before.
-    u64 n_ours;
-    u64 n_before = block_scan(n_mine, n_ours, sm);
-    float m_inc = m_mine;
+    float c_inc = c_mine, m_inc = m_mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
+      const float x = __shfl_up_sync(0xffffffffu, c_inc, off);
       const float y = __shfl_up_sync(0xffffffffu, m_inc, off);
-      if (tid % 32 >= off) m_inc += y;
+      if (tid % 32 >= off) c_inc += x, m_inc += y;
     }
     __syncthreads();
-    if (tid % 32 == 31) sm.fpart[tid / 32] = m_inc;
+    if (tid % 32 == 31)
+      sm.part[tid / 32] = ((u64)__float_as_uint(c_inc) << 32) | __float_as_uint(m_inc);
     __syncthreads();
-    float rough = m_inc - m_mine, m_ours = 0.0f;
+    float c_run = c_inc - c_mine, m_run = m_inc - m_mine, c_ours = 0.0f, m_ours = 0.0f;
     for (int w = 0; w < kWarps; ++w) {
-      if (w < tid / 32) rough += sm.fpart[w];
-      m_ours += sm.fpart[w];
+      const float x = __uint_as_float((uint32_t)(sm.part[w] >> 32));
+      const float y = __uint_as_float((uint32_t)sm.part[w]);
+      if (w < tid / 32) c_run += x, m_run += y;
+      c_ours += x, m_ours += y;
     }
-    const Pair* all_bins = exchange(n_ours, __float_as_uint(m_ours));
-    u64 n_all = 0;
-    for (int r = 0; r < n_blocks; ++r) {
-      if (r < (int)rank) n_before += all_bins[r].a, rough += __uint_as_float((uint32_t)all_bins[r].b);
-      n_all += all_bins[r].a;
+    const Pair* p = exchange(__float_as_uint(c_ours), __float_as_uint(m_ours));
+    for (int r = 0; r < (int)rank; ++r) {
+      c_run += __uint_as_float((uint32_t)p[r].a);
+      m_run += __uint_as_float((uint32_t)p[r].b);
     }
-    clear_list();  // the bins have been read: lists may be written over them
-
-    u64 C = 0;
-    u64 mass_k = total;  // exact weight of the top-k, once known
-    int last_bin = kBins - 1;
-    if (k > 0 && (u64)k < n_all) {
-      if (tid == 0) sm.found = -1;
-      __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n_before < (u64)k && (u64)k <= n_before + c[e]) sm.found = first_bin + e;
-        n_before += c[e];
-      }
-      __syncthreads();
-      const Pair* p = exchange((u64)(sm.found + 1), 0);
-      int at = -1;  // one block has it
-      for (int r = 0; r < n_blocks; ++r) at = max(at, (int)p[r].a - 1);
-      last_bin = min(kBins - 1, at + 1);
-      uint32_t count;
-      const u64 mine = split(bins.upper(at - 1), bins.lower(last_bin), 0, use_p || min_p <= 0.0f,
-                             count);
-      const Pair above = cluster_sum(mine, count);
-      const int n = collect_list();
-      const int need = (int)((u64)k - above.b);
-      if (n <= kCap && above.b < (u64)k && need <= n) {
-        u64 within = 0;
-        if (rank == 0) {
-          const u64 c = select<kCount>(n, (u64)need, 0);
-          within = list_mass(n, c, false);
-        }
-        C = shared_cut();
-        if (!use_p) {
-          if (min_p > 0.0f)
-            by_weight(C, u, token);
-          else
-            draw_from_split(mine, n, C, u, token);
-          return;
-        }
-        mass_k = above.a + exchange(within, 0)[0].a;
+    for (int e = 0; e < 4; ++e) {
+      if (e >= n_bins) break;
+      const int b = first_bin + e;
+      if (n_blocks == 1) {
+        sm.cum_n[b] = c_run, sm.cum_m[b] = m_run;
       } else {
+        for (int r = 0; r < n_blocks; ++r) {
+          remote_store32(remote(&sm.cum_n[b], r), __float_as_uint(c_run));
+          remote_store32(remote(&sm.cum_m[b], r), __float_as_uint(m_run));
+        }
+      }
+      c_run += c[e], m_run += m[e];
+    }
+    sync();
+  }
+  // The last bin before which `cum` is below `want`.
+  __device__ __forceinline__ int bin_at(const float* cum, float want) const {
+    int lo = 0, hi = kBins - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (cum[mid] < want)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    return lo;
+  }
+  // The bin to look at next: where `want` is guessed, within the bins that are
+  // left; after three misses the one that halves them.
+  __device__ __forceinline__ int guess(const float* cum, float want, int tries, int from,
+                                       int upto) const {
+    return tries < 3 ? max(from, min(upto, bin_at(cum, want))) : (from + upto) / 2;
+  }
+  // The bins around bin `at`, `half` tokens to each side.
+  __device__ __forceinline__ void window(int at, float half, int& b0, int& b1) const {
+    b0 = min(max(0, at - 1), bin_at(sm.cum_n, sm.cum_n[at] - half));
+    b1 = max(min(kBins - 1, at + 1), bin_at(sm.cum_n, sm.cum_n[min(kBins - 1, at + 1)] + half));
+  }
+
+  // The draw where the cuts go by histogram (see the head of the file). k <= 0:
+  // no top-k, then `total` is the row's weight where it is known (else 0).
+  __device__ void by_bins(int k, bool use_p, uint32_t part, u64 total, float least, float u,
+                          long long* token) {
+    const Bins bins = bins_over(least);
+    guess_bins(bins, use_p);
+    u64 C = 0, none = 0;
+    uint32_t count;
+    if (k > 0) {
+      bool known = false;
+      float want = (float)k, half = kWindow;
+      int from = 0, upto = kBins - 1;  // bins that can hold the cut
+      for (int tries = 0; tries < kTries && !known; ++tries) {
+        int b0, b1;
+        window(guess(sm.cum_n, want, tries, from, upto), half, b0, b1);
+        clear_list();
+        const u64 mine = split<false>(bins.upper(b0), bins.lower(b1), 0, use_p || min_p <= 0.0f,
+                                      count, none);
+        const Pair above = cluster_sum(mine, count);
+        const int n = collect_list();
+        if (n > kCap) {
+          half *= 0.25f;
+        } else if (above.b < (u64)k && (u64)k <= above.b + n) {
+          u64 within = 0;
+          if (rank == 0) {
+            const u64 c = select<kCount>(n, (u64)k - above.b, 0);
+            within = list_mass(n, c, false);
+          }
+          C = shared_cut();
+          if (!use_p) {
+            if (min_p > 0.0f)
+              by_weight(C, u, token);
+            else
+              draw_from_split(mine, n, C, u, token);
+            return;
+          }
+          total = above.a + exchange(within, 0)[0].a;
+          known = true;
+        } else if (b1 == kBins - 1 && above.b < (u64)k) {  // fewer live tokens: all are kept
+          if (!use_p) {
+            if (min_p > 0.0f)
+              by_weight(0, u, token);
+            else
+              draw_from_split(mine, n, 0, u, token);
+            return;
+          }
+          u64 within = 0;
+          if (rank == 0) within = list_mass(n, 0, false);
+          total = above.a + exchange(within, 0)[0].a;
+          known = true;
+        } else {
+          want = sm.cum_n[b0] + ((float)k - (float)above.b);
+          if (above.b >= (u64)k)
+            upto = max(from, b0);
+          else
+            from = min(upto, b1);
+        }
+      }
+      if (!known) {
         C = bisect((u64)k, true, 0);
         if (!use_p) {
           by_row(C, u, token);
@@ -990,51 +1046,42 @@ struct Sampler {
         each([&](float x, int i) {
           if (x > -INFINITY && composite(x, i) >= C) s += whole_of(weight(x));
         });
-        mass_k = cluster_sum(s);
+        total = cluster_sum(s);
       }
-    } else if (!use_p) {  // fewer live tokens than k: all are kept
-      if (min_p > 0.0f)
-        by_weight(0, u, token);
-      else
-        by_row(0, u, token);
-      return;
-    } else if (total == 0) {
-      mass_k = cluster_sum(mass());
     }
-
-    // The bin that the mass bound falls into, by the rough weights; it and its
-    // neighbours are collected, and the exact sums decide or correct the guess.
-    const u64 bound = max(share_of(mass_k, part), (u64)1);
+    // Where the weight reaches its share.
     const float most = C ? logit_of(C) : -INFINITY;
-    float want = (float)bound / kOne;
-    for (int tries = 0; tries < 4; ++tries) {
-      if (tid == 0) sm.found = last_bin;
+    const float share = (float)part * (1.0f / 16777216.0f);
+    // (an unknown total is guessed too: the last bin's start is nearly all)
+    float want = total ? (float)total / kOne * share : sm.cum_m[kBins - 1] * share;
+    float half = kWindow;
+    int from = 0, upto = kBins - 1;
+    for (int tries = 0; tries < kTries; ++tries) {
+      int b0, b1;
+      window(guess(sm.cum_m, want, tries, from, upto), half, b0, b1);
       clear_list();
-      float run = rough;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        run += m[e];
-        if (e < n_bins && run >= want) {
-          atomicMin(&sm.found, first_bin + e);
-          break;
-        }
+      const float hi = fmaxf(bins.upper(b0), most), lo = bins.lower(b1);
+      u64 mine, above;
+      if (total) {
+        mine = split<false>(hi, lo, C, true, count, none);
+        above = cluster_sum(mine);
+      } else {
+        u64 all = 0;
+        mine = split<true>(hi, lo, C, true, count, all);
+        const Pair sums = cluster_sum(mine, all);
+        above = sums.a;
+        total = sums.b;
       }
-      __syncthreads();
-      int at = last_bin;
-      {
-        const Pair* p = exchange((u64)sm.found, 0);
-        for (int r = 0; r < n_blocks; ++r) at = min(at, (int)p[r].a);
-      }
-      const int b0 = max(0, at - 1), b1 = min(last_bin, at + 1);
-      uint32_t count;
-      const u64 mine = split(fmaxf(bins.upper(b0), most), bins.lower(b1), C, true, count);
-      const u64 above = cluster_sum(mine);
       const int n = collect_list();
-      if (n > kCap) break;
-      u64 all = 0;
-      if (rank == 0) all = list_mass(n, C, false);
-      all = exchange(all, 0)[0].a;
-      if (above < bound && bound <= above + all) {
+      const u64 bound = max(share_of(total, part), (u64)1);
+      if (n > kCap) {
+        half *= 0.25f;
+        continue;
+      }
+      u64 listed = 0;
+      if (rank == 0) listed = list_mass(n, C, false);
+      listed = exchange(listed, 0)[0].a;
+      if (above < bound && bound <= above + listed) {
         if (rank == 0) select<kMass>(n, bound - above, C);
         C = shared_cut();
         if (min_p > 0.0f)
@@ -1043,19 +1090,14 @@ struct Sampler {
           draw_from_split(mine, n, C, u, token);
         return;
       }
-      // The rough sum at the start of bin b0 is off by what the exact one says.
-      run = rough;
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e < n_bins && first_bin + e == b0) sm.fpart[0] = run;
-        run += m[e];
-      }
-      __syncthreads();
-      const Pair* p = exchange(__float_as_uint(sm.fpart[0]), 0);
-      want = __uint_as_float((uint32_t)p[b0 / per].a) + ((float)bound - (float)above) / kOne;
+      // The guess before bin b0 is off by what the exact sum says.
+      want = sm.cum_m[b0] + ((float)bound - (float)above) / kOne;
+      if (above >= bound)
+        upto = max(from, b0);
+      else
+        from = min(upto, b1);
     }
-    by_row(bisect(bound, false, C), u, token);
+    by_row(bisect(max(share_of(total, part), (u64)1), false, C), u, token);
   }
 
   // ------------------------------------------------------- group candidates
