@@ -54,7 +54,11 @@ constexpr int kMaxCluster = 8;
 constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
 constexpr int kTries = 16;       // passes with guessed bins (the last halve what is left)
-constexpr int kWindow = 650;     // tokens listed to each side of a guessed cut
+// One vector in kSample goes into the histogram, kWindow tokens are listed to
+// each side of a guessed cut. Measured (256 flat rows of 131072, top-p 0.9, us):
+// 4 and 650: 185, 8 and 800: 255 (more wrong guesses), 4 and 300: 198.
+constexpr int kSample = 4;
+constexpr int kWindow = 650;
 constexpr float kOne = 1099511627776.0f;  // 2^40
 constexpr uint32_t kNoCut = ~0u;  // in place of a top-p share
 constexpr float kLive = 28.0f;   // weights below exp(-28) < 2^-40 are zero
@@ -204,6 +208,10 @@ __device__ __forceinline__ uint32_t index_of(u64 comp) { return ~(uint32_t)comp;
 struct Pair {
   u64 a, b;
 };
+struct Sums {
+  u64 above, all;
+  uint32_t count;
+};
 
 // What a block knows about its row, for the paths that are functions of their
 // own: inlined they would take the common path's registers.
@@ -317,6 +325,9 @@ struct Groups {  // maxima of a thread's groups
 };
 template <bool kF32>
 __device__ __noinline__ void draw_by_bins(Shared& sm, Groups gm, int k, uint32_t part, u64 total);
+template <bool kF32>
+__device__ __noinline__ Sums split_row(Shared& sm, float hi, float lo, float least, bool weigh,
+                                       bool all);
 template <bool kF32>
 __device__ __noinline__ void draw_by_weight(Shared& sm, Groups gm, u64 C);
 template <bool kF32>
@@ -797,25 +808,24 @@ struct Sampler {
     b.light = b.of(top - 7.0f / inv_t);
     return b;
   }
-  __device__ __forceinline__ void count_in(const Bins& bins, float x, bool weigh) const {
+  __device__ __forceinline__ void count_in(const Bins& bins, float x, bool weigh, int n) const {
     if (!(x >= bins.low)) return;
     const int b = bins.of(x);
-    atomicAdd(&sm.bins[b], 1u);
-    if (b < bins.light && weigh) atomicAdd(&sm.heavy[b], __expf((x - top) * inv_t));
+    atomicAdd(&sm.bins[b], (uint32_t)n);
+    if (b < bins.light && weigh)
+      atomicAdd(&sm.heavy[b], (float)n * (x == top ? 1.0f : __expf((x - top) * inv_t)));
   }
   __device__ void clear_bins() const {
     for (int t = threadIdx.x; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
     __syncthreads();
   }
   // One pass that divides the row by value: this thread's sum of the whole
-  // weights above `hi` (where weigh is set) and their number, and with kAll the
-  // sum of all; the tokens of [lo, hi] whose logit is not below C's go to the
+  // weights above `hi` (where weigh is set), their number, and where asked for
+  // the sum of all; the tokens of [lo, hi] that are not below `least` go to the
   // list (its users leave out those with C's logit and a higher index).
-  template <bool kAll>
-  __device__ u64 split(float hi, float lo, u64 C, bool weigh, uint32_t& count, u64& all) const {
-    u64 s = 0;
-    count = 0;
-    const float least = C ? logit_of(C) : -INFINITY;
+  __device__ Sums split(float hi, float lo, float least, bool weigh, bool all) const {
+    Sums s{0, 0, 0};
+    lo = fmaxf(lo, least);
     const int end = end_vec();
     for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
       WholeSum w, a;
@@ -825,22 +835,22 @@ struct Sampler {
         for (int e = 0; e < E; ++e) {
           const float v = x.at(e);
           n += v > hi;
-          inside |= v >= lo && !(v > hi) && v >= least ? 1u << e : 0u;
+          inside |= v >= lo && !(v > hi) ? 1u << e : 0u;
         }
         push(x, j, inside);
-        count += n;
-        if (kAll || (n && weigh)) {
+        s.count += n;
+        if (all || (n && weigh)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             const float v = x.at(e);
-            const float f = kAll ? (v > -INFINITY ? weight(v) : 0.0f) : weight(v);
+            const float f = v > -INFINITY ? weight(v) : 0.0f;
             w.add(v > hi ? f : 0.0f);
-            if (kAll) a.add(f);
+            a.add(f);
           }
         }
       });
-      s += w.total();
-      if (kAll) all += a.total();
+      s.above += w.total();
+      s.all += a.total();
     }
     return s;
   }
@@ -877,15 +887,21 @@ struct Sampler {
     if (w / kWarps == (int)rank) draw_from_range(w, target, C, token);
   }
 
-  // Fills cum_n and cum_m of every block from a sample of the row.
+  // Fills cum_n and cum_m of every block from the groups' maxima and a sample of
+  // the rest of the row: a few heavy tokens, mostly maxima, may carry much of it.
   __device__ void guess_bins(const Bins& bins, bool weigh) {
     const int tid = threadIdx.x;
     clear_bins();
-    const int every = per_warp / 32 > 8 ? 4 : 1;
+    const int every = per_warp / 32 > 8 ? kSample : 1;
     const int end = end_vec();
-    each_vec(first_vec(), end, 32 * every, [&](const Vec<kF32>& x, int) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) count_in(bins, x.at(e), weigh);
+    for (int g = 0; g < kGroups; ++g) count_in(bins, gm.m[g], weigh, 1);
+    each_vec(first_vec(), end, 32 * every, [&](const Vec<kF32>& x, int j) {
+      const int g = (j - first_vec()) / 32 / per_group;
+      const float most = g & 2 ? (g & 1 ? gm.m[3] : gm.m[2]) : (g & 1 ? gm.m[1] : gm.m[0]);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x.at(e) < most) count_in(bins, x.at(e), weigh, every);
     });
     sync();
     // Each block takes a run of the bins over the whole row, a thread up to four
@@ -909,8 +925,8 @@ struct Sampler {
           }
         }
       }
-      c[e] = (float)n * (float)every;
-      m[e] = b < bins.light ? heavy * (float)every
+      c[e] = (float)n;
+      m[e] = b < bins.light ? heavy
                             : c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
       c_mine += c[e];
       m_mine += m[e];
@@ -984,8 +1000,7 @@ struct Sampler {
                           long long* token) {
     const Bins bins = bins_over(least);
     guess_bins(bins, use_p);
-    u64 C = 0, none = 0;
-    uint32_t count;
+    u64 C = 0;
     if (k > 0) {
       bool known = false;
       float want = (float)k, half = kWindow;
@@ -994,9 +1009,10 @@ struct Sampler {
         int b0, b1;
         window(guess(sm.cum_n, want, tries, from, upto), half, b0, b1);
         clear_list();
-        const u64 mine = split<false>(bins.upper(b0), bins.lower(b1), 0, use_p || min_p <= 0.0f,
-                                      count, none);
-        const Pair above = cluster_sum(mine, count);
+        const Sums sums = split_row<kF32>(sm, bins.upper(b0), bins.lower(b1), -INFINITY,
+                                          use_p || min_p <= 0.0f, false);
+        const u64 mine = sums.above;
+        const Pair above = cluster_sum(mine, sums.count);
         const int n = collect_list();
         if (n > kCap) {
           half *= 0.25f;
@@ -1061,17 +1077,11 @@ struct Sampler {
       window(guess(sm.cum_m, want, tries, from, upto), half, b0, b1);
       clear_list();
       const float hi = fmaxf(bins.upper(b0), most), lo = bins.lower(b1);
-      u64 mine, above;
-      if (total) {
-        mine = split<false>(hi, lo, C, true, count, none);
-        above = cluster_sum(mine);
-      } else {
-        u64 all = 0;
-        mine = split<true>(hi, lo, C, true, count, all);
-        const Pair sums = cluster_sum(mine, all);
-        above = sums.a;
-        total = sums.b;
-      }
+      const Sums sums = split_row<kF32>(sm, hi, lo, most, true, total == 0);
+      const u64 mine = sums.above;
+      const Pair both = cluster_sum(mine, sums.all);
+      const u64 above = both.a;
+      if (total == 0) total = both.b;
       const int n = collect_list();
       const u64 bound = max(share_of(total, part), (u64)1);
       if (n > kCap) {
@@ -1368,6 +1378,11 @@ __device__ __noinline__ void draw_by_bins(Shared& sm, Groups gm, int k, uint32_t
   Sampler<kF32> s(sm);
   s.gm = gm;
   s.by_bins(k, part != kNoCut, part, total, sm.row.least, sm.row.u, sm.row.token);
+}
+template <bool kF32>
+__device__ __noinline__ Sums split_row(Shared& sm, float hi, float lo, float least, bool weigh,
+                                       bool all) {
+  return Sampler<kF32>(sm).split(hi, lo, least, weigh, all);
 }
 template <bool kF32>
 __device__ __noinline__ void draw_by_weight(Shared& sm, Groups gm, u64 C) {
