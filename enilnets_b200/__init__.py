@@ -10,6 +10,8 @@ Python host side that mirrors the reference's layer interface:
 * AttentionNet (alias NeuralNet): same layer dicts, Forward on the device
 * KVCache / cached_forward_step: device-resident incremental decoding
 * graph.MultiHeadAttention: key-padding-mask attention
+* PagedKVCache / paged_forward_step / TextGenerator.serve: ragged batches over a
+  paged cache, with on-device sampling
 * kernels: one tensor-level wrapper per C-ABI entry point
 """
 __version__ = "0.2.0"
@@ -22,5 +24,6 @@ from .layers import (add_cross_attention, add_multihead_attention,  # noqa: F401
                      add_transformer_block, init_weights)
 from .network import AttentionNet  # noqa: F401
 from .generation import TextGenerator  # noqa: F401
+from .serving import PagedKVCache, paged_forward_step  # noqa: F401
 
 NeuralNet = AttentionNet

@@ -157,6 +157,42 @@ def project(x, layer: dict, which: str, rope_pos0: Optional[int] = None, out_dty
     return (y, rope is not None) if rope_pos0 is not None else y
 
 
+def qk_norm_args(layer: dict):
+    """(q_weight, k_weight, eps) of a layer's query/key norms on the device, or
+    (None, None, 0.0) for a layer without."""
+    import torch
+    if layer.get("q_norm") is None:
+        return None, None, 0.0
+    return (_WEIGHTS.get(layer, ("q_norm",), "b", torch.float32),
+            _WEIGHTS.get(layer, ("k_norm",), "b", torch.float32),
+            float(layer.get("qk_norm_eps", 1e-6)))
+
+
+def project_qkv(layer: dict, x, pos0: int):
+    """(q, k, v) head views of one fused projection, normalised and rotated as
+    the layer asks, at positions pos0 + s: the rotation runs in the projection's
+    epilogue, or with the norms in one pass after it."""
+    H, D = layer["num_heads"], layer["head_dim"]
+    Hkv = layer.get("num_kv_heads") or H
+    rope = layer.get("positional_scheme", "absolute") == "rope"
+    normed = layer.get("q_norm") is not None
+    if rope and not normed:
+        qkv, rotated = project(x, layer, "qkv", rope_pos0=pos0)
+    else:
+        qkv, rotated = project(x, layer, "qkv"), not rope
+    q = split_heads(qkv, H, D, 0)
+    k = split_heads(qkv, Hkv, D, H * D)
+    v = split_heads(qkv, Hkv, D, H * D + Hkv * D)
+    if normed:
+        wq, wk, eps = qk_norm_args(layer)
+        kernels.qk_norm_rope(q, k, wq, wk, eps=eps, pos0=pos0, out=(q, k),
+                             rope=rope_tables(pos0 + x.shape[-2], D) if rope else None)
+    elif not rotated:
+        apply_rope(q, pos0)
+        apply_rope(k, pos0)
+    return q, k, v
+
+
 def split_heads(t, heads: int, head_dim: int, offset: int = 0):
     """(B, S, *) -> strided (B, S, heads, head_dim) view at column offset."""
     return t[..., offset:offset + heads * head_dim].unflatten(-1, (heads, head_dim))
@@ -225,16 +261,7 @@ def self_attention(layer: dict, x, key_padding_mask=None, mask_mode: Optional[st
     H, D = layer["num_heads"], layer["head_dim"]
     Hkv = layer.get("num_kv_heads") or H
     scheme = layer.get("positional_scheme", "absolute")
-    if scheme == "rope":
-        qkv, rotated = project(x, layer, "qkv", rope_pos0=0)
-    else:
-        qkv, rotated = project(x, layer, "qkv"), True
-    q = split_heads(qkv, H, D, 0)
-    k = split_heads(qkv, Hkv, D, H * D)
-    v = split_heads(qkv, Hkv, D, H * D + Hkv * D)
-    if not rotated:
-        apply_rope(q, 0)
-        apply_rope(k, 0)
+    q, k, v = project_qkv(layer, x, 0)
     if layer.get("attention_kernel", "softmax") in LINEAR_KERNELS:
         if key_padding_mask is not None:
             raise ValueError("key_padding_mask is not supported with a linearized "

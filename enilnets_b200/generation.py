@@ -303,6 +303,57 @@ class TextGenerator:
                 for ids in self.batch_ids(prompts, max_new_tokens, temperature, top_p, top_k,
                                           greedy)]
 
+    def serve_ids(self, prompts: List[str], max_new_tokens: int = 100, temperature: float = 1.0,
+                  top_p: Optional[float] = None, top_k: Optional[int] = None,
+                  min_p: Optional[float] = None, greedy: bool = False, page_size: int = 16,
+                  window: Optional[int] = None, sinks: int = 0) -> List[List[int]]:
+        """Token ids of `serve`, one list per prompt in order: all prompts as one
+        ragged batch over a paged cache, the next tokens drawn on the device with
+        one number of NumPy's global RNG for each live sequence and step. A single
+        prompt draws as `generate` does."""
+        from .serving import PagedKVCache, paged_forward_step, sample
+        if not prompts:
+            return []
+        end_id = self._id(self.tokenizer.end_token)
+        seqs = [self._prompt_ids(p) for p in prompts]
+        # As generate: a step follows every token but the last, up to max_seq_len.
+        most = [min(self.max_seq_len, len(s) + max_new_tokens) for s in seqs]
+        pages = sum(-(-n // page_size) for n in most)
+        cache = PagedKVCache(pages, page_size, self.max_seq_len, window=window, sinks=sinks)
+        live = list(range(len(seqs)))
+        handle = [cache.add() for _ in seqs]
+        step = [s[-self.max_seq_len:] for s in seqs]
+        logits = paged_forward_step(self.network, step, cache, handle)
+        for _ in range(max_new_tokens):
+            drawn = sample(logits, np.random.random_sample(len(live)), temperature, top_p, top_k,
+                           min_p, greedy)
+            step, rest = [], []
+            for b, tok in zip(live, drawn):
+                if tok != end_id:
+                    seqs[b].append(tok)
+                if tok == end_id or cache.length[handle[b]] >= self.max_seq_len:
+                    cache.release(handle[b])
+                else:
+                    step.append([tok])
+                    rest.append(b)
+            live = rest
+            if not live:
+                break
+            logits = paged_forward_step(self.network, step, cache, [handle[b] for b in live])
+        return seqs
+
+    def serve(self, prompts: List[str], max_new_tokens: int = 100, temperature: float = 1.0,
+              top_p: Optional[float] = None, top_k: Optional[int] = None,
+              min_p: Optional[float] = None, greedy: bool = False, page_size: int = 16,
+              window: Optional[int] = None, sinks: int = 0) -> List[str]:
+        """Texts for prompts of any lengths, decoded together over a paged cache
+        with on-device sampling (generate_batch groups prompts by length and
+        samples on the host). window, sinks: a streaming cache that keeps the last
+        `window` positions and the first `sinks`."""
+        return [self.tokenizer.decode(ids, skip_special=True)
+                for ids in self.serve_ids(prompts, max_new_tokens, temperature, top_p, top_k, min_p,
+                                          greedy, page_size, window, sinks)]
+
     def perplexity(self, text: str) -> float:
         """exp(mean next-token cross-entropy) over `text`, in non-overlapping
         windows of up to max_seq_len - 1 tokens (text_generation.py:383-398)."""

@@ -167,27 +167,17 @@ def attention_step(layer: Dict[str, Any], x, idx: int, cache: KVCache, B: int, S
     Hkv = layer.get("num_kv_heads") or H
     scheme = layer.get("positional_scheme", "absolute")
     window = layer.get("window_size")
-    if scheme == "rope":
-        # Rotated at absolute positions in the projection's epilogue; the
-        # cache stores rotated K.
-        qkv, rotated = attention.project(x, layer, "qkv", rope_pos0=pos)
-    else:
-        qkv, rotated = attention.project(x, layer, "qkv"), True
-    q = attention.split_heads(qkv, H, D, 0)
-    k_new = attention.split_heads(qkv, Hkv, D, H * D)
-    v_new = attention.split_heads(qkv, Hkv, D, H * D + Hkv * D)
-    if not rotated:
-        attention.apply_rope(q, pos)
-        attention.apply_rope(k_new, pos)
+    # Rotated at absolute positions; the cache stores normalised and rotated K.
+    q, k_new, v_new = attention.project_qkv(layer, x, pos)
     if layer.get("attention_kernel", "softmax") in attention.LINEAR_KERNELS:
         return _linear_step(layer, q, k_new, v_new, idx, cache)
     lc = cache._kv.get(idx)
     if lc is None:
-        lc = _LayerKV(B, Hkv, D, base=pos, need=S_new, dtype=qkv.dtype)
+        lc = _LayerKV(B, Hkv, D, base=pos, need=S_new, dtype=q.dtype)
         cache._kv[idx] = lc
-    elif lc.k.dtype != qkv.dtype:
+    elif lc.k.dtype != q.dtype:
         raise ValueError(f"the cache of layer {idx} holds {lc.k.dtype} K/V but the precision is "
-                         f"now {qkv.dtype}; start a new KVCache after set_precision")
+                         f"now {q.dtype}; start a new KVCache after set_precision")
     lc.reserve(S_new)
     kernels.kv_append(lc.k, k_new, lc.end)
     kernels.kv_append(lc.v, v_new, lc.end)
@@ -206,18 +196,18 @@ def attention_step(layer: Dict[str, Any], x, idx: int, cache: KVCache, B: int, S
         kv_v = lc.v[:, :, lc.begin:lc.end].permute(0, 2, 1, 3)
         ctx = sparse.attention(q, kv_k, kv_v, sparse.normalize_pattern(spec), causal=True,
                                alibi_slopes=slopes, q_pos0=pos, k_pos0=lc.base + lc.begin,
-                               out_dtype=qkv.dtype)
+                               out_dtype=q.dtype)
     elif S_new == 1:
         ctx = kernels.attention_decode(q[:, 0], lc.k, lc.v, slot_begin=lc.begin,
                                        slot_end=lc.end, pos_slot0=lc.base, q_pos=pos,
                                        window=window, alibi_slopes=slopes,
-                                       out_dtype=qkv.dtype).unsqueeze(1)
+                                       out_dtype=q.dtype).unsqueeze(1)
     else:
         kv_k = lc.k[:, :, lc.begin:lc.end].permute(0, 2, 1, 3)
         kv_v = lc.v[:, :, lc.begin:lc.end].permute(0, 2, 1, 3)
         ctx = kernels.attention_prefill(q, kv_k, kv_v, causal=True, window=window,
                                         alibi_slopes=slopes, q_pos0=pos,
-                                        k_pos0=lc.base + lc.begin, out_dtype=qkv.dtype)
+                                        k_pos0=lc.base + lc.begin, out_dtype=q.dtype)
     return attention.project(ctx.flatten(-2), layer, "o", out_dtype=torch.float32)
 
 

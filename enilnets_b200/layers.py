@@ -20,6 +20,7 @@ from .backend import default_dtype
 
 NORMAL_INIT_STD = 0.1          # core/constants.py:67
 SINUSOIDAL_BASE = 10000.0      # core/constants.py:70
+QK_NORM_EPS = 1e-6
 
 
 # ------------------------------------------------------------------- init
@@ -146,13 +147,16 @@ def add_multihead_attention(self: Any, embed_dim: Optional[int] = None, num_head
                             attention_kernel: str = "softmax",
                             num_features: Optional[int] = None,
                             sparse_pattern: Optional[Dict[str, int]] = None,
-                            tiled_block_size: Optional[int] = None) -> None:
+                            tiled_block_size: Optional[int] = None,
+                            qk_norm: bool = False) -> None:
     """Multi-head self-attention, nn/layers.py:256-354. attention_kernel
     "softmax" runs the fused softmax kernels; "linear" (elu + 1) and
     "performer" (FAVOR+) run the linearized-attention kernels; a
     sparse_pattern (nn/sparse_attention.py) runs the softmax kernel over the
     pattern's key tiles only. tiled_block_size is accepted (the softmax kernel
-    always streams) and validated as the reference does."""
+    always streams) and validated as the reference does. qk_norm (not in the
+    reference) adds an RMS norm over each query and key head before the position
+    rotation, with weights "q_norm" and "k_norm" (head_dim,), ones at the start."""
     if embed_dim is None:
         embed_dim = _require_width(self, "add_multihead_attention")
     if embed_dim % num_heads != 0:
@@ -209,6 +213,10 @@ def add_multihead_attention(self: Any, embed_dim: Optional[int] = None, num_head
     })
     if omega is not None:
         self.layers[-1]["omega"] = omega
+    if qk_norm:
+        dt = default_dtype()
+        self.layers[-1].update(q_norm=np.ones(head_dim, dtype=dt),
+                               k_norm=np.ones(head_dim, dtype=dt), qk_norm_eps=QK_NORM_EPS)
     _set_width(self, embed_dim)
 
 
@@ -335,9 +343,10 @@ def add_transformer_block(self: Any, embed_dim: Optional[int] = None, num_heads:
                           attention_kernel: str = "softmax",
                           num_features: Optional[int] = None,
                           sparse_pattern: Optional[Any] = None,
-                          tiled_block_size: Optional[int] = None) -> None:
+                          tiled_block_size: Optional[int] = None,
+                          qk_norm: bool = False) -> None:
     """Pre-norm block LN -> MHA -> residual -> LN -> MLP -> residual,
-    nn/transformer_layers.py:13-57."""
+    nn/transformer_layers.py:13-57 (qk_norm: see add_multihead_attention)."""
     if embed_dim is None:
         if self._last_width is None:
             raise ValueError(
@@ -349,7 +358,7 @@ def add_transformer_block(self: Any, embed_dim: Optional[int] = None, num_heads:
                             positional_scheme=positional_scheme, num_kv_heads=num_kv_heads,
                             window_size=window_size, attention_kernel=attention_kernel,
                             num_features=num_features, sparse_pattern=sparse_pattern,
-                            tiled_block_size=tiled_block_size)
+                            tiled_block_size=tiled_block_size, qk_norm=qk_norm)
     add_residual_end(self)
     add_residual_start(self)
     add_layernorm(self, (embed_dim,))

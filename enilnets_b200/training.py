@@ -11,6 +11,8 @@ attention core read, its output and LSE) and the backward runs K5
   d_Wo = dout^T context, d_bo = sum dout, dcontext = dout Wo
   dQh, dKh, dVh = K5(Q, K, V, O, LSE, dcontext)     (GQA already summed)
   RoPE layers: dQh, dKh rotated back by -angle     (nn/backward.py:300-308)
+  layers with query/key norms: norm and rotation in one pass each way
+  (enl_qk_norm_rope and its backward, which also gives d_q_norm, d_k_norm)
   d_Wq = dQ^T x_in, d_bq = sum dQ, ... ; dx = dQ Wq + dK Wk + dV Wv.
 
 The projections run in fp32 GEMMs. The attention core follows set_precision
@@ -91,7 +93,13 @@ def self_attention_forward_train(layer: Dict[str, Any], x) -> Tuple[Any, Dict[st
     k = attention.split_heads(qkv, Hkv, D, H * D)
     v = attention.split_heads(qkv, Hkv, D, H * D + Hkv * D)
     scheme = layer.get("positional_scheme", "absolute")
-    if scheme == "rope":
+    norm = None
+    if layer.get("q_norm") is not None:
+        wq, wk, eps = attention.qk_norm_args(layer)
+        tables = attention.rope_tables(S, D) if scheme == "rope" else None
+        norm = {"q": q, "k": k, "wq": wq, "wk": wk, "eps": eps, "rope": tables}
+        q, k = kernels.qk_norm_rope(q, k, wq, wk, eps=eps, rope=tables)
+    elif scheme == "rope":
         attention.apply_rope(q, 0)
         attention.apply_rope(k, 0)
     causal = bool(layer.get("causal", False))
@@ -105,14 +113,16 @@ def self_attention_forward_train(layer: Dict[str, Any], x) -> Tuple[Any, Dict[st
     bo = attention._WEIGHTS.get(layer, ("bo",), "b", torch.float32)
     y = F.linear(ctx, wo, bo)
     cache = {"x": x, "q": q, "k": k, "v": v, "o": o, "lse": lse, "ctx": ctx,
-             "causal": causal, "window": window, "slopes": slopes, "rope": scheme == "rope"}
+             "causal": causal, "window": window, "slopes": slopes, "rope": scheme == "rope",
+             "norm": norm}
     return y, cache
 
 
 def self_attention_backward(layer: Dict[str, Any], cache: Dict[str, Any],
                             dout) -> Tuple[Any, Dict[str, Any]]:
     """(dx, grads) of the layer for dout (B, S, E) on the device: grads holds
-    d_Wq, d_bq, d_Wk, d_bk, d_Wv, d_bv, d_Wo, d_bo as fp32 device tensors."""
+    d_Wq, d_bq, d_Wk, d_bk, d_Wv, d_bv, d_Wo, d_bo (and d_q_norm, d_k_norm of a
+    layer with query/key norms) as fp32 device tensors."""
     import torch
     B, S, E = dout.shape
     H, D = layer["num_heads"], layer["head_dim"]
@@ -126,7 +136,12 @@ def self_attention_backward(layer: Dict[str, Any], cache: Dict[str, Any],
                                             cache["lse"], dctx, causal=cache["causal"],
                                             window=cache["window"],
                                             alibi_slopes=cache["slopes"])
-    if cache["rope"]:
+    norm = cache["norm"]
+    if norm is not None:
+        dq, dk, grads["d_q_norm"], grads["d_k_norm"] = kernels.qk_norm_rope_backward(
+            dq, dk, norm["q"], norm["k"], norm["wq"], norm["wk"], eps=norm["eps"],
+            rope=norm["rope"], out=(dq, dk))
+    elif cache["rope"]:
         _unrotate(dq)
         _unrotate(dk)
     x2 = cache["x"].reshape(-1, E)

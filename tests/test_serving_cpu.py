@@ -183,3 +183,57 @@ def test_oracle_sampling_edges():
     assert ref.sample([1.0, 1.0, 1.0], 0.99, top_k=2) == 1   # ties: lowest indices first
     assert ref.sample([0.0, 1.0, 1.0], 0.9, temperature=0.0) == 1
     assert ref.sample([0.0, 5.0], 0.999999, top_p=0.0) == 1
+
+
+def test_page_bookkeeping():
+    """Pages are handed out as sequences grow and come back when they end or
+    leave the window; a refused request takes none."""
+    from enilnets_b200.serving import PagedKVCache
+    c = PagedKVCache(6, 4, 100)
+    a, b = c.add(), c.add()
+    c.reserve([a, b], [5, 1])
+    c.advance([a, b], [5, 1])
+    assert c.free_pages == 3 and c.length == {a: 5, b: 1}
+    c.reserve([a], [3])
+    assert c.free_pages == 3
+    with pytest.raises(ValueError, match="more pages"):
+        c.reserve([a, b], [12, 9])
+    assert c.free_pages == 3
+    c.release(b)
+    assert c.free_pages == 4
+    with pytest.raises(ValueError, match="not in this cache"):
+        c.release(b)
+    with pytest.raises(ValueError, match="max_seq_len=100"):
+        c.reserve([a], [96])
+    for kw in (dict(num_pages=0), dict(num_pages=1, page_size=0), dict(num_pages=1, sinks=2),
+               dict(num_pages=1, window=-1), dict(num_pages=1, max_seq_len=0)):
+        with pytest.raises(ValueError):
+            PagedKVCache(**kw)
+
+
+def test_windowed_cache_keeps_first_and_last_pages():
+    from enilnets_b200.serving import PagedKVCache
+    c = PagedKVCache(20, 4, 1000, window=9, sinks=5)
+    s = c.add()
+    for n in range(1, 200):
+        c.reserve([s], [1])
+        # every position that the query at n - 1 sees has its page
+        seen = [j for j in range(n) if n - 1 - j <= 9 or j < 5]
+        assert all(c._pages[s][j // 4] >= 0 for j in seen), n
+        c.advance([s], [1])
+    assert 20 - c.free_pages <= 2 + 4
+
+
+def test_qk_norm_builder_keeps_the_default_contract():
+    """qk_norm adds weights without drawing random numbers; without it the layer
+    dict is what it was."""
+    import enilnets_b200 as enl
+    layers = []
+    for kw in (dict(), dict(qk_norm=True)):
+        enl.set_seed(1)
+        net = enl.AttentionNet()
+        net.add_multihead_attention(64, 4, **kw)
+        layers.append(net.layers[0])
+    plain, normed = layers
+    assert "q_norm" not in plain and set(normed) - set(plain) == {"q_norm", "k_norm", "qk_norm_eps"}
+    assert np.array_equal(plain["Wo"], normed["Wo"]) and np.array_equal(normed["q_norm"], np.ones(16))
