@@ -34,7 +34,14 @@
 // are exact; the probabilities are split into two bf16 parts (16 bits of
 // mantissa), which costs a second product and keeps their rounding out of the
 // output. fp32: each factor is split into two tf32 parts (values into three) and
-// the three (four) largest products are added, about 2^-21 of each.
+// the three (four) largest products are added, about 2^-21 of each. The tensor
+// pipe cuts its sums instead of rounding them, always towards zero, so nothing
+// is summed in it for long: a few products at a time start from zero and are
+// added to the running sums by rounded additions (without that, 16000 equal fp32
+// values came out 3e-5 small). Only bf16 with two column tiles has no registers
+// for it (342 us against 298 for 64 sequences of 6144 with 16 query heads a key
+// head): its running sums stay in the pipe, and 16000 equal values come out 2e-6
+// small, far below the rounding of a bf16 output.
 #include <algorithm>
 #include <atomic>
 
@@ -142,6 +149,27 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c = a b, for sums that start here.
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_tf32_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void add4(float (&c)[4], const float (&t)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] += t[i];
 }
 __device__ __forceinline__ float4 lds4(uint32_t addr) {
   float4 f;
@@ -367,48 +395,53 @@ struct Decoder {
 
   // Scores of the warp's 16 keys: rows r and r + 8, heads 2q and 2q + 1.
   __device__ __forceinline__ void scores(uint32_t kbase, float (&s)[C::NT][4]) const {
-    float s2[C::NT][4];
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
     if constexpr (C::kF32) {
       const int row = warp * 16 + r;
 #pragma unroll
       for (int ks = 0; ks < C::D / 16; ++ks) {
         const float4 x = lds4(kbase + place<C>(row, ks * 4 + q));
         const float4 y = lds4(kbase + place<C>(row + 8, ks * 4 + q));
-        uint32_t hi[4], lo[4];
+        uint32_t hi[2][4], lo[2][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          split_tf32(half ? x.z : x.x, hi[0], lo[0]);
-          split_tf32(half ? y.z : y.x, hi[1], lo[1]);
-          split_tf32(half ? x.w : x.y, hi[2], lo[2]);
-          split_tf32(half ? y.w : y.y, hi[3], lo[3]);
+          split_tf32(half ? x.z : x.x, hi[half][0], lo[half][0]);
+          split_tf32(half ? y.z : y.x, hi[half][1], lo[half][1]);
+          split_tf32(half ? x.w : x.y, hi[half][2], lo[half][2]);
+          split_tf32(half ? y.w : y.y, hi[half][3], lo[half][3]);
+        }
 #pragma unroll
-          for (int nt = 0; nt < C::NT; ++nt) {
-            const uint32_t* f = qf[nt][ks] + 2 * half;
-            mma_tf32(s2[nt], lo, f[0], f[1]);
-            mma_tf32(s2[nt], hi, f[4], f[5]);
-            mma_tf32(s[nt], hi, f[0], f[1]);
-          }
+        for (int nt = 0; nt < C::NT; ++nt) {
+          const uint32_t* f = qf[nt][ks];
+          float t[4];  // the small products first
+          mma_tf32_first(t, lo[0], f[0], f[1]);
+          mma_tf32(t, hi[0], f[4], f[5]);
+          mma_tf32(t, lo[1], f[2], f[3]);
+          mma_tf32(t, hi[1], f[6], f[7]);
+          mma_tf32(t, hi[0], f[0], f[1]);
+          mma_tf32(t, hi[1], f[2], f[3]);
+          add4(s[nt], t);
         }
       }
     } else {
       const int row = warp * 16 + (lane & 15);
 #pragma unroll
-      for (int ks = 0; ks < C::D / 16; ++ks) {
-        uint32_t a[4];
+      for (int ks = 0; ks < C::D / 16; ks += 2) {
+        uint32_t a[4], b[4];
         ldmatrix4(a, kbase + place<C>(row, ks * 2 + (lane >> 4)));
+        ldmatrix4(b, kbase + place<C>(row, ks * 2 + 2 + (lane >> 4)));
 #pragma unroll
-        for (int nt = 0; nt < C::NT; ++nt)
-          mma_bf16(ks % 2 ? s2[nt] : s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        for (int nt = 0; nt < C::NT; ++nt) {
+          float t[4];
+          mma_bf16_first(t, a, qf[nt][ks][0], qf[nt][ks][1]);
+          mma_bf16(t, b, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+          add4(s[nt], t);
+        }
       }
     }
-#pragma unroll
-    for (int nt = 0; nt < C::NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] += s2[nt][i];
   }
 
   // O^T += V^T P^T for the warp's 16 keys.
@@ -428,28 +461,37 @@ struct Decoder {
             split_tf32(__uint_as_float(__byte_perm(tl, th, i ? 0x7632 : 0x5410)),
                        ph[nt][2 * half + i], pl[nt][2 * half + i]);
         }
+      const int row = warp * 16 + 2 * q;  // and row + 1; row + 8, row + 9
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = warp * 16 + half * 8 + 2 * q;
+      for (int blk = 0; blk < C::D / 32; ++blk) {
+        float4 x[2], y[2];
 #pragma unroll
-        for (int blk = 0; blk < C::D / 32; ++blk) {
-          const float4 x = lds4(vbase + place<C>(row, blk * 8 + r));
-          const float4 y = lds4(vbase + place<C>(row + 1, blk * 8 + r));
-          uint32_t hi[4], lo[4], rest[4];
+        for (int half = 0; half < 2; ++half) {
+          x[half] = lds4(vbase + place<C>(row + 8 * half, blk * 8 + r));
+          y[half] = lds4(vbase + place<C>(row + 8 * half + 1, blk * 8 + r));
+        }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            split_tf32(u ? x.z : x.x, hi[0], lo[0], rest[0]);
-            split_tf32(u ? x.w : x.y, hi[1], lo[1], rest[1]);
-            split_tf32(u ? y.z : y.x, hi[2], lo[2], rest[2]);
-            split_tf32(u ? y.w : y.y, hi[3], lo[3], rest[3]);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t hi[2][4], lo[2][4], rest[2][4];
 #pragma unroll
-            for (int nt = 0; nt < C::NT; ++nt) {
-              float(&acc)[4] = o[nt][blk * 2 + u];
-              mma_tf32(acc, rest, ph[nt][2 * half], ph[nt][2 * half + 1]);
-              mma_tf32(acc, lo, ph[nt][2 * half], ph[nt][2 * half + 1]);
-              mma_tf32(acc, hi, pl[nt][2 * half], pl[nt][2 * half + 1]);
-              mma_tf32(acc, hi, ph[nt][2 * half], ph[nt][2 * half + 1]);
-            }
+          for (int half = 0; half < 2; ++half) {
+            split_tf32(u ? x[half].z : x[half].x, hi[half][0], lo[half][0], rest[half][0]);
+            split_tf32(u ? x[half].w : x[half].y, hi[half][1], lo[half][1], rest[half][1]);
+            split_tf32(u ? y[half].z : y[half].x, hi[half][2], lo[half][2], rest[half][2]);
+            split_tf32(u ? y[half].w : y[half].y, hi[half][3], lo[half][3], rest[half][3]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < C::NT; ++nt) {
+            float t[4];
+            mma_tf32_first(t, rest[0], ph[nt][0], ph[nt][1]);
+            mma_tf32(t, rest[1], ph[nt][2], ph[nt][3]);
+            mma_tf32(t, lo[0], ph[nt][0], ph[nt][1]);
+            mma_tf32(t, lo[1], ph[nt][2], ph[nt][3]);
+            mma_tf32(t, hi[0], pl[nt][0], pl[nt][1]);
+            mma_tf32(t, hi[1], pl[nt][2], pl[nt][3]);
+            mma_tf32(t, hi[0], ph[nt][0], ph[nt][1]);
+            mma_tf32(t, hi[1], ph[nt][2], ph[nt][3]);
+            add4(o[nt][blk * 2 + u], t);
           }
         }
       }
@@ -471,8 +513,15 @@ struct Decoder {
         ldmatrix4_trans(a, vbase + place<C>(row, mt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
-          mma_bf16(o[nt][mt], a, bl[nt][0], bl[nt][1]);
-          mma_bf16(o[nt][mt], a, bh[nt][0], bh[nt][1]);
+          if constexpr (C::NT > 1) {
+            mma_bf16(o[nt][mt], a, bl[nt][0], bl[nt][1]);
+            mma_bf16(o[nt][mt], a, bh[nt][0], bh[nt][1]);
+          } else {
+            float t[4];
+            mma_bf16_first(t, a, bl[nt][0], bl[nt][1]);
+            mma_bf16(t, a, bh[nt][0], bh[nt][1]);
+            add4(o[nt][mt], t);
+          }
         }
       }
     }

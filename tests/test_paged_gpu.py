@@ -118,6 +118,24 @@ def test_long_uneven_batch(cuda, dtype):
     _check(*case, out, lse)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_sums_are_not_cut(cuda, dtype, D):
+    """Equal values of one sign over a long sequence: the output is that value.
+    Sums that were cut towards zero instead of rounded would fall short by the
+    number of additions times 2^-24; rounded ones stay within sqrt of it, checked
+    at 1e-6 (bf16 inputs included: the output is fp32)."""
+    import torch
+    from enilnets_b200 import kernels
+    q, kp, vp, table, lens = _case(40, [16000], 64, 64, D, 16, dtype)  # long runs per block
+    kp = torch.where(torch.isnan(kp), kp, 0.01 * kp)
+    value = 1.0 + torch.rand((D,), device="cuda").to(vp.dtype)
+    vp = torch.where(torch.isnan(vp), vp, value)
+    out = kernels.attention_decode_paged(q, kp, vp, table, lens, out_dtype=torch.float32)
+    want = value.double()
+    assert ((out[0].double() - want).abs() / want).max() <= 1e-6
+
+
 def test_many_sequences(cuda):
     """More (sequence, head) pairs than blocks: several whole ones each."""
     lens = list(np.random.RandomState(0).randint(0, 90, 300))
