@@ -55,10 +55,16 @@ constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
 constexpr int kTries = 16;       // passes with guessed bins (the last halve what is left)
 // One vector in kSample goes into the histogram, kWindow tokens are listed to
-// each side of a guessed cut. Measured (256 flat rows of 131072, top-p 0.9, us):
-// 4 and 650: 185, 8 and 800: 255 (more wrong guesses), 4 and 300: 198.
+// each side of a guessed cut: wider samples and windows cost more than the wrong
+// guesses that they save (256 flat rows of 131072, top-p 0.9: 161 us; with 8 and
+// 800 a third more, with 4 and 300 a fifteenth).
 constexpr int kSample = 4;
 constexpr int kWindow = 650;
+// Tokens above e^-kHeavy are weighed one by one in the histogram, lighter ones by
+// their bin's centre: the second atomic costs more than it tells (one flat row's
+// histogram: 4: 16 us, 7: 22 us, 7 with float atomics: 30 us). In
+// whole units of 2^-13; rows so long that they overflow only guess worse.
+constexpr float kHeavy = 4.0f;
 constexpr float kOne = 1099511627776.0f;  // 2^40
 constexpr uint32_t kNoCut = ~0u;  // in place of a top-p share
 constexpr float kLive = 28.0f;   // weights below exp(-28) < 2^-40 are zero
@@ -100,6 +106,14 @@ struct WholeSum {
     hi += __float_as_uint(a);
     lo += __float_as_uint(b);
     ++n;
+  }
+  __device__ __forceinline__ static WholeSum of(float w) {
+    WholeSum s;
+    s.add(w);
+    return s;
+  }
+  __device__ __forceinline__ void operator+=(const WholeSum& s) {
+    hi += s.hi, lo += s.lo, n += s.n;
   }
   __device__ __forceinline__ u64 total() const {
     const uint32_t off = (uint32_t)n * 0x4B000000u;
@@ -227,8 +241,8 @@ struct Shared {
   union {
     u64 list[kCap];  // candidates (composites)
     struct {
-      uint32_t bins[kBins];  // histogram: tokens, and the weight of
-      float heavy[kBins];    // those above 2^-10 of the largest
+      uint32_t bins[kBins];   // histogram: tokens, and the
+      uint32_t heavy[kBins];  // weight of those that are weighed one by one, in 2^-13
     };
   };
   float cum_n[kBins], cum_m[kBins];  // guessed tokens and weight before each bin
@@ -491,11 +505,11 @@ struct Sampler {
   // Adds the tokens of vector j whose bits are set to the block's list, which
   // may overflow (its count says so).
   __device__ __forceinline__ void push(const Vec<kF32>& x, int j, uint32_t bits) const {
-    while (bits) {
+    if (!bits) return;
+    int at = atomicAdd(&sm.count, __popc(bits));
+    for (; bits && at < kCap; bits &= bits - 1, ++at) {
       const int e = __ffs(bits) - 1;
-      bits &= bits - 1;
-      const int at = atomicAdd(&sm.count, 1);
-      if (at < kCap) sm.list[at] = composite(x.pick(e), j * E - row.mis + e);
+      sm.list[at] = composite(x.pick(e), j * E - row.mis + e);
     }
   }
   // Empties the lists, before a pass that fills them.
@@ -805,7 +819,7 @@ struct Sampler {
     b.scale = range > 0.0f ? (float)kBins / range : 0.0f;
     b.width = range / kBins;
     b.light = 0;
-    b.light = b.of(top - 7.0f / inv_t);
+    b.light = b.of(top - kHeavy / inv_t);
     return b;
   }
   __device__ __forceinline__ void count_in(const Bins& bins, float x, bool weigh, int n) const {
@@ -813,10 +827,11 @@ struct Sampler {
     const int b = bins.of(x);
     atomicAdd(&sm.bins[b], (uint32_t)n);
     if (b < bins.light && weigh)
-      atomicAdd(&sm.heavy[b], (float)n * (x == top ? 1.0f : __expf((x - top) * inv_t)));
+      atomicAdd(&sm.heavy[b],
+                (uint32_t)((float)(n << 13) * (x == top ? 1.0f : __expf((x - top) * inv_t)) + 0.5f));
   }
   __device__ void clear_bins() const {
-    for (int t = threadIdx.x; t < kBins; t += kThreads) sm.bins[t] = 0, sm.heavy[t] = 0.0f;
+    for (int t = threadIdx.x; t < kBins; t += kThreads) sm.bins[t] = sm.heavy[t] = 0;
     __syncthreads();
   }
   // One pass that divides the row by value: this thread's sum of the whole
@@ -830,24 +845,24 @@ struct Sampler {
     for (int j0 = first_vec(); j0 < end; j0 += 32 * 128) {
       WholeSum w, a;
       each_vec(j0, min(end, j0 + 32 * 128), 32, [&](const Vec<kF32>& x, int j) {
-        uint32_t n = 0, inside = 0;
+        uint32_t above = 0, inside = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float v = x.at(e);
-          n += v > hi;
-          inside |= v >= lo && !(v > hi) ? 1u << e : 0u;
+          above |= x.at(e) > hi ? 1u << e : 0u;
+          inside |= x.at(e) >= lo ? 1u << e : 0u;
         }
-        push(x, j, inside);
-        s.count += n;
-        if (all || (n && weigh)) {
+        push(x, j, inside & ~above);
+        if (all || (above && weigh)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const float v = x.at(e);
-            const float f = v > -INFINITY ? weight(v) : 0.0f;
-            w.add(v > hi ? f : 0.0f);
-            a.add(f);
+            const float v = x.at(e);  // NaN and -inf take the bound, whose weight is zero
+            const float t = v == top ? 0.0f : fmaxf((v - top) * inv_t, -100.0f);
+            const WholeSum one = WholeSum::of(expf(t));
+            a += one;
+            if (above >> e & 1) w += one;
           }
         }
+        s.count += __popc(above);
       });
       s.above += w.total();
       s.all += a.total();
@@ -913,20 +928,19 @@ struct Sampler {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int b = first_bin + e;
-      float heavy = 0.0f;
-      uint32_t n = 0;
+      uint32_t n = 0, heavy = 0;
       if (e < n_bins) {
         if (n_blocks == 1) {
           n = sm.bins[b], heavy = sm.heavy[b];
         } else {
           for (int r = 0; r < n_blocks; ++r) {
             n += remote_load(remote(&sm.bins[b], r));
-            heavy += __uint_as_float(remote_load(remote(&sm.heavy[b], r)));
+            heavy += remote_load(remote(&sm.heavy[b], r));
           }
         }
       }
       c[e] = (float)n;
-      m[e] = b < bins.light ? heavy
+      m[e] = b < bins.light ? (float)heavy * (1.0f / 8192.0f)
                             : c[e] * __expf(-((float)b + 0.5f) * bins.width * inv_t);
       c_mine += c[e];
       m_mine += m[e];
@@ -1417,7 +1431,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 }
 
 // Blocks per row: as many as keep two a SM, a power of two up to 8, with at least
-// one vector for each thread.
+// one vector for each thread. (256 rows of 131072, two blocks a row: top-k and
+// top-p 42 us against 21, top-p alone the same; 64 rows of 100003, four blocks
+// against two: 90 us against 79.)
 int choose_cluster(int B, int V, bool fp32, int n_sms) {
   const int per_block = kThreads * (fp32 ? 4 : 8);
   int c = 1;
