@@ -10,10 +10,14 @@
 // for each query head of its group. So every key is loaded once for all the
 // query heads that share it, and the products run on mma.sync with the keys as
 // the rows and the heads as the columns (S^T = K Q^T, O^T = V^T P^T; eight heads
-// are one column tile, so a group of one wastes products but no bytes). At the
-// HBM rate an SM gets 16 bf16 keys of 128 every 350 cycles and spends about 30
-// issue slots of each scheduler on them; tcgen05's 128-row tiles would need the
-// probabilities in shared or tensor memory for no gain.
+// are one column tile, so a group of one wastes products but no bytes). fp32
+// products on that pipe take three or four tf32 ones and the splits of every
+// element, so up to four fp32 heads a group are computed on the FMA pipe instead,
+// two products an instruction, each element used as it is loaded (16 x 6144 keys
+// of 128: 130 us against 177). At the HBM rate an SM gets 16 bf16 keys of 128
+// every 350 cycles and spends about 30 issue slots of each scheduler on them;
+// tcgen05's 128-row tiles would need the probabilities in shared or tensor memory
+// for no gain.
 //
 // Work: a sequence's visible positions are cut into tiles of 16 keys a warp;
 // tiles are numbered sequence by sequence, head group by head group, and every
@@ -33,9 +37,10 @@
 // Precision: scores, softmax and sums in fp32. bf16: products of bf16 inputs
 // are exact; the probabilities are split into two bf16 parts (16 bits of
 // mantissa), which costs a second product and keeps their rounding out of the
-// output. fp32: each factor is split into two tf32 parts (values into three) and
-// the three (four) largest products are added, about 2^-21 of each. The tensor
-// pipe cuts its sums instead of rounding them, always towards zero, so nothing
+// output. fp32 on the FMA pipe: a tile's sum by itself, then added to the running
+// one, so that equal values do not add up equal roundings. fp32 on the tensor
+// pipe: each factor is split into two tf32 parts (values into three) and the
+// three (four) largest products are added, about 2^-21 of each. The tensor pipe cuts its sums instead of rounding them, always towards zero, so nothing
 // is summed in it for long: a few products at a time start from zero and are
 // added to the running sums by rounded additions (without that, 16000 equal fp32
 // values came out 3e-5 small). Only bf16 with two column tiles has no registers
@@ -44,6 +49,7 @@
 // small, far below the rounding of a bf16 output.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "enl_common.cuh"
 #include "enl_kernels.h"
@@ -75,11 +81,14 @@ constexpr int kLens = 256;  // sequence lengths kept in shared memory
 constexpr int kWholeTiles = 6;
 
 // Kernel shapes: D is the padded head dim, NT column tiles of 8 heads per item,
-// NW computing warps, S stages.
-template <int D_, bool kF32_, int NT_, int NW_, int S_>
+// NW computing warps, S stages. kFma: not on the tensor pipe, with that many
+// heads per item (fp32).
+template <int D_, bool kF32_, int NT_, int NW_, int S_, int kFma_ = 0>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, NW = NW_, S = S_;
   static constexpr bool kF32 = kF32_;
+  static constexpr int kFma = kFma_;
+  static constexpr int kItem = kFma ? kFma : NT * 8;  // heads of an item
   static constexpr int kKeys = NW * 16;  // keys of a tile
   static constexpr int NP = kKeys / 32;  // loading warps, a key a lane
   static constexpr int kThreads = (NW + NP) * 32;
@@ -87,12 +96,12 @@ struct Cfg {
   static constexpr int kRow = D * kEsz;  // bytes of a row in shared memory
   static constexpr int kTile = kKeys * kRow;
   static constexpr int kStage = 2 * kTile;  // K, then V
-  static constexpr int kMerge = (NW - 1) * 8 * D * 4;
+  static constexpr int kMerge = (kFma ? (2 * NW - 1) * kFma : (NW - 1) * 8) * D * 4;
   static constexpr int kSmem = S * kStage + kMerge;
   static constexpr int kStatic = kLens * 4 + S * 64 + 768;           // at most
   static constexpr int kFit = 228 * 1024 / (kSmem + kStatic + 1024);
   static constexpr int kPerSm = NT > 1 && kFit > 2 ? 2 : kFit;  // blocks a SM (registers)
-  static constexpr int kSlot = NT * 8 * D + NT * 16;                 // floats of one part
+  static constexpr int kSlot = kFma ? kFma * (D + 4) : NT * 8 * D + NT * 16;  // floats of a part
   static constexpr int kRegs = D / 16 * 4;  // accumulators of a column tile
 };
 
@@ -180,6 +189,10 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
   return f;
 }
 
+__device__ __forceinline__ void lds2x2(uint32_t addr, uint64_t& a, uint64_t& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
+}
+
 // x = hi + lo with hi the upper 11 bits (tf32); lo's own tail past 11 bits is
 // dropped by the product. Cutting takes one logic instruction where rounding
 // takes a conversion at a quarter of the rate.
@@ -227,15 +240,48 @@ struct Block {  // shared by a block's warps
   float m[4][16], l[4][16];
 };
 
+// What a block's warps know.
 template <class C>
-struct Decoder {
+struct Base {
   const PagedDecodeParams& p;
   Block& sh;
   uint8_t* smem;
   uint32_t sbase;
   int G, HB, SUB;  // heads a group, head blocks a group, head blocks in all
-  int lane, warp, r, q;
-  int lens_b;
+  int lane, warp;
+
+  __device__ Base(const PagedDecodeParams& p_, Block& sh_, uint8_t* smem_)
+      : p(p_), sh(sh_), smem(smem_), sbase(smem_u32(smem_)) {
+    G = p.H / p.Hkv;
+    HB = (G + C::kItem - 1) / C::kItem;
+    SUB = p.Hkv * HB;
+    lane = threadIdx.x % 32;
+    warp = threadIdx.x / 32;
+  }
+
+  __device__ __forceinline__ void sync_warps() const { named_bar_sync(1, C::NW * 32); }
+
+  __device__ int heads_of(const Note& w) const {  // real heads of the item
+    return min(C::kItem, G - (w.sub % HB) * (C::kItem));
+  }
+  __device__ int first_head(const Note& w) const {
+    return (w.sub / HB) * G + (w.sub % HB) * (C::kItem);
+  }
+};
+
+// The computing warps on the tensor pipe.
+template <class C>
+struct MmaMath : Base<C> {
+  using Base<C>::p;
+  using Base<C>::sh;
+  using Base<C>::smem;
+  using Base<C>::sbase;
+  using Base<C>::lane;
+  using Base<C>::warp;
+  using Base<C>::sync_warps;
+  using Base<C>::heads_of;
+  using Base<C>::first_head;
+  const int r = lane / 4, q = lane % 4;
 
   // Softmax state of the warp: heads 8 nt + 2q (+1) of the item, this lane's
   // share of the sums; O^T fragments (rows: dims, columns: heads).
@@ -243,128 +289,25 @@ struct Decoder {
   // Q^T fragments.
   uint32_t qf[C::NT][C::D / 16][C::kF32 ? 8 : 2];
 
-  __device__ int read_length(int b) const {
-    int L = p.lens[b];
-    const long long most = (long long)p.max_pages * p.page_size;
-    if (L > most) L = (int)most;
-    return max(L, 0);
-  }
-  __device__ int length(int b) const {
-    const int at = b - lens_b;
-    return at >= 0 && at < kLens ? sh.lens[at] : read_length(b);
-  }
-  __device__ __forceinline__ int tiles_of(int n) const { return (n + C::kKeys - 1) / C::kKeys; }
+  using Base<C>::Base;
 
-  // ------------------------------------------------------- loading warps
-  __device__ void enter(Walker& w, int b) const {
-    w.b = b;
-    w.L = length(b);
-    w.vis = visible_of(w.L, p.window, p.sinks);
-    w.nt = tiles_of(w.vis.n);
-  }
-  __device__ void advance(Walker& w) const {
-    if (++w.t < w.nt) return;
-    w.t = 0;
-    if (++w.sub < SUB) return;
-    w.sub = 0;
-    int b = w.b + 1;
-    while (b < p.B && length(b) == 0) ++b;
-    if (b < p.B) enter(w, b);
-  }
-
-  // A key's row in the pools: the page number as read (whose latency passes
-  // while the tile before is loaded), then the address.
-  struct Key {
-    int page, slot;  // slot < 0: past the end
-  };
-  __device__ __forceinline__ Key find_key(const Walker& w, int key) const {
-    Key k{0, -1};
-    const int i = w.t * C::kKeys + key;
-    if (i < w.vis.n) {
-      const int j = i < w.vis.n_sink ? i : i + w.vis.gap;
-      const int col = j / p.page_size;
-      k.slot = j - col * p.page_size;
-      k.page = p.table[w.b * p.t_sb + col];
-    }
-    return k;
-  }
-
-  __device__ void load_run(const Walker& start, int n) {
-    constexpr int kChunks = C::kRow / 16, kRows = 32 / kChunks;  // rows a pass
-    const int pw = warp - C::NW;
-    const int chunk = lane % kChunks, sub_row = lane / kChunks;
-    const bool real = chunk * 16 < p.D * C::kEsz;
-    const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k) + chunk * 16;
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + chunk * 16;
-    Walker w = start;
-    Key next = find_key(w, pw * 32 + lane);
-    for (int i = 0; i < n; ++i) {
-      const Walker now = w;
-      const Key key = next;
-      if (i + 1 < n) {
-        advance(w);
-        next = find_key(w, pw * 32 + lane);
-      }
-      const int stage = i % C::S;
-      if (i >= C::S) mbar_wait(&sh.empty[stage], (i / C::S - 1) & 1, &sh.abort, kSite);
-      // Byte offset of this lane's key, or -1 for none or a page outside the
-      // pool (which counts as masked).
-      long long off = -1;
-      if (key.slot >= 0) {
-        if (key.page < 0 || key.page >= p.n_pages)
-          report_error(kDevBadIndex, now.b);
-        else
-          off = (key.page * p.p_sp + (now.sub / HB) * p.p_sh + key.slot * p.p_ss) * C::kEsz;
-      }
-      const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
-      const int n_keys = min(C::kKeys, now.vis.n - now.t * C::kKeys);
-      const uint32_t dst = sbase + stage * C::kStage;
-      // Rows of warps without keys stay as they are: those skip the tile.
-      const int passes = min(32, (n_keys + 15) / 16 * 16 - pw * 32) / kRows;
-#pragma unroll 4
-      for (int s = 0; s < passes; ++s) {
-        const int row = s * kRows + sub_row;
-        const long long o = __shfl_sync(0xffffffffu, off, row);
-        const int bytes = real && o >= 0 ? 16 : 0;
-        const long long e = bytes ? o : -chunk * 16;
-        const uint32_t at = dst + place<C>(pw * 32 + row, chunk);
-        cp_async16(at, kb + e, bytes);
-        cp_async16(at + C::kTile, vb + e, bytes);
-      }
-      cp_arrive(&sh.full[stage]);
-      if (lane == 0) {
-        Note& note = sh.note[stage];
-        note.ok[pw] = ok;
-        if (pw == 0) {
-          note.b = now.b, note.sub = now.sub, note.t = now.t, note.nt = now.nt;
-          note.L = now.L, note.n_sink = now.vis.n_sink, note.gap = now.vis.gap;
-          note.n_keys = n_keys;
-        }
-        mbar_arrive(&sh.full[stage]);
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  }
-
-  // ----------------------------------------------------- computing warps
-  __device__ __forceinline__ void sync_warps() const { named_bar_sync(1, C::NW * 32); }
-
-  __device__ int heads_of(const Note& w) const {  // real heads of the item
-    return min(C::NT * 8, G - (w.sub % HB) * (C::NT * 8));
-  }
-  __device__ int first_head(const Note& w) const {
-    return (w.sub / HB) * G + (w.sub % HB) * (C::NT * 8);
-  }
-
-  __device__ void begin_item(const Note& w) {
-    const int n = heads_of(w);
-    const long long q0 = w.b * p.q_sb + first_head(w) * p.q_sh;
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < C::kRegs; ++i) o[nt][i / 4][i % 4] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void fold() {}
+
+  __device__ void begin_item(const Note& w) {
+    const int n = heads_of(w);
+    const long long q0 = w.b * p.q_sb + first_head(w) * p.q_sh;
+    clear();
+#pragma unroll
+    for (int nt = 0; nt < C::NT; ++nt) {
       const int h = nt * 8 + r;  // this lane's column
       const long long e = q0 + h * p.q_sh;
 #pragma unroll
@@ -686,9 +629,6 @@ struct Decoder {
       }
   }
 
-  __device__ __forceinline__ float* slot_of(long long cta, int which) const {
-    return reinterpret_cast<float*>(p.workspace) + (cta * 2 + which) * C::kSlot;
-  }
   __device__ void write_part(float* part) const {  // warp 0
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt) {
@@ -732,7 +672,378 @@ struct Decoder {
         o[nt][i / 4][i % 4] = fmaf(po[nt][i], f[i % 2], o[nt][i / 4][i % 4]);
     }
   }
+};
 
+// The computing warps on the FMA pipe: two lanes share a key's dims for its
+// score, then each lane adds up four dims over its keys (with 64 dims, half a
+// warp each for the even and the odd keys).
+template <class C>
+struct FmaMath : Base<C> {
+  using Base<C>::p;
+  using Base<C>::sh;
+  using Base<C>::smem;
+  using Base<C>::sbase;
+  using Base<C>::lane;
+  using Base<C>::warp;
+  using Base<C>::sync_warps;
+  using Base<C>::heads_of;
+  using Base<C>::first_head;
+  static constexpr int N = C::kFma;
+  static constexpr int kAlike = 128 / C::D;  // keys at a time
+  const int chunk = lane % (C::D / 4), odd = lane / (C::D / 4);
+
+  float m[N], l[N];     // l: this lane's share
+  uint64_t o[N][2];     // dims 4 chunk + {0, 1}, {2, 3}
+  using Base<C>::Base;
+
+  __device__ __forceinline__ float* merge_buffer() const {
+    return reinterpret_cast<float*>(smem + C::S * C::kStage);
+  }
+  // This warp's queries.
+  __device__ __forceinline__ float* queries() const {
+    return merge_buffer() + (C::NW - 1 + warp) * N * C::D;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int g = 0; g < N; ++g) m[g] = -INFINITY, l[g] = 0.0f, o[g][0] = o[g][1] = 0;
+  }
+  __device__ void begin_item(const Note& w) {
+    clear();
+    const int n = heads_of(w);
+    const float* src = reinterpret_cast<const float*>(p.q) + w.b * p.q_sb + first_head(w) * p.q_sh;
+    for (int i = lane; i < N * (C::D / 4); i += 32) {
+      const int g = i / (C::D / 4), d = i % (C::D / 4) * 4;
+      float4 x = make_float4(0, 0, 0, 0);
+      if (g < n && d < p.D) x = *reinterpret_cast<const float4*>(src + g * p.q_sh + d);
+      *reinterpret_cast<float4*>(queries() + g * C::D + d) = x;
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void raise(const float (&mx)[N]) {
+#pragma unroll
+    for (int g = 0; g < N; ++g)
+      if (mx[g] > m[g]) {  // alike in all lanes
+        const float f = fast_exp2(m[g] - mx[g]);
+        const uint64_t ff = f2_pack(f, f);
+        m[g] = mx[g];
+        l[g] *= f;
+        o[g][0] = f2_mul(o[g][0], ff), o[g][1] = f2_mul(o[g][1], ff);
+      }
+  }
+
+  __device__ __forceinline__ void tile(const Note& w, int stage) {
+    const uint32_t kbase = sbase + stage * C::kStage, vbase = kbase + C::kTile;
+    const int key = warp * 16 + lane / 2;
+    const uint32_t qbase = smem_u32(queries());
+    uint64_t acc[N][2];
+#pragma unroll
+    for (int g = 0; g < N; ++g) acc[g][0] = acc[g][1] = 0;
+#pragma unroll
+    for (int i = 0; i < C::D / 8; ++i) {
+      const int c = 2 * i + lane % 2;  // (other halves would share banks)
+      uint64_t k0, k1;
+      lds2x2(kbase + place<C>(key, c), k0, k1);
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+        uint64_t q0, q1;
+        lds2x2(qbase + (g * C::D + c * 4) * 4, q0, q1);
+        acc[g][0] = f2_fma(k0, q0, acc[g][0]);
+        acc[g][1] = f2_fma(k1, q1, acc[g][1]);
+      }
+    }
+    const bool ok = w.ok[C::NP > 1 ? warp / 2 : 0] >> (key & 31) & 1;
+    const int n = heads_of(w), h0 = first_head(w);
+    float s[N], mx[N];
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      float a, b;
+      f2_unpack(f2_add(acc[g][0], acc[g][1]), a, b);
+      s[g] = a + b;
+      s[g] += __shfl_xor_sync(0xffffffffu, s[g], 1);
+      s[g] *= p.scale * kLog2e;
+      if (p.alibi && g < n) {
+        const int idx = w.t * C::kKeys + key;
+        const int j = idx < w.n_sink ? idx : idx + w.gap;
+        s[g] -= p.alibi[h0 + g] * kLog2e * (float)(w.L - 1 - j);
+      }
+      if (!ok) s[g] = -INFINITY;
+      mx[g] = s[g];
+#pragma unroll
+      for (int off = 2; off < 32; off <<= 1)
+        mx[g] = fmaxf(mx[g], __shfl_xor_sync(0xffffffffu, mx[g], off));
+    }
+    raise(mx);
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      s[g] = fast_exp2(s[g] - (m[g] > -INFINITY ? m[g] : 0.0f));  // no visible key yet
+      if (lane % 2 == 0) l[g] += s[g];
+      acc[g][0] = acc[g][1] = 0;
+    }
+    // A tile's sum by itself, then one addition to the running one.
+#pragma unroll
+    for (int i = 0; i < 16 / kAlike; ++i) {
+      const int at = i * kAlike + odd;
+      uint64_t v0, v1;
+      lds2x2(vbase + place<C>(warp * 16 + at, chunk), v0, v1);
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+        const float x = __shfl_sync(0xffffffffu, s[g], at * 2);
+        const uint64_t xx = f2_pack(x, x);
+        acc[g][0] = f2_fma(v0, xx, acc[g][0]);
+        acc[g][1] = f2_fma(v1, xx, acc[g][1]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < N; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) o[g][i] = f2_add(o[g][i], acc[g][i]);
+  }
+
+  // Even and odd keys together, in both.
+  __device__ __forceinline__ void fold() {
+    if constexpr (kAlike > 1) {
+#pragma unroll
+      for (int g = 0; g < N; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          o[g][i] = f2_add(o[g][i], __shfl_xor_sync(0xffffffffu, o[g][i], 16));
+    }
+  }
+
+  // As MmaMath's.
+  __device__ void join_warps(int n) {
+    float* buf = merge_buffer();
+    if (warp < n) {
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], off);
+        if (lane == 0) sh.m[warp][g] = m[g], sh.l[warp][g] = l[g];
+      }
+    }
+    if (n == 1) return;
+    sync_warps();
+    if (warp < n) {
+      float top[N];
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+        top[g] = m[g];
+        for (int w = 0; w < n; ++w) top[g] = fmaxf(top[g], sh.m[w][g]);
+      }
+      raise(top);
+      if (warp == 0) {
+#pragma unroll
+        for (int g = 0; g < N; ++g)
+          for (int w = 1; w < n; ++w)
+            if (sh.m[w][g] > -INFINITY) l[g] += sh.l[w][g] * fast_exp2(sh.m[w][g] - m[g]);
+      } else if (odd == 0) {
+#pragma unroll
+        for (int g = 0; g < N; ++g)
+          *reinterpret_cast<ulonglong2*>(buf + ((warp - 1) * N + g) * C::D + chunk * 4) =
+              make_ulonglong2(o[g][0], o[g][1]);
+      }
+    }
+    sync_warps();
+    if (warp == 0) {
+      for (int w = 0; w < n - 1; ++w)
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          const ulonglong2 x =
+              *reinterpret_cast<const ulonglong2*>(buf + (w * N + g) * C::D + chunk * 4);
+          o[g][0] = f2_add(o[g][0], x.x), o[g][1] = f2_add(o[g][1], x.y);
+        }
+    }
+  }
+
+  __device__ void write_output(const Note& w) const {  // warp 0
+    const int n = heads_of(w);
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      if (g >= n) break;
+      const int head = first_head(w) + g;
+      const float inv = l[g] > 0.0f ? 1.0f / l[g] : l[g] == 0.0f ? 0.0f : l[g];
+      const long long e = w.b * p.o_sb + head * p.o_sh + chunk * 4;
+      if (odd == 0 && chunk * 4 < p.D) {
+        float x[4];
+        f2_unpack(o[g][0], x[0], x[1]);
+        f2_unpack(o[g][1], x[2], x[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (p.out_fp32)
+            reinterpret_cast<float*>(p.o)[e + i] = x[i] * inv;
+          else
+            reinterpret_cast<__nv_bfloat16*>(p.o)[e + i] = __float2bfloat16_rn(x[i] * inv);
+        }
+      }
+      if (lane == 0 && p.lse)
+        p.lse[(long long)w.b * p.H + head] =
+            l[g] == 0.0f ? -INFINITY : (m[g] + log2f(l[g])) * kLn2;
+    }
+  }
+
+  __device__ void write_part(float* part) const {  // warp 0
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      if (odd == 0)
+        *reinterpret_cast<ulonglong2*>(part + g * C::D + chunk * 4) =
+            make_ulonglong2(o[g][0], o[g][1]);
+      if (lane == 0) part[N * C::D + 2 * g] = m[g], part[N * C::D + 2 * g + 1] = l[g];
+    }
+  }
+  // Adds a part to the state (its sums count in lane 0 only).
+  __device__ void add_part(const float* part) {
+    float pm[N], pl[N];
+    ulonglong2 po[N];
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      pm[g] = __ldcg(part + N * C::D + 2 * g);
+      pl[g] = __ldcg(part + N * C::D + 2 * g + 1);
+      po[g] = __ldcg(reinterpret_cast<const ulonglong2*>(part + g * C::D + chunk * 4));
+    }
+    raise(pm);
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      const float f = pm[g] > -INFINITY ? fast_exp2(pm[g] - m[g]) : 0.0f;
+      const uint64_t ff = f2_pack(f, f);
+      if (lane == 0) l[g] += pl[g] * f;
+      o[g][0] = f2_fma(po[g].x, ff, o[g][0]);
+      o[g][1] = f2_fma(po[g].y, ff, o[g][1]);
+    }
+  }
+};
+
+template <class C>
+struct Decoder : std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>> {
+  using Math = std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>>;
+  using Base<C>::p;
+  using Base<C>::sh;
+  using Base<C>::smem;
+  using Base<C>::sbase;
+  using Base<C>::lane;
+  using Base<C>::warp;
+  using Base<C>::sync_warps;
+  using Base<C>::heads_of;
+  using Base<C>::first_head;
+  using Base<C>::HB;
+  using Base<C>::SUB;
+  using Math::begin_item;
+  using Math::tile;
+  using Math::clear;
+  using Math::fold;
+  using Math::join_warps;
+  using Math::write_output;
+  using Math::write_part;
+  using Math::add_part;
+  using Math::Math;
+  int lens_b = 0;
+
+  __device__ int read_length(int b) const {
+    int L = p.lens[b];
+    const long long most = (long long)p.max_pages * p.page_size;
+    if (L > most) L = (int)most;
+    return max(L, 0);
+  }
+  __device__ int length(int b) const {
+    const int at = b - lens_b;
+    return at >= 0 && at < kLens ? sh.lens[at] : read_length(b);
+  }
+  __device__ __forceinline__ int tiles_of(int n) const { return (n + C::kKeys - 1) / C::kKeys; }
+
+  // ------------------------------------------------------- loading warps
+  __device__ void enter(Walker& w, int b) const {
+    w.b = b;
+    w.L = length(b);
+    w.vis = visible_of(w.L, p.window, p.sinks);
+    w.nt = tiles_of(w.vis.n);
+  }
+  __device__ void advance(Walker& w) const {
+    if (++w.t < w.nt) return;
+    w.t = 0;
+    if (++w.sub < SUB) return;
+    w.sub = 0;
+    int b = w.b + 1;
+    while (b < p.B && length(b) == 0) ++b;
+    if (b < p.B) enter(w, b);
+  }
+
+  // A key's row in the pools: the page number as read (whose latency passes
+  // while the tile before is loaded), then the address.
+  struct Key {
+    int page, slot;  // slot < 0: past the end
+  };
+  __device__ __forceinline__ Key find_key(const Walker& w, int key) const {
+    Key k{0, -1};
+    const int i = w.t * C::kKeys + key;
+    if (i < w.vis.n) {
+      const int j = i < w.vis.n_sink ? i : i + w.vis.gap;
+      const int col = j / p.page_size;
+      k.slot = j - col * p.page_size;
+      k.page = p.table[w.b * p.t_sb + col];
+    }
+    return k;
+  }
+
+  __device__ void load_run(const Walker& start, int n) {
+    constexpr int kChunks = C::kRow / 16, kRows = 32 / kChunks;  // rows a pass
+    const int pw = warp - C::NW;
+    const int chunk = lane % kChunks, sub_row = lane / kChunks;
+    const bool real = chunk * 16 < p.D * C::kEsz;
+    const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k) + chunk * 16;
+    const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + chunk * 16;
+    Walker w = start;
+    Key next = find_key(w, pw * 32 + lane);
+    for (int i = 0; i < n; ++i) {
+      const Walker now = w;
+      const Key key = next;
+      if (i + 1 < n) {
+        advance(w);
+        next = find_key(w, pw * 32 + lane);
+      }
+      const int stage = i % C::S;
+      if (i >= C::S) mbar_wait(&sh.empty[stage], (i / C::S - 1) & 1, &sh.abort, kSite);
+      // Byte offset of this lane's key, or -1 for none or a page outside the
+      // pool (which counts as masked).
+      long long off = -1;
+      if (key.slot >= 0) {
+        if (key.page < 0 || key.page >= p.n_pages)
+          report_error(kDevBadIndex, now.b);
+        else
+          off = (key.page * p.p_sp + (now.sub / HB) * p.p_sh + key.slot * p.p_ss) * C::kEsz;
+      }
+      const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+      const int n_keys = min(C::kKeys, now.vis.n - now.t * C::kKeys);
+      const uint32_t dst = sbase + stage * C::kStage;
+      // Rows of warps without keys stay as they are: those skip the tile.
+      const int passes = min(32, (n_keys + 15) / 16 * 16 - pw * 32) / kRows;
+#pragma unroll 4
+      for (int s = 0; s < passes; ++s) {
+        const int row = s * kRows + sub_row;
+        const long long o = __shfl_sync(0xffffffffu, off, row);
+        const int bytes = real && o >= 0 ? 16 : 0;
+        const long long e = bytes ? o : -chunk * 16;
+        const uint32_t at = dst + place<C>(pw * 32 + row, chunk);
+        cp_async16(at, kb + e, bytes);
+        cp_async16(at + C::kTile, vb + e, bytes);
+      }
+      cp_arrive(&sh.full[stage]);
+      if (lane == 0) {
+        Note& note = sh.note[stage];
+        note.ok[pw] = ok;
+        if (pw == 0) {
+          note.b = now.b, note.sub = now.sub, note.t = now.t, note.nt = now.nt;
+          note.L = now.L, note.n_sink = now.vis.n_sink, note.gap = now.vis.gap;
+          note.n_keys = n_keys;
+        }
+        mbar_arrive(&sh.full[stage]);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+
+  __device__ __forceinline__ float* slot_of(long long cta, int which) const {
+    return reinterpret_cast<float*>(p.workspace) + (cta * 2 + which) * C::kSlot;
+  }
   // How the tiles are shared out: block c of n takes tiles [c T / n, (c + 1) T / n);
   // this one's run starts at `first`. Whole: runs of whole items instead.
   struct Share {
@@ -753,6 +1064,7 @@ struct Decoder {
   // The note's item ends with this tile, or the block's run does. g: the tile's
   // number among all.
   __device__ void end_segment(const Note& w, long long g, const Share& share) {
+    fold();
     // A segment of one tile may leave warps without keys.
     join_warps(w.t > 0 && g > share.first ? C::NW : min(C::NW, (w.n_keys + 15) / 16));
     const long long a = g - w.t, z = a + w.nt;  // the item's tiles
@@ -780,13 +1092,7 @@ struct Decoder {
       return;
     }
     // The warps share the parts, each in ascending order.
-#pragma unroll
-    for (int nt = 0; nt < C::NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < C::kRegs; ++i) o[nt][i / 4][i % 4] = 0.0f;
-    }
+    clear();
     for (long long c = c0 + warp; c <= c1; c += C::NW)
       add_part(slot_of(c, share.begin(c) >= a ? 0 : 1));
     join_warps((int)min((long long)C::NW, c1 - c0 + 1));
@@ -920,16 +1226,7 @@ template <class C>
 __global__ void __launch_bounds__(C::kThreads, C::kPerSm) paged_kernel(const PagedDecodeParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Block sh;
-  Decoder<C> d{p, sh};
-  d.smem = smem;
-  d.sbase = smem_u32(smem);
-  d.G = p.H / p.Hkv;
-  d.HB = (d.G + C::NT * 8 - 1) / (C::NT * 8);
-  d.SUB = p.Hkv * d.HB;
-  d.lane = threadIdx.x % 32;
-  d.warp = threadIdx.x / 32;
-  d.r = d.lane / 4;
-  d.q = d.lane % 4;
+  Decoder<C> d(p, sh, smem);
   d.run();
 }
 
@@ -939,7 +1236,7 @@ cudaError_t launch(const PagedDecodeParams& p, cudaStream_t stream) {
   static_assert(C::kPerSm >= 1 && sizeof(Block) <= C::kStatic && C::S <= 4, "a block fits an SM");
   const int G = p.H / p.Hkv;
   const long long most = std::min<long long>((long long)p.max_pages * p.page_size, 0x7fffffff);
-  const long long tiles = (long long)p.B * p.Hkv * ((G + C::NT * 8 - 1) / (C::NT * 8)) *
+  const long long tiles = (long long)p.B * p.Hkv * ((G + C::kItem - 1) / C::kItem) *
                           ((most + C::kKeys - 1) / C::kKeys);
   const int grid = (int)std::min<long long>(tiles, (long long)p.n_sms * C::kPerSm);
   static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
@@ -967,16 +1264,28 @@ size_t paged_decode_workspace(int B, int H, int Hkv, int D, int n_sms) {
 
 cudaError_t launch_paged_decode(const PagedDecodeParams& p, cudaStream_t stream) {
   using namespace paged;
-  // Stages and warps, measured (us): fp32 spends longer on a tile, so more and
-  // smaller blocks serve it better. Heads of 128 (16 x 6144 keys, 8 kv heads,
-  // floor 123): 2 warps with 2 stages, 3 blocks a SM, 166; 3 stages, 2 blocks
-  // 182; 4 warps, 1 block 177. Heads of 64: 2 warps with 3 stages, 4 blocks, 142;
-  // 4 warps with 2 or 3 stages 145. bf16, heads of 128 (64 x 6144 keys, floor
-  // 246): 4 warps with 3 stages, 2 blocks, 244; with 2 stages, 3 blocks 259.
-  const bool wide = p.H / p.Hkv > 8;  // more than one column tile
-  if (p.in_fp32)
-    return p.D > 64 ? launch<Cfg<128, true, 1, 2, 2>>(p, stream)
-                    : launch<Cfg<64, true, 1, 2, 3>>(p, stream);
+  // Warps and stages, measured (us). fp32 on the FMA pipe (16 x 6144 keys,
+  // floor 123), 8 kv heads of 128: 2 warps with 2 stages, 3 blocks a SM, 130 for
+  // one or two heads a group, 138 for four; 3 stages, 2 blocks 128, 142, 156;
+  // 4 warps with 2 stages 147, 148, 169. 16 kv heads of 64: 4 warps with 3 stages,
+  // 2 blocks, 129, 127, 136; 2 stages, 3 blocks 132, 131, 139; 2 warps with 4
+  // stages 128, 138, and 24 against 15 for one sequence of 5000. On the tensor pipe
+  // any group of fp32 heads takes 180 (128 dims) or 147 (64).
+  // bf16, heads of 128 (64 x 6144 keys, floor 246): 4 warps with 3 stages, 2 blocks,
+  // 244; with 2 stages, 3 blocks 259.
+  const int group = p.H / p.Hkv;
+  const bool wide = group > 8;  // more than one column tile
+  if (p.in_fp32) {
+    if (p.D > 64)
+      return group == 1   ? launch<Cfg<128, true, 1, 2, 2, 1>>(p, stream)
+             : group == 2 ? launch<Cfg<128, true, 1, 2, 2, 2>>(p, stream)
+             : group <= 4 ? launch<Cfg<128, true, 1, 2, 2, 4>>(p, stream)
+                          : launch<Cfg<128, true, 1, 2, 2>>(p, stream);
+    return group == 1   ? launch<Cfg<64, true, 1, 4, 3, 1>>(p, stream)
+           : group == 2 ? launch<Cfg<64, true, 1, 4, 3, 2>>(p, stream)
+           : group <= 4 ? launch<Cfg<64, true, 1, 4, 3, 4>>(p, stream)
+                        : launch<Cfg<64, true, 1, 2, 3>>(p, stream);
+  }
   if (p.D > 64)
     return wide ? launch<Cfg<128, false, 2, 4, 3>>(p, stream)
                 : launch<Cfg<128, false, 1, 4, 3>>(p, stream);

@@ -136,6 +136,22 @@ def test_long_sums_are_not_cut(cuda, dtype, D):
     assert ((out[0].double() - want).abs() / want).max() <= 1e-6
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [2, 4, 8])
+def test_long_sums_are_not_cut_in_groups(cuda, D, G):
+    """The same in fp32 for groups of query heads, whose products take other
+    pipes than single heads'; the bound's reason is the same."""
+    import torch
+    from enilnets_b200 import kernels
+    q, kp, vp, table, lens = _case(41, [16000], 64 * G, 64, D, 16, "fp32")
+    kp = torch.where(torch.isnan(kp), kp, 0.01 * kp)
+    value = 1.0 + torch.rand((D,), device="cuda").to(vp.dtype)
+    vp = torch.where(torch.isnan(vp), vp, value)
+    out = kernels.attention_decode_paged(q, kp, vp, table, lens, out_dtype=torch.float32)
+    want = value.double()
+    assert ((out[0].double() - want).abs() / want).max() <= 1e-6
+
+
 def test_many_sequences(cuda):
     """More (sequence, head) pairs than blocks: several whole ones each."""
     lens = list(np.random.RandomState(0).randint(0, 90, 300))
