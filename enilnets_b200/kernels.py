@@ -722,6 +722,7 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
 # A decode step makes several of these calls per layer, each a few microseconds
 # of GPU time, so their host side is kept short: one test per operand (the
 # message is built only on failure), one struct built from positional values.
+_DENSE = torch.contiguous_format  # (empty_like: two thirds of new_empty's host time)
 _raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index
 _current_device = torch._C._cuda_getDevice
 
@@ -839,8 +840,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     if out is None:
         out_dtype = out_dtype or dt
-        q_out = q.new_empty(qshape, dtype=out_dtype)
-        k_out = q.new_empty(kshape, dtype=out_dtype)
+        q_out = torch.empty_like(q, dtype=out_dtype, memory_format=_DENSE)
+        k_out = torch.empty_like(k, dtype=out_dtype, memory_format=_DENSE)
     else:
         q_out, k_out = out
     qos = _require_heads("q_out", q_out, qshape, None, dev)
@@ -887,7 +888,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     pool, ps = _require_pool(k_pages, v_pages, block_table, B, Hkv, D, dt, dev)
     wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     if out is None:
-        out = q.new_empty(qshape)
+        out = torch.empty_like(q, memory_format=_DENSE)
     os_ = _require_heads("out", out, qshape, dt, dev)
     code = _DTYPES[dt]
     a = nat.QkNormRopeArgs(
@@ -936,8 +937,8 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: Optiona
         ks = _require_heads("k", k, kshape, in_dt, dev)
     if out is None:
         out_dtype = out_dtype or in_dt
-        dq = dq_out.new_empty(qshape, dtype=out_dtype)
-        dk = dq_out.new_empty(kshape, dtype=out_dtype)
+        dq = torch.empty_like(dq_out, dtype=out_dtype, memory_format=_DENSE)
+        dk = torch.empty_like(dk_out, dtype=out_dtype, memory_format=_DENSE)
     else:
         dq, dk = out
     dqs = _require_heads("dq", dq, qshape, None, dev)
