@@ -23,9 +23,9 @@
 //    estimated from the maxima and one vector a thread, one more pass for the
 //    exact total, and the same list, provided that it carries the exact share.
 //  * larger top-k, flatter nuclei: a histogram of a quarter of the logits guesses
-//    the bins around the cut (shared-memory atomics take 1.4 tokens a cycle, so
-//    one of all the logits cost 92 us of 256 rows of 131072); one pass sums what
-//    lies above them, and the total where it is not known, and lists their
+//    the bins around the cut (16 us a row of 131072; one of all the logits would
+//    cost more than the wrong guesses do); one pass (34 us) sums what lies above
+//    them, and the total where it is not known, and lists their
 //    tokens. The exact sums confirm the guess or correct it for another pass.
 //    The cut and the draw follow from the list and the warps' sums.
 //  * rows that defeat the bins (thousands of equal logits at the cut): bisection
@@ -55,9 +55,9 @@ constexpr int kGroupBins = 256;  // bins over the group maxima
 constexpr int kBins = 2048;      // bins over the row
 constexpr int kTries = 16;       // passes with guessed bins (the last halve what is left)
 // One vector in kSample goes into the histogram, kWindow tokens are listed to
-// each side of a guessed cut: wider samples and windows cost more than the wrong
-// guesses that they save (256 flat rows of 131072, top-p 0.9: 161 us; with 8 and
-// 800 a third more, with 4 and 300 a fifteenth).
+// each side of a guessed cut. Measured (256 flat rows of 131072, top-p 0.9 and
+// 0.99, us): 4 and 650: 159, 179; 4 and 500: 168, 153; 4 and 780: 212, 214 (lists
+// that overflow); 2 and 650: 172, 179.
 constexpr int kSample = 4;
 constexpr int kWindow = 650;
 // Tokens above e^-kHeavy are weighed one by one in the histogram, lighter ones by
