@@ -396,6 +396,14 @@ struct Sampler {
     return top == INFINITY ? top : top - kLive / inv_t;
   }
 
+  // A block's shared memory may be reached only once the block runs: each says so
+  // at its start and waits for the others before its first access to theirs.
+  __device__ __forceinline__ void started() const {
+    if (n_blocks > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  }
+  __device__ __forceinline__ void wait_started() const {
+    if (n_blocks > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+  }
   // Waits for the cluster's blocks; shared memory written before is visible
   // after, to all of them.
   __device__ __forceinline__ void sync() const {
@@ -1224,6 +1232,7 @@ struct Sampler {
       }
     }
     if (n_blocks > 1) {
+      wait_started();
       const Pair* p = exchange(__float_as_uint(top),
                                ((u64)__float_as_uint(low) << 32) | __float_as_uint(least));
       for (int r = 0; r < n_blocks; ++r) {
@@ -1422,6 +1431,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int b = blockIdx.x / n_blocks;
   const uint8_t* row = reinterpret_cast<const uint8_t*>(p.logits) + b * p.stride * (kF32 ? 4 : 2);
   Sampler<kF32> s(row, p.V, sm, n_blocks, n_blocks > 1 ? cluster_rank() : 0);
+  s.started();
   const float T = p.temperature ? p.temperature[b] : p.temperature_all;
   s.inv_t = T > 0.0f ? 1.0f / fminf(T, 1.0e38f) : 1.0f;
   s.min_p = fminf(p.min_p ? p.min_p[b] : p.min_p_all, 1.0f);  // the best token stays

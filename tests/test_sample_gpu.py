@@ -180,6 +180,26 @@ def test_mixed_settings_per_row(cuda):
                                            float(p[b]), float(m[b])), b
 
 
+@pytest.mark.parametrize("dtype,V", [("fp32", 2049), ("fp32", 4097), ("fp32", 8200),
+                                     ("bf16", 4097), ("bf16", 8195), ("bf16", 16401)])
+def test_rows_just_long_enough_for_several_blocks(cuda, dtype, V):
+    """Vocabularies one vector past the size that gives a row another block: the
+    last block has next to nothing to read and reaches the exchange of the row's
+    extremes at once. The same tokens every time, and the definition's."""
+    from enilnets_b200 import kernels
+    B = 6
+    x = _dev(_rows(V, B, V), dtype)
+    host = x.double().cpu().numpy()
+    u = np.random.RandomState(V).random_sample(B).astype(np.float32)
+    for kw in (dict(temperature=0.0), dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.8),
+               dict(min_p=0.1)):
+        first = kernels.sample_tokens(x, _dev(u), **kw).cpu().numpy()
+        for b in range(B):
+            assert first[b] in ref.sample_answers(host[b], float(u[b]), **kw), (kw, b)
+        again = [kernels.sample_tokens(x, _dev(u), **kw) for _ in range(50)]
+        assert all((t.cpu().numpy() == first).all() for t in again), kw
+
+
 def test_weights_equal_the_elementary_form(cuda):
     """The kernel's weights are those of elementary fp32 operations bit for bit:
     the draw, exact in whole numbers, equals one computed from exp() of torch."""
