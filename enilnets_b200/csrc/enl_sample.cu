@@ -251,6 +251,9 @@ struct Shared {
   u64 part[kWarps];
   u64 wsum[kWarps * kMaxCluster];  // rank 0: kept weight of every warp's range
   float fpart[kWarps];
+  // Warps' shares of the estimated total: not in `part`, whose extremes slower
+  // warps of a lone block may still be reading.
+  u64 est[kWarps];
   Pair swap[2][kMaxCluster];  // what the cluster's blocks tell each other
   uint32_t gbins[kGroupBins], gmass[kGroupBins];  // groups, and their maxima's weight
   union {
@@ -1306,13 +1309,13 @@ struct Sampler {
           sample += __shfl_xor_sync(0xffffffffu, sample, off);
         }
         if (lane == 0)
-          sm.part[tid / 32] = ((u64)__float_as_uint(sure) << 32) | __float_as_uint(sample);
+          sm.est[tid / 32] = ((u64)__float_as_uint(sure) << 32) | __float_as_uint(sample);
         __syncthreads();
         sure = sample = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          sure += __uint_as_float((uint32_t)(sm.part[w] >> 32));
-          sample += __uint_as_float((uint32_t)sm.part[w]);
+          sure += __uint_as_float((uint32_t)(sm.est[w] >> 32));
+          sample += __uint_as_float((uint32_t)sm.est[w]);
         }
         if (n_blocks > 1) {
           const Pair* p = exchange(__float_as_uint(sure), __float_as_uint(sample));

@@ -200,6 +200,25 @@ def test_rows_just_long_enough_for_several_blocks(cuda, dtype, V):
         assert all((t.cpu().numpy() == first).all() for t in again), kw
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V", [3, 40, 515, 2047, 4095])
+def test_top_p_of_rows_with_a_block_each(cuda, dtype, V):
+    """More rows than SMs and small vocabularies, so that a row has one block and
+    some of its warps have nothing to read: the estimate of the total follows the
+    extremes at once. The same tokens every time, and the definition's."""
+    from enilnets_b200 import kernels
+    B = 300
+    x = _dev(np.concatenate([_rows(V, B // 2, V), _rows(V + 1, B // 2, V, flat=0.8)]), dtype)
+    host = x.double().cpu().numpy()
+    u = np.random.RandomState(V).random_sample(B).astype(np.float32)
+    for kw in (dict(top_p=0.5), dict(top_p=0.9), dict(top_p=0.99, temperature=1.4)):
+        first = kernels.sample_tokens(x, _dev(u), **kw).cpu().numpy()
+        for b in range(B):
+            assert first[b] in ref.sample_answers(host[b], float(u[b]), **kw), (kw, b)
+        again = [kernels.sample_tokens(x, _dev(u), **kw) for _ in range(50)]
+        assert all((t.cpu().numpy() == first).all() for t in again), kw
+
+
 def test_weights_equal_the_elementary_form(cuda):
     """The kernel's weights are those of elementary fp32 operations bit for bit:
     the draw, exact in whole numbers, equals one computed from exp() of torch."""
