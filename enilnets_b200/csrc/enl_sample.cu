@@ -592,8 +592,8 @@ struct Sampler {
   // The entry of the list (n of them) at which the running sum reaches `need`:
   // of ones or whole weights from the largest composite down, or (kIndex) of
   // those with w >= min_p in index order; only entries at or above C count.
-  // Entries are narrowed to one of 256 bins of the order's value at a time (equal
-  // logits by their indices), and the last few ranked by counting.
+  // Entries are narrowed to one of 256 bins of the order's value at a time, and
+  // the last few ranked by counting.
   template <Order kOrder>
   __device__ u64 select(int n, u64 need, u64 C) const {
     const int tid = threadIdx.x;
@@ -613,35 +613,59 @@ struct Sampler {
       if (q[e]) alive |= 1 << e;
     }
     u64 base = 0;  // weight before the entries that are left
-    bool by_index = kOrder == kIndex;
-    auto place = [&](u64 x) { return by_index ? (float)index_of(x) : top - logit_of(x); };
+    // Bins are even in the distance from the top. Unequal logits can share that
+    // distance (1e-9 and 2e-9 are both 1 away from 1), so where all that are left
+    // do, bins go by the logits' bits, and where those are equal, by index.
+    enum { kValue, kBits, kPlace } by = kOrder == kIndex ? kPlace : kValue;
+    auto distance = [&](u64 x) { return top - logit_of(x); };
+    auto number = [&](u64 x) { return by == kBits ? ~(uint32_t)(x >> 32) : index_of(x); };
     int left = (int)block_sum(__popc(alive), sm);
     while (left > kRank) {
       float lo = INFINITY, hi = -INFINITY;
+      uint32_t first = ~0u, last = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (alive >> e & 1) lo = fminf(lo, place(c[e])), hi = fmaxf(hi, place(c[e]));
+        if (alive >> e & 1) {
+          if (by == kValue)
+            lo = fminf(lo, distance(c[e])), hi = fmaxf(hi, distance(c[e]));
+          else
+            first = min(first, number(c[e])), last = max(last, number(c[e]));
+        }
+      if (by == kValue) {
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        for (int off = 16; off > 0; off >>= 1) {
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        }
+      } else {
+        first = __reduce_min_sync(0xffffffffu, first);
+        last = __reduce_max_sync(0xffffffffu, last);
       }
       __syncthreads();
       if (tid % 32 == 0)
-        sm.part[tid / 32] = ((u64)__float_as_uint(lo) << 32) | __float_as_uint(hi);
+        sm.part[tid / 32] = by == kValue
+                                ? ((u64)__float_as_uint(lo) << 32) | __float_as_uint(hi)
+                                : ((u64)first << 32) | last;
       if (tid < kGroupBins) sm.mass[tid] = 0;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        lo = fminf(lo, __uint_as_float((uint32_t)(sm.part[w] >> 32)));
-        hi = fmaxf(hi, __uint_as_float((uint32_t)sm.part[w]));
+        const uint32_t a = (uint32_t)(sm.part[w] >> 32), b = (uint32_t)sm.part[w];
+        if (by == kValue)
+          lo = fminf(lo, __uint_as_float(a)), hi = fmaxf(hi, __uint_as_float(b));
+        else
+          first = min(first, a), last = max(last, b);
       }
-      if (!(hi > lo)) {  // equal logits follow each other by index
-        by_index = true;
+      if (by == kValue ? !(hi > lo) : first == last) {  // never by index: those differ
+        by = by == kValue ? kBits : kPlace;
         continue;
       }
       const float scale = (float)kGroupBins / fminf(hi - lo, 3.0e38f);
-      auto bin_of = [&](u64 x) { return min(kGroupBins - 1, (int)((place(x) - lo) * scale)); };
+      const u64 span = (u64)(last - first) + 1;
+      auto bin_of = [&](u64 x) {
+        return by == kValue ? min(kGroupBins - 1, (int)((distance(x) - lo) * scale))
+                            : (int)((u64)(number(x) - first) * kGroupBins / span);
+      };
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (alive >> e & 1) atomicAdd(&sm.mass[bin_of(c[e])], q[e]);

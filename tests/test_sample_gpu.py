@@ -219,6 +219,27 @@ def test_top_p_of_rows_with_a_block_each(cuda, dtype, V):
         assert all((t.cpu().numpy() == first).all() for t in again), kw
 
 
+@pytest.mark.parametrize("B", [3, 200])
+@pytest.mark.parametrize("top", [1.0, 3e4, 1e30])
+def test_logits_that_share_their_distance_from_the_largest(cuda, B, top):
+    """One logit above many unequal ones that are all the same fp32 distance below
+    it: their order is still theirs, not their indices'. Temperatures that keep
+    their weights well above zero."""
+    from enilnets_b200 import kernels
+    rng = np.random.RandomState(3)
+    for V, k in ((1000, 300), (1500, 1000), (9000, 700), (9000, 5000)):
+        x = (1e-9 * top * rng.standard_normal((B, V))).astype(np.float32)
+        x[:, V // 3] = top
+        u = rng.random_sample(B).astype(np.float32)
+        for kw in (dict(top_k=k), dict(top_k=k, top_p=0.9), dict(top_p=0.4),
+                   dict(top_k=k, top_p=0.7, min_p=0.3)):
+            kw["temperature"] = top
+            got = kernels.sample_tokens(_dev(x), _dev(u), **kw).tolist()
+            for b in range(0, B, max(1, B // 8)):
+                answers = ref.sample_answers(x[b].astype(np.float64), float(u[b]), **kw)
+                assert got[b] in answers, (V, kw, b, got[b], answers)
+
+
 def test_weights_equal_the_elementary_form(cuda):
     """The kernel's weights are those of elementary fp32 operations bit for bit:
     the draw, exact in whole numbers, equals one computed from exp() of torch."""
