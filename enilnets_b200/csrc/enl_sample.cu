@@ -1460,7 +1460,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   Sampler<kF32> s(row, p.V, sm, n_blocks, n_blocks > 1 ? cluster_rank() : 0);
   s.started();
   const float T = p.temperature ? p.temperature[b] : p.temperature_all;
-  s.inv_t = T > 0.0f ? 1.0f / fminf(T, 1.0e38f) : 1.0f;
+  // (finite and not zero: a difference of zero weighs one at any temperature)
+  s.inv_t = T > 0.0f ? 1.0f / fminf(fmaxf(T, 1.2e-38f), 1.0e38f) : 1.0f;
   s.min_p = fminf(p.min_p ? p.min_p[b] : p.min_p_all, 1.0f);  // the best token stays
   s.run(row, T, p.top_k ? p.top_k[b] : p.top_k_all, p.top_p ? p.top_p[b] : p.top_p_all, p.u[b],
         p.tokens + b);

@@ -574,7 +574,7 @@ typedef struct enl_sample_args {
   const int32_t* top_k;
   const float* top_p;
   const float* min_p;
-  float temperature_all; /* <= 0: greedy */
+  float temperature_all; /* <= 0: greedy; else taken within [1.2e-38, 1e38] */
   int32_t top_k_all;     /* <= 0: off */
   float top_p_all;       /* >= 1: off */
   float min_p_all;       /* <= 0: off */

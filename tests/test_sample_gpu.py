@@ -240,6 +240,30 @@ def test_logits_that_share_their_distance_from_the_largest(cuda, B, top):
                 assert got[b] in answers, (V, kw, b, got[b], answers)
 
 
+@pytest.mark.parametrize("T", [1e-45, 1e-40, 1e-38, 1e-30])
+def test_lowest_temperatures(cuda, T):
+    """A temperature whose reciprocal passes fp32 leaves the largest logit alone,
+    under any setting; equal ones share the draw."""
+    import torch
+    from enilnets_b200 import kernels
+    rng = np.random.RandomState(2)
+    for B, V in ((3, 9), (3, 5000), (3, 70000), (200, 5000)):
+        x = _dev(rng.standard_normal((B, V)))
+        want = x.argmax(-1)
+        u = _dev(rng.random_sample(B))
+        tie = torch.zeros((B, V), device="cuda")
+        tie[:, V // 2:V // 2 + 4] = 3.0
+        for kw in (dict(), dict(min_p=0.1), dict(top_k=5), dict(top_k=2000), dict(top_p=0.5),
+                   dict(top_k=50, top_p=1.0 - 2.0 ** -10, min_p=0.5)):
+            out = torch.full((B,), -77, dtype=torch.int64, device="cuda")
+            t = torch.full((B,), T, device="cuda")
+            assert torch.equal(kernels.sample_tokens(x, u, temperature=T, out=out, **kw), want), kw
+            assert torch.equal(kernels.sample_tokens(x, u, temperature=t, **kw), want), kw
+            if "top_p" not in kw:
+                got = kernels.sample_tokens(tie, u, temperature=T, **kw)
+                assert torch.equal(got, V // 2 + (u * 4).long()), kw
+
+
 def test_weights_equal_the_elementary_form(cuda):
     """The kernel's weights are those of elementary fp32 operations bit for bit:
     the draw, exact in whole numbers, equals one computed from exp() of torch."""
