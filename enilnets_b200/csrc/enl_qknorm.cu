@@ -305,7 +305,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           ss = f2_fma(x1, x1, f2_fma(x2, x2, ss));
           gx = f2_fma(f2_mul(d1[e], w1.pair(e)), x1, f2_fma(f2_mul(d2[e], w2.pair(e)), x2, gx));
         }
-        const float r = rsqrtf(fmaf(group_sum<LG>(pair_sum(ss)), inv_d, p.eps));
+        // Zeros stand in for heads that are not there: with eps = 0 the floor, the
+        // smallest fp32 number, keeps their rstd finite and their share of dw zero
+        // (training backward 62.8 us; with a test for them 65.9).
+        const float r = rsqrtf(fmaxf(fmaf(group_sum<LG>(pair_sum(ss)), inv_d, p.eps), 1.4e-45f));
         const float m = group_sum<LG>(pair_sum(gx)) * inv_d * r * r;  // mean(g xh) rstd
         const uint64_t rr = both(r), nm = both(-m);
 #pragma unroll

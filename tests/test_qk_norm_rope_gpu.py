@@ -149,6 +149,35 @@ def test_backward(cuda, B, S, H, Hkv, D, in_dtype, grad_dtype, norm, rope):
         assert a is None or torch.equal(a, b)  # the sums' order is fixed
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("B,S,H,Hkv,D", [(1, 1, 1, 1, 64), (2, 7, 4, 1, 64), (2, 7, 4, 2, 40),
+                                         (3, 5, 3, 3, 128), (1, 33, 5, 5, 24), (2, 9, 8, 4, 128)])
+def test_backward_without_eps(cuda, B, S, H, Hkv, D, dtype):
+    """eps = 0 over heads that are not zero: heads and tokens that only fill up a
+    block's share, and tokens outside the tables, add nothing to the weights'
+    gradients."""
+    import torch
+    from enilnets_b200 import _native, kernels
+    rng = np.random.RandomState(S + D)
+    q, k, _, wq, wk = _inputs(S + D, B, S, H, Hkv, D, dtype)
+    wq, wk = wq.astype(np.float32), wk.astype(np.float32)
+    dq, dk = _t(rng.standard_normal(q.shape)), _t(rng.standard_normal(k.shape))
+    cos, sin = _tables(S + 1, D)
+    for rows in (S + 1, S):  # all tokens have angles; all but the last one
+        _native.device_error(clear=True)
+        gq, gk, gwq, gwk = kernels.qk_norm_rope_backward(
+            dq, dk, q, k, _t(wq), _t(wk), eps=0.0, rope=(_t(cos[:rows]), _t(sin[:rows])), pos0=1,
+            out_dtype=torch.float32)
+        assert _native.device_error(clear=True)[0] == (0 if rows > S else 2)
+        n = rows - 1
+        c, s = cos[1:rows, None], sin[1:rows, None]
+        for got, dw, x, dy, w in ((gq, gwq, q, dq, wq), (gk, gwk, k, dk, wk)):
+            want, wantw = ref.norm_rope_backward(_np(dy)[:, :n], _np(x)[:, :n], w, 0.0, c, s)
+            _close(_np(got)[:, :n], want, "fp32")
+            assert torch.count_nonzero(got[:, n:]) == 0
+            assert np.abs(_np(dw) - wantw).max() <= 1e-5 * np.sqrt(x[..., 0].numel()) + 1e-5
+
+
 def test_backward_matches_differences_of_the_forward(cuda):
     """<gradient, direction> against central differences of the fp32 forward.
     The loss sums N = 2*40*6*64 products; fp32 rounding of the forward gives it
