@@ -725,6 +725,7 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
 _DENSE = torch.contiguous_format  # (empty_like: two thirds of new_empty's host time)
 _raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index
 _current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _describe(t) -> str:
@@ -972,10 +973,22 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: Optiona
 _zeroed: dict = {}
 
 
-def _zeroed_workspace(dev: int, nbytes: int) -> torch.Tensor:
+def _paged_counter_bytes(B: int, H: int, Hkv: int) -> int:
+    """The end of attention_decode_paged's workspace that has to be zero before
+    its first use: four bytes for each eight heads of a group, in units of 256."""
+    return -(-(B * Hkv * -(-H // (8 * Hkv)) * 4) // 256) * 256
+
+
+def _zeroed_workspace(dev: int, nbytes: int, counters: int) -> torch.Tensor:
     """Scratch of attention_decode_paged, one per (device, stream) like
     _workspace, zeroed when it is made: its kernels leave the counters in it at
-    zero for the next call."""
+    zero for the next call. A call under capture gets scratch of its graph
+    instead, whose counters every replay zeroes: what is kept here may be replaced,
+    and freed, when a later call needs more, and a graph would go on writing to it."""
+    if _capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+        ws[nbytes - counters:].zero_()
+        return ws
     key = (dev, _raw_stream(dev))
     ws = _zeroed.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -1008,8 +1021,8 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     are seen, or with a window those at most `window` back and the sequence's
     first `sinks`. H % Hkv == 0 with any ratio; D a multiple of 8 up to 128.
     A sequence of length 0 gives zeros and an LSE of -inf. workspace: a zeroed
-    uint8 tensor of paged_decode_workspace_bytes (kept per stream by default; a
-    CUDA graph that replays beside other calls needs its own).
+    uint8 tensor of paged_decode_workspace_bytes, for calls that do not overlap
+    (default: one kept per stream, or under capture one of the graph's own memory).
     Returns out (B, H, D) in out_dtype (default: q's) [and lse (B, H) fp32].
     """
     dev = _device_of("q", q, "batch, heads, head_dim")
@@ -1043,7 +1056,8 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         lib = nat.load()
         if workspace is None:
             workspace = _zeroed_workspace(
-                dev, lib.enl_paged_decode_workspace_bytes(ctypes.byref(a)))
+                dev, lib.enl_paged_decode_workspace_bytes(ctypes.byref(a)),
+                _paged_counter_bytes(B, H, pool[1]))
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}, got "
                              f"{_describe(workspace)}")

@@ -293,6 +293,80 @@ def test_graph_replay_with_growing_lengths(cuda):
         assert torch.equal(out, kernels.attention_decode_paged(q, kp, vp, table, lens)), step
 
 
+def _captured(case, stream):
+    """(graph, its output) of one call with the default workspace."""
+    import torch
+    from enilnets_b200 import kernels
+    out = torch.zeros_like(case[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        kernels.attention_decode_paged(*case, out=out)
+    return g, out
+
+
+def test_graphs_do_not_share_the_streams_workspace(cuda):
+    """Graphs captured on one stream with the default workspace, from the largest
+    batch down and replayed in the other order, with the stream's own calls in
+    between and whatever the memory held before."""
+    import torch
+    from enilnets_b200 import kernels
+    cases = [_case(50 + n, [900 + 10 * i for i in range(n)], 8, 2, 64, 16, "bf16")
+             for n in (40, 8, 2)]
+    want = [kernels.attention_decode_paged(*c) for c in cases]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graphs = [_captured(c, stream) for c in cases]
+    kept = kernels._zeroed.get((torch.cuda.current_device(), stream.cuda_stream))
+    if kept is not None:  # made under capture, not zeroed before the first graph replays
+        kept.fill_(255)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            for (g, out), w, c in zip(graphs[::-1], want[::-1], cases[::-1]):
+                out.zero_()
+                g.replay()
+                eager = kernels.attention_decode_paged(*c)
+                stream.synchronize()
+                assert torch.equal(out, w) and torch.equal(eager, w)
+
+
+@pytest.mark.parametrize("B,H,Hkv", [(2, 8, 2), (3, 40, 2), (65, 9, 1), (20, 16, 16)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_only_the_counters_need_zeros(cuda, dtype, B, H, Hkv):
+    import torch
+    from enilnets_b200 import kernels
+    case = _case(B, [2000 + 7 * i for i in range(B)], H, Hkv, 64, 16, dtype)
+    n = kernels.paged_decode_workspace_bytes(B, H, Hkv, 64)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    ws[n - kernels._paged_counter_bytes(B, H, Hkv):] = 0
+    want = kernels.attention_decode_paged(*case)
+    for _ in range(2):
+        assert torch.equal(kernels.attention_decode_paged(*case, workspace=ws), want)
+
+
+def test_graph_keeps_its_workspace_when_the_streams_grows(cuda):
+    """A graph captured after a small eager call; a larger one then replaces the
+    stream's workspace, whose memory goes to the next tensor of its size."""
+    import torch
+    from enilnets_b200 import kernels
+    small = _case(60, [700, 300], 8, 2, 64, 16, "bf16")
+    large = _case(61, [300] * 64, 8, 2, 64, 16, "bf16")
+    want = kernels.attention_decode_paged(*small)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        kernels.attention_decode_paged(*small)
+        stream.synchronize()
+        g, out = _captured(small, stream)
+        n = kernels.paged_decode_workspace_bytes(2, 8, 2, 64)
+        kernels.attention_decode_paged(*large)
+        others = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        g.replay()
+        stream.synchronize()
+        assert torch.equal(out, want)
+        assert all((t == 255).all() for t in others)
+
+
 def test_refusals(cuda):
     import torch
     from enilnets_b200 import kernels
