@@ -268,9 +268,14 @@ def sample(logits, u, temperature: float = 1.0, top_p: Optional[float] = None,
            top_k: Optional[int] = None, min_p: Optional[float] = None,
            greedy: bool = False) -> List[int]:
     """Token ids drawn from logits (B, V) with the uniform numbers u (B,), one
-    device call and one copy of B numbers back."""
+    device call and one copy of B numbers back. Raises ValueError when a row has
+    no logit to draw from (all of them NaN or -inf)."""
     import torch
     out = kernels.sample_tokens(
         logits, to_device(np.asarray(u, dtype=np.float32), torch.float32),
         temperature=0.0 if greedy else float(temperature), top_k=top_k, top_p=top_p, min_p=min_p)
-    return out.tolist()
+    tokens = out.tolist()
+    dead = [b for b, t in enumerate(tokens) if t < 0]
+    if dead:
+        raise ValueError(f"no token to draw in rows {dead}: every logit is NaN or -inf")
+    return tokens

@@ -177,6 +177,23 @@ def test_serve_samples_as_generate_does(cuda, gen):
         assert gen.serve_ids(["keys"], **kw) == [want]
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(greedy=True), dict(top_k=3, temperature=0.5)])
+def test_rows_without_a_logit_are_refused(cuda, gen, kw):
+    """A row of NaN and -inf has no token: the draw raises, and so does serve on a
+    model that gives such rows, instead of feeding a token number -1 on."""
+    import torch
+    nan, inf = float("nan"), float("inf")
+    x = torch.tensor([[0.0, 1.0, -inf], [nan, -inf, nan], [1.0, nan, -inf], [-inf] * 3],
+                     device="cuda")
+    with pytest.raises(ValueError, match=r"rows \[1, 3\]"):
+        serving.sample(x, [0.5] * 4, **kw)
+    assert serving.sample(x[::2].contiguous(), [0.999, 0.5], **kw) == [1, 0]
+    head = gen.network.layers[-1]
+    head["bias"] = np.full_like(head["bias"], nan)
+    with pytest.raises(ValueError, match="every logit is NaN or -inf"):
+        gen.serve_ids(["keys", "a"], max_new_tokens=3, **kw)
+
+
 def test_serve_stops_at_the_model_length(cuda, gen):
     ids = gen.serve_ids(["the cache keeps keys", "a"], max_new_tokens=60, greedy=True)
     want = [gen.generate_ids(p, max_new_tokens=60, greedy=True)
