@@ -34,19 +34,22 @@
 // the result does not depend on timing. Short sequences (up to kWholeTiles
 // tiles) are not divided: joining two parts costs about four tiles' time.
 //
-// Precision: scores, softmax and sums in fp32. bf16: products of bf16 inputs
-// are exact; the probabilities are split into two bf16 parts (16 bits of
-// mantissa), which costs a second product and keeps their rounding out of the
-// output. fp32 on the FMA pipe: a tile's sum by itself, then added to the running
-// one, so that equal values do not add up equal roundings. fp32 on the tensor
-// pipe: each factor is split into two tf32 parts (values into three) and the
-// three (four) largest products are added, about 2^-21 of each. The tensor pipe cuts its sums instead of rounding them, always towards zero, so nothing
-// is summed in it for long: a few products at a time start from zero and are
-// added to the running sums by rounded additions (without that, 16000 equal fp32
-// values came out 3e-5 small). Only bf16 with two column tiles has no registers
-// for it (342 us against 298 for 64 sequences of 6144 with 16 query heads a key
-// head): its running sums stay in the pipe, and 16000 equal values come out 2e-6
-// small, far below the rounding of a bf16 output.
+// Precision: scores, softmax and sums in fp32. bf16: products of bf16 inputs are
+// exact, and a probability is cut into three bf16 parts that hold it exactly. (With
+// two parts the relative error of an fp32 output over 4000 random keys is 1.7e-6
+// instead of 1.8e-7, in the same time up to eight heads a group, where the bytes
+// bound it.) The parts have one sign and none is zero, so that an infinite value
+// comes out infinite. fp32 on the FMA pipe: a tile's sum by itself, then added to
+// the running one, so that equal values do not add up equal roundings. fp32 on the
+// tensor pipe: each factor is split into two tf32 parts (values into three) and the
+// three (four) largest products are added, about 2^-21 of each. The tensor pipe
+// cuts its sums instead of rounding them, always towards zero, so nothing is summed
+// in it for long: a few products at a time start from zero and are added to the
+// running sums by rounded additions, two an instruction (without that, 16000 equal
+// fp32 values came out 3e-5 small). With two column tiles these additions show: 64
+// sequences of 12288, four key heads of 128 with 16 query heads each, take 308 us,
+// against 304 with sums that stay in the pipe (16000 equal values then come out
+// 1e-5 small instead of 4e-7) and 293 with two parts of a probability as well.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -177,8 +180,8 @@ __device__ __forceinline__ void mma_tf32_first(float (&c)[4], const uint32_t (&a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void add4(float (&c)[4], const float (&t)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] += t[i];
+  f2_unpack(f2_add(f2_pack(c[0], c[1]), f2_pack(t[0], t[1])), c[0], c[1]);
+  f2_unpack(f2_add(f2_pack(c[2], c[3]), f2_pack(t[2], t[3])), c[2], c[3]);
 }
 __device__ __forceinline__ float4 lds4(uint32_t addr) {
   float4 f;
@@ -207,9 +210,22 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo, 
   lo = __float_as_uint(left) & 0xffffe000u;
   rest = __float_as_uint(left - __uint_as_float(lo));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
+// The upper 8 bits of the mantissas of x and y as two bf16; x and y are left with
+// the rest. After three cuts nothing is left.
+__device__ __forceinline__ uint32_t cut_bf16(float& x, float& y) {
+  const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+  x -= __uint_as_float(u & 0xffff0000u);
+  y -= __uint_as_float(v & 0xffff0000u);
+  return __byte_perm(u, v, 0x7632);
+}
+// The smallest normal number in place of zeros: a probability's lower parts times
+// an infinite value are infinite like the upper part times it, where zero (or a
+// part of the other sign) would make NaN.
+__device__ __forceinline__ uint32_t above_zero(uint32_t pair) {
+  const uint32_t tiny = 0x00800080u;
+  const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&pair),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&tiny));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Swizzled place of 16-byte chunk `chunk` of row `row`: eight rows of one chunk
@@ -439,15 +455,15 @@ struct MmaMath : Base<C> {
         }
       }
     } else {
-      uint32_t bh[C::NT][2], bl[C::NT][2];
+      uint32_t hi[C::NT][2], mid[C::NT][2], lo[C::NT][2];
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const float x = pr[nt][2 * half], y = pr[nt][2 * half + 1];
-          const uint32_t hi = pack_bf16(x, y);
-          bh[nt][half] = transpose8(hi);
-          bl[nt][half] = transpose8(pack_bf16(x - bf16lo_to_f32(hi), y - bf16hi_to_f32(hi)));
+          float x = pr[nt][2 * half], y = pr[nt][2 * half + 1];
+          hi[nt][half] = transpose8(cut_bf16(x, y));
+          mid[nt][half] = transpose8(above_zero(cut_bf16(x, y)));
+          lo[nt][half] = transpose8(above_zero(cut_bf16(x, y)));
         }
       const int row = warp * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
@@ -456,15 +472,11 @@ struct MmaMath : Base<C> {
         ldmatrix4_trans(a, vbase + place<C>(row, mt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
         for (int nt = 0; nt < C::NT; ++nt) {
-          if constexpr (C::NT > 1) {
-            mma_bf16(o[nt][mt], a, bl[nt][0], bl[nt][1]);
-            mma_bf16(o[nt][mt], a, bh[nt][0], bh[nt][1]);
-          } else {
-            float t[4];
-            mma_bf16_first(t, a, bl[nt][0], bl[nt][1]);
-            mma_bf16(t, a, bh[nt][0], bh[nt][1]);
-            add4(o[nt][mt], t);
-          }
+          float t[4];
+          mma_bf16_first(t, a, lo[nt][0], lo[nt][1]);
+          mma_bf16(t, a, mid[nt][0], mid[nt][1]);
+          mma_bf16(t, a, hi[nt][0], hi[nt][1]);
+          add4(o[nt][mt], t);
         }
       }
     }

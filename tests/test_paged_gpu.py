@@ -213,6 +213,79 @@ def test_extreme_scores(cuda):
            torch.log(torch.tensor([[200.0]], device="cuda")))
 
 
+def _check_infinite_value(dtype, D, G, window=None):
+    """One infinite value among visible keys: that dim of the output is infinite
+    for every query head of the key head, the other dims are the oracle's; a
+    second one of the other sign makes it NaN; outside the window it changes
+    nothing. A key whose score is minus infinity has no weight."""
+    import torch
+    from enilnets_b200 import kernels
+    H, inf = 2 * G, float("inf")
+    q, kp, vp, table, lens = _case(D + G, [200, 37], H, 2, D, 16, dtype)
+    kw = dict(out_dtype=torch.float32, return_lse=True, window=window)
+    plain, _ = kernels.attention_decode_paged(q, kp, vp, table, lens, **kw)
+    at = (table[0, 11].long(), 1, 9)  # position 185 of the first sequence, its second key head
+    for value in (inf, -inf):
+        v = vp.clone()
+        v[at][5] = value
+        out, lse = kernels.attention_decode_paged(q, kp, v, table, lens, **kw)
+        assert (out[0, G:, 5] == value).all()
+        out[0, G:, 5] = plain[0, G:, 5]
+        _check(q, kp, vp, table, lens, out, lse, window=window)
+        v[table[0, 10].long(), 1, 3, 5] = -value
+        out, _ = kernels.attention_decode_paged(q, kp, v, table, lens, **kw)
+        assert torch.isnan(out[0, G:, 5]).all()
+        assert torch.isfinite(out).sum() == out.numel() - G
+        if window is not None:
+            v = vp.clone()
+            v[table[0, 1].long(), 1, 3, 5] = value
+            out, _ = kernels.attention_decode_paged(q, kp, v, table, lens, **kw)
+            assert torch.equal(out, plain)
+        k, qq = kp.clone(), q.clone()
+        k[at][7] = value
+        qq[0, :, 7] = -np.sign(value) * (qq[0, :, 7].abs() + 0.1)
+        qq[0, G, 7] = -np.sign(value)  # a power of two
+        out, lse = kernels.attention_decode_paged(qq, k, vp, table, lens, **kw)
+        _check(qq, k, vp, table, lens, out, lse, window=window)
+
+
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("G", [1, 4, 8, 16, 20])
+@pytest.mark.parametrize("window", [None, 50])
+def test_infinite_values_in_bf16(cuda, D, G, window):
+    _check_infinite_value("bf16", D, G, window)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [1, 4, 8, 16])
+def test_bf16_probabilities_keep_their_bits(cuda, D, G):
+    """An fp32 output from bf16 keys and values. A score below 16 in base 2 has
+    an error of at most 2^-20, a weight 2^-20 ln 2 and the exponential's 2^-22: 9e-7
+    at most, and the sum's roundings less."""
+    import torch
+    from enilnets_b200 import kernels
+    q, kp, vp, table, lens = _case(70, [4000], G, 1, D, 16, "bf16")
+    out = kernels.attention_decode_paged(q, kp, vp, table, lens, out_dtype=torch.float32)
+    k, v = (p[table[0].long(), 0].reshape(-1, D)[:4000].double() for p in (kp, vp))
+    want = torch.softmax(q[0].double() @ k.T / D ** 0.5, -1) @ v
+    assert float((out[0].double() - want).norm() / want.norm()) <= 9e-7
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hkv", [8, 64])
+def test_long_sums_are_not_cut_in_wide_groups(cuda, D, Hkv):
+    """As test_long_sums_are_not_cut, for bf16 groups of 16 query heads."""
+    import torch
+    from enilnets_b200 import kernels
+    q, kp, vp, table, lens = _case(42, [16000], 16 * Hkv, Hkv, D, 16, "bf16")
+    kp = torch.where(torch.isnan(kp), kp, 0.01 * kp)
+    value = 1.0 + torch.rand((D,), device="cuda").to(vp.dtype)
+    vp = torch.where(torch.isnan(vp), vp, value)
+    out = kernels.attention_decode_paged(q, kp, vp, table, lens, out_dtype=torch.float32)
+    want = value.double()
+    assert ((out[0].double() - want).abs() / want).max() <= 1e-6
+
+
 @pytest.mark.parametrize("bad", [-1, 99])
 def test_bad_page_counts_as_masked(cuda, bad):
     import torch
