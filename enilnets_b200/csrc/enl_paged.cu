@@ -14,7 +14,7 @@
 // products on that pipe take three or four tf32 ones and the splits of every
 // element, so up to four fp32 heads a group are computed on the FMA pipe instead,
 // two products an instruction, each element used as it is loaded (16 x 6144 keys
-// of 128: 130 us against 177). At the HBM rate an SM gets 16 bf16 keys of 128
+// of 128: 130 us against 186). At the HBM rate an SM gets 16 bf16 keys of 128
 // every 350 cycles and spends about 30 issue slots of each scheduler on them;
 // tcgen05's 128-row tiles would need the probabilities in shared or tensor memory
 // for no gain.
@@ -42,11 +42,12 @@
 // comes out infinite. fp32 on the FMA pipe: a tile's sum by itself, then added to
 // the running one, so that equal values do not add up equal roundings. fp32 on the
 // tensor pipe: each factor is split into two tf32 parts (values into three) and the
-// three (four) largest products are added, about 2^-21 of each. The tensor pipe
-// cuts its sums instead of rounding them, always towards zero, so nothing is summed
-// in it for long: a few products at a time start from zero and are added to the
-// running sums by rounded additions, two an instruction (without that, 16000 equal
-// fp32 values came out 3e-5 small). With two column tiles these additions show: 64
+// three (four) largest products are added, about 2^-21 of each; infinities are kept
+// whole, and no part of a probability is zero. The tensor pipe cuts its sums instead
+// of rounding them, always towards zero, so nothing is summed in it for long: a few
+// products at a time start from zero and are added to the running sums by rounded
+// additions, two an instruction (without that, 16000 equal fp32 values came out
+// 3e-5 small). With two column tiles these additions show: 64
 // sequences of 12288, four key heads of 128 with 16 query heads each, take 308 us,
 // against 304 with sums that stay in the pipe (16000 equal values then come out
 // 1e-5 small instead of 4e-7) and 293 with two parts of a probability as well.
@@ -198,17 +199,26 @@ __device__ __forceinline__ void lds2x2(uint32_t addr, uint64_t& a, uint64_t& b) 
 
 // x = hi + lo with hi the upper 11 bits (tf32); lo's own tail past 11 bits is
 // dropped by the product. Cutting takes one logic instruction where rounding
-// takes a conversion at a quarter of the rate.
+// takes a conversion at a quarter of the rate. kInf: of an infinity too, whose
+// difference would be NaN.
+template <bool kInf = false>
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xffffe000u;
-  lo = __float_as_uint(x - __uint_as_float(hi));
+  const float h = __uint_as_float(hi);
+  lo = __float_as_uint(kInf && x == h ? 0.0f : x - h);
 }
-// x = hi + lo + rest, exact: a probability of one returns its value unchanged.
+// x = hi + lo + rest, exact (of an infinity, hi): a probability of one returns its
+// value unchanged.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo, uint32_t& rest) {
-  hi = __float_as_uint(x) & 0xffffe000u;
-  const float left = x - __uint_as_float(hi);
-  lo = __float_as_uint(left) & 0xffffe000u;
+  split_tf32<true>(x, hi, lo);
+  const float left = __uint_as_float(lo);
+  lo &= 0xffffe000u;
   rest = __float_as_uint(left - __uint_as_float(lo));
+}
+// For a lower part of zero the smallest normal number of the upper part's sign:
+// zero times infinity would be NaN.
+__device__ __forceinline__ uint32_t not_zero(uint32_t lo, uint32_t hi) {
+  return lo << 1 ? lo : (hi & 0x80000000u) | 0x00800000u;
 }
 // The upper 8 bits of the mantissas of x and y as two bf16; x and y are left with
 // the rest. After three cuts nothing is left.
@@ -235,6 +245,56 @@ template <class C>
 __device__ __forceinline__ uint32_t place(int row, int chunk) {
   const int f = C::kF32 ? (row & 6) ^ ((row & 1) << 2) : row & 7;
   return row * C::kRow + ((chunk ^ f) << 4);
+}
+
+// Adds 16 dims' products of 16 keys with eight heads, in fp32 on the tensor pipe. x, y:
+// this lane's dims of keys r and r + 8, f: of its head, split.
+template <bool kInf>
+__device__ __forceinline__ void add_scores(float (&s)[4], const float4& x, const float4& y,
+                                           const uint32_t* f) {
+  uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    split_tf32<kInf>(half ? x.z : x.x, hi[half][0], lo[half][0]);
+    split_tf32<kInf>(half ? y.z : y.x, hi[half][1], lo[half][1]);
+    split_tf32<kInf>(half ? x.w : x.y, hi[half][2], lo[half][2]);
+    split_tf32<kInf>(half ? y.w : y.y, hi[half][3], lo[half][3]);
+  }
+  float t[4];  // the small products first
+  mma_tf32_first(t, lo[0], f[0], f[1]);
+  mma_tf32(t, hi[0], f[4], f[5]);
+  mma_tf32(t, lo[1], f[2], f[3]);
+  mma_tf32(t, hi[1], f[6], f[7]);
+  mma_tf32(t, hi[0], f[0], f[1]);
+  mma_tf32(t, hi[1], f[2], f[3]);
+  add4(s, t);
+}
+
+// A warp's scores once more, for infinite keys: the common path's splits make their
+// products NaN, for every head (an infinite query's weights are NaN in any case). row: of key r in the tile; query: this
+// lane's dims of its head, or null. A function of its own, which the common path's
+// registers do not pay for: splits for infinities everywhere would make 16
+// sequences of 6144 keys, 8 key heads of 128 with 8 query heads each, 193 us
+// instead of 186, checks of the values' products like this one 204.
+template <class C>
+__device__ __noinline__ float4 scores_again(uint32_t kbase, int row, int q, const float* query,
+                                            int D) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int ks = 0; ks < C::D / 16; ++ks) {
+    float4 x = make_float4(0, 0, 0, 0);
+    if (query && ks * 16 + q * 4 < D) x = *reinterpret_cast<const float4*>(query + ks * 16);
+    uint32_t f[8];
+    split_tf32<true>(x.x, f[0], f[4]);
+    split_tf32<true>(x.y, f[1], f[5]);
+    split_tf32<true>(x.z, f[2], f[6]);
+    split_tf32<true>(x.w, f[3], f[7]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[4 + i] = not_zero(f[4 + i], f[i]);
+    add_scores<true>(s, lds4(kbase + place<C>(row, ks * 4 + q)),
+                     lds4(kbase + place<C>(row + 8, ks * 4 + q)), f);
+  }
+  return make_float4(s[0], s[1], s[2], s[3]);
 }
 
 // One tile's place in the work: item (sequence b, kv head and head block sub),
@@ -353,37 +413,25 @@ struct MmaMath : Base<C> {
   }
 
   // Scores of the warp's 16 keys: rows r and r + 8, heads 2q and 2q + 1.
-  __device__ __forceinline__ void scores(uint32_t kbase, float (&s)[C::NT][4]) const {
+  __device__ __forceinline__ void scores(const Note& w, uint32_t kbase,
+                                         float (&s)[C::NT][4]) const {
 #pragma unroll
     for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
     if constexpr (C::kF32) {
+      static_assert(C::NT == 1, "one column tile in fp32");
       const int row = warp * 16 + r;
 #pragma unroll
-      for (int ks = 0; ks < C::D / 16; ++ks) {
-        const float4 x = lds4(kbase + place<C>(row, ks * 4 + q));
-        const float4 y = lds4(kbase + place<C>(row + 8, ks * 4 + q));
-        uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          split_tf32(half ? x.z : x.x, hi[half][0], lo[half][0]);
-          split_tf32(half ? y.z : y.x, hi[half][1], lo[half][1]);
-          split_tf32(half ? x.w : x.y, hi[half][2], lo[half][2]);
-          split_tf32(half ? y.w : y.y, hi[half][3], lo[half][3]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < C::NT; ++nt) {
-          const uint32_t* f = qf[nt][ks];
-          float t[4];  // the small products first
-          mma_tf32_first(t, lo[0], f[0], f[1]);
-          mma_tf32(t, hi[0], f[4], f[5]);
-          mma_tf32(t, lo[1], f[2], f[3]);
-          mma_tf32(t, hi[1], f[6], f[7]);
-          mma_tf32(t, hi[0], f[0], f[1]);
-          mma_tf32(t, hi[1], f[2], f[3]);
-          add4(s[nt], t);
-        }
+      for (int ks = 0; ks < C::D / 16; ++ks)
+        add_scores<false>(s[0], lds4(kbase + place<C>(row, ks * 4 + q)),
+                          lds4(kbase + place<C>(row + 8, ks * 4 + q)), qf[0][ks]);
+      if (__any_sync(0xffffffffu, isnan(s[0][0] + s[0][2]))) {  // key r, key r + 8
+        const float* query = reinterpret_cast<const float*>(p.q) + w.b * p.q_sb +
+                             (first_head(w) + r) * p.q_sh + q * 4;
+        const float4 x =
+            scores_again<C>(kbase, row, q, r < heads_of(w) ? query : nullptr, p.D);
+        s[0][0] = x.x, s[0][1] = x.y, s[0][2] = x.z, s[0][3] = x.w;
       }
     } else {
       const int row = warp * 16 + (lane & 15);
@@ -416,9 +464,11 @@ struct MmaMath : Base<C> {
           const uint32_t tl = transpose8(__byte_perm(x, y, 0x5410));
           const uint32_t th = transpose8(__byte_perm(x, y, 0x7632));
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            split_tf32(__uint_as_float(__byte_perm(tl, th, i ? 0x7632 : 0x5410)),
-                       ph[nt][2 * half + i], pl[nt][2 * half + i]);
+          for (int i = 0; i < 2; ++i) {
+            uint32_t &hi = ph[nt][2 * half + i], &lo = pl[nt][2 * half + i];
+            split_tf32(__uint_as_float(__byte_perm(tl, th, i ? 0x7632 : 0x5410)), hi, lo);
+            lo = not_zero(lo, hi);
+          }
         }
       const int row = warp * 16 + 2 * q;  // and row + 1; row + 8, row + 9
 #pragma unroll
@@ -509,7 +559,7 @@ struct MmaMath : Base<C> {
   __device__ __forceinline__ void tile(const Note& w, int stage) {
     const uint32_t kbase = sbase + stage * C::kStage;
     float s[C::NT][4];
-    scores(kbase, s);
+    scores(w, kbase, s);
     const int key = warp * 16 + r;  // this lane's keys: key and key + 8
     const uint32_t ok = w.ok[C::NP > 1 ? warp / 2 : 0] >> (key & 31);
     float mx[C::NT][2];
@@ -1282,7 +1332,7 @@ cudaError_t launch_paged_decode(const PagedDecodeParams& p, cudaStream_t stream)
   // 4 warps with 2 stages 147, 148, 169. 16 kv heads of 64: 4 warps with 3 stages,
   // 2 blocks, 129, 127, 136; 2 stages, 3 blocks 132, 131, 139; 2 warps with 4
   // stages 128, 138, and 24 against 15 for one sequence of 5000. On the tensor pipe
-  // any group of fp32 heads takes 180 (128 dims) or 147 (64).
+  // any group of fp32 heads takes 186 (128 dims) or 155 (64).
   // bf16, heads of 128 (64 x 6144 keys, floor 246): 4 warps with 3 stages, 2 blocks,
   // 244; with 2 stages, 3 blocks 259.
   const int group = p.H / p.Hkv;

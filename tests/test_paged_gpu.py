@@ -256,6 +256,13 @@ def test_infinite_values_in_bf16(cuda, D, G, window):
     _check_infinite_value("bf16", D, G, window)
 
 
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("G", [1, 2, 4, 5, 8, 16])
+@pytest.mark.parametrize("window", [None, 50])
+def test_infinite_values_in_fp32(cuda, D, G, window):
+    _check_infinite_value("fp32", D, G, window)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("G", [1, 4, 8, 16])
 def test_bf16_probabilities_keep_their_bits(cuda, D, G):
