@@ -723,9 +723,12 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
 # of GPU time, so their host side is kept short: one test per operand (the
 # message is built only on failure), one struct built from positional values.
 _DENSE = torch.contiguous_format  # (empty_like: two thirds of new_empty's host time)
-_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index
-_current_device = torch._C._cuda_getDevice
-_capturing = torch._C._cuda_isCurrentStreamCapturing
+# (A torch without these, as one built without CUDA, still imports the package.)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
+                     torch.cuda.is_current_stream_capturing)
 
 
 def _describe(t) -> str:

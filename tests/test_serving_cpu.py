@@ -237,3 +237,21 @@ def test_qk_norm_builder_keeps_the_default_contract():
     plain, normed = layers
     assert "q_norm" not in plain and set(normed) - set(plain) == {"q_norm", "k_norm", "qk_norm_eps"}
     assert np.array_equal(plain["Wo"], normed["Wo"]) and np.array_equal(normed["q_norm"], np.ones(16))
+
+
+def test_package_imports_with_a_torch_built_without_cuda():
+    """Building networks, tokenizing and the CPU paths need no CUDA torch, whose
+    bindings such a build lacks."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, n)\n"
+            "import enilnets_b200 as enl\n"
+            "net = enl.AttentionNet()\n"
+            "net.add_multihead_attention(64, 4, qk_norm=True)\n"
+            "print(len(net.layers))\n")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                         cwd=Path(__file__).resolve().parent.parent)
+    assert out.returncode == 0 and out.stdout.strip() == "1", out.stderr
