@@ -318,7 +318,8 @@ class TextGenerator:
         seqs = [self._prompt_ids(p) for p in prompts]
         # As generate: a step follows every token but the last, up to max_seq_len.
         most = [min(self.max_seq_len, len(s) + max_new_tokens) for s in seqs]
-        pages = sum(-(-n // page_size) for n in most)
+        pages = sum(PagedKVCache.pages_held(min(len(s), n), n, page_size, window, sinks)
+                    for s, n in zip(seqs, most))
         cache = PagedKVCache(pages, page_size, self.max_seq_len, window=window, sinks=sinks)
         live = list(range(len(seqs)))
         handle = [cache.add() for _ in seqs]

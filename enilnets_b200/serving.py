@@ -53,6 +53,18 @@ class PagedKVCache:
         self.length: Dict[int, int] = {}
         self._next = 0
 
+    @staticmethod
+    def pages_held(prompt: int, total: int, page_size: int, window: Optional[int] = None,
+                   sinks: int = 0) -> int:
+        """The most pages a sequence holds at once that starts with `prompt` positions
+        in one step and grows by single tokens to `total`."""
+        all_of_it = -(-total // page_size)
+        if window is None:
+            return all_of_it
+        # A step holds the first tokens' pages and those of the last window + 1 positions.
+        step = -(-sinks // page_size) + -(-window // page_size) + 1
+        return min(all_of_it, max(-(-prompt // page_size), step))
+
     @property
     def free_pages(self) -> int:
         return len(self._free)

@@ -224,6 +224,29 @@ def test_windowed_cache_keeps_first_and_last_pages():
     assert 20 - c.free_pages <= 2 + 4
 
 
+def test_pages_held_is_enough_and_bounded():
+    """A pool of pages_held pages serves a sequence from its prompt to its end; a
+    windowed one's does not grow with the end."""
+    from enilnets_b200.serving import PagedKVCache
+    rng = np.random.RandomState(0)
+    for _ in range(300):
+        prompt, page = int(rng.randint(1, 60)), int(rng.randint(1, 20))
+        total = prompt + int(rng.randint(0, 200))
+        window = None if rng.rand() < 0.2 else int(rng.randint(0, 60))
+        sinks = 0 if window is None else int(rng.randint(0, 12))
+        n = PagedKVCache.pages_held(prompt, total, page, window, sinks)
+        c = PagedKVCache(n, page, 1000, window=window, sinks=sinks)
+        s = c.add()
+        c.reserve([s], [prompt])
+        c.advance([s], [prompt])
+        while c.length[s] < total:
+            c.reserve([s], [1])
+            c.advance([s], [1])
+    held = [PagedKVCache.pages_held(20, total, 16, 100, 4) for total in (1000, 100000)]
+    assert held[0] == held[1] == 1 + 7 + 1
+    assert PagedKVCache.pages_held(20, 1000, 16) == 63
+
+
 def test_qk_norm_builder_keeps_the_default_contract():
     """qk_norm adds weights without drawing random numbers; without it the layer
     dict is what it was."""

@@ -177,6 +177,39 @@ def test_serve_samples_as_generate_does(cuda, gen):
         assert gen.serve_ids(["keys"], **kw) == [want]
 
 
+def test_serve_with_a_window_holds_its_pages_only(cuda, gen, monkeypatch):
+    """serve with a window: the tokens of the same steps on a roomy cache, from a
+    pool that does not hold every position."""
+    made = []
+
+    class Cache(serving.PagedKVCache):
+        def __init__(self, pages, *args, **kw):
+            made.append(pages)
+            super().__init__(pages, *args, **kw)
+
+    kw = dict(window=7, sinks=2)
+    want = []
+    for ids in (gen._prompt_ids("the cache keeps keys"), gen._prompt_ids("a")):
+        cache = serving.PagedKVCache(100, 2, gen.max_seq_len, **kw)
+        seq, ids = cache.add(), list(ids)
+        logits = serving.paged_forward_step(gen.network, [ids], cache, [seq])
+        for _ in range(40):
+            tok = serving.sample(logits, [0.0], greedy=True)[0]
+            if tok == gen._id(gen.tokenizer.end_token):
+                break
+            ids.append(tok)
+            if cache.length[seq] >= gen.max_seq_len:
+                break
+            logits = serving.paged_forward_step(gen.network, [[tok]], cache, [seq])
+        want.append(ids)
+    monkeypatch.setattr(serving, "PagedKVCache", Cache)
+    got = gen.serve_ids(["the cache keeps keys", "a"], max_new_tokens=40, greedy=True, page_size=2,
+                        **kw)
+    assert got == want
+    prompt = -(-len(gen._prompt_ids("the cache keeps keys")) // 2)
+    assert made == [max(prompt, 6) + 6]
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(greedy=True), dict(top_k=3, temperature=0.5)])
 def test_rows_without_a_logit_are_refused(cuda, gen, kw):
     """A row of NaN and -inf has no token: the draw raises, and so does serve on a
