@@ -240,6 +240,60 @@ def test_logits_that_share_their_distance_from_the_largest(cuda, B, top):
                 assert got[b] in answers, (V, kw, b, got[b], answers)
 
 
+def _hard_rows(rng, V):
+    """Rows whose cuts a histogram of a quarter of the logits guesses badly: flat
+    ones, narrow clusters with thousands of tokens a bin, steps, a heavy tail, whole
+    numbers (long ties) and one that is flat but for a single far token."""
+    flat = rng.standard_normal(V)
+    step = np.where(np.arange(V) % 7 == 0, 2.0, 0.0) + 1e-4 * rng.standard_normal(V)
+    far = 1e-3 * rng.standard_normal(V)
+    far[V // 2] = 12.0
+    return [flat, 0.1 * flat, 3.0 + 1e-5 * flat, step, -rng.exponential(4.0, V),
+            np.round(2.0 * flat), far, np.where(np.arange(V) < V // 3, flat, -1e30)]
+
+
+def _may_draw(row, order, u, token, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, eps=1e-5):
+    """Whether the draw u may give the token where weights are right to eps: with each
+    threshold where it is or eps to a side, u is within eps of its stretch of the
+    running sum."""
+    w = np.exp((row - row[order[0]]) / temperature)
+    for p in {top_p, *((top_p - eps, top_p + eps) if top_p < 1.0 else ())}:
+        ws = w[order]
+        if top_k > 0:
+            ws[top_k:] = 0.0
+        if p < 1.0:
+            before = np.cumsum(ws) - ws
+            ws[1:][before[1:] >= p * ws.sum()] = 0.0
+        for m in {min_p, min_p * (1 - eps), min_p * (1 + eps)}:
+            kept = np.zeros_like(w)
+            kept[order] = np.where(ws < m, 0.0, ws)
+            end = np.cumsum(kept) / kept.sum()
+            start = end[token - 1] if token else 0.0
+            if kept[token] > 0 and start - eps <= u <= end[token] + eps:
+                return True
+    return False
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,repeat", [(40009, 1), (20001, 20), (131072, 2)])
+def test_rows_that_defeat_the_guesses(cuda, dtype, V, repeat):
+    """Large top-k and flat nuclei over such rows, one block and several a row."""
+    from enilnets_b200 import kernels
+    rng = np.random.RandomState(V)
+    rows = _hard_rows(rng, V)
+    n = len(rows)
+    x = _dev(np.stack(rows * repeat), dtype)
+    host = x[:n].double().cpu().numpy()
+    orders = [np.argsort(-r, kind="stable") for r in host]
+    for kw in (dict(top_k=2500), dict(top_k=V // 3), dict(top_p=0.5), dict(top_p=0.99),
+               dict(top_k=V // 5, top_p=0.7), dict(top_k=6000, top_p=0.9, min_p=0.3),
+               dict(top_p=0.95, temperature=3.0)):
+        u = rng.random_sample(len(x)).astype(np.float32)
+        got = kernels.sample_tokens(x, _dev(u), **kw).tolist()
+        for b in sorted({*range(n), *range(len(x) - n, len(x))}):
+            assert _may_draw(host[b % n], orders[b % n], float(u[b]), got[b], **kw), (kw, b, got[b])
+
+
 @pytest.mark.parametrize("T", [1e-45, 1e-40, 1e-38, 1e-30])
 def test_lowest_temperatures(cuda, T):
     """A temperature whose reciprocal passes fp32 leaves the largest logit alone,
