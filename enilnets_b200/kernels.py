@@ -935,6 +935,8 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: Optiona
     wq, wk, cos, sin, rows = _norm_rope_operands(D, q_weight, k_weight, rope, dev)
     norm = wq is not None
     in_dt = q.dtype if isinstance(q, torch.Tensor) else gdt
+    if in_dt not in _DTYPES:
+        raise ValueError(f"q must be bf16 or fp32, got {_describe(q)}")
     qs = ks = (0, 0, 0)
     if norm:
         qs = _require_heads("q", q, qshape, None, dev)

@@ -338,6 +338,18 @@ def test_refusals(cuda):
             call()
 
 
+def test_backward_refuses_inputs_of_other_types(cuda):
+    """Without weights the inputs are not read, but their type names the
+    gradients'."""
+    import torch
+    from enilnets_b200 import kernels
+    dq, dk = torch.ones((1, 3, 2, 64), device="cuda"), torch.ones((1, 3, 1, 64), device="cuda")
+    tables = tuple(map(_t, _tables(3, 64)))
+    for out in (None, (torch.empty_like(dq), torch.empty_like(dk))):
+        with pytest.raises(ValueError, match="q must be"):
+            kernels.qk_norm_rope_backward(dq, dk, dq.half(), dk.half(), rope=tables, out=out)
+
+
 def test_empty_batches(cuda):
     import torch
     from enilnets_b200 import kernels
