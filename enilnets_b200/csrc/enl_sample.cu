@@ -1468,10 +1468,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   if (n_blocks > 1) s.sync();  // no block's shared memory goes while another reads it
 }
 
-// Blocks per row: as many as keep two a SM, a power of two up to 8, with at least
-// one vector for each thread. (256 rows of 131072, two blocks a row: top-k and
-// top-p 42 us against 21, top-p alone the same; 64 rows of 100003, four blocks
-// against two: 90 us against 79.)
+// Blocks per row: a power of two up to 8, doubled while the blocks before it leave
+// room for two a SM, with at least one vector for each thread. Flat rows gain by it
+// and sharp ones under a small top-k, which read little more than once, lose the
+// exchanges' time. Measured, us with 1, 2, 4 and 8 blocks a row (the rule's choice in
+// brackets): 16 rows of 131072 bf16, top-p alone 70, 60, 55, [48], top-k and top-p
+// 11, 14, 13, [15]; 64 rows of 100003 fp32 with mixed settings 121, 94, [81], 90, top-k
+// and top-p 24, 26, [21], 36; 128 rows of 131072 bf16, top-p alone 92, [89], 103, 147,
+// top-k and top-p 15, [22], 35, 63. 256 rows of 131072 with two: top-k and top-p 42
+// against [21].
 int choose_cluster(int B, int V, bool fp32, int n_sms) {
   const int per_block = kThreads * (fp32 ? 4 : 8);
   int c = 1;

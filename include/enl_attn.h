@@ -552,7 +552,9 @@ typedef struct enl_paged_decode_args {
 /* Attention of one new token per sequence over a paged cache: the query of
  * sequence b sits at position seq_lens[b] - 1. A sequence of length 0 gets a
  * zero output and an LSE of -inf. Any num_heads / num_kv_heads ratio; head_dim
- * a multiple of 8 up to 128; bf16 or fp32 (fp32-accurate products either way).
+ * a multiple of 8 up to 128; bf16 or fp32. Scores, softmax and sums in fp32 on
+ * products of bf16 inputs or of fp32 ones (groups of more than four fp32 heads:
+ * of parts that carry 21 bits), infinities as they come.
  * The lengths are read on the device, so a call can sit in a CUDA graph while
  * they grow. A length above max_pages * page_size is cut to it, and a page
  * outside the pool counts as masked; both set the device error word (code 2). */
