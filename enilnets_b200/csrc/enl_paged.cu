@@ -310,7 +310,8 @@ struct Block {  // shared by a block's warps
   Note note[4];
   long long scan[8];
   int longest[8];
-  int b, rest;  // where the run starts
+  int b;  // where the run starts: the sequence, and the units of it before
+  long long rest;
   int last;
   int abort;  // a wait ran out: the others stop waiting
   float m[4][16], l[4][16];
@@ -1010,7 +1011,9 @@ struct Decoder : std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>> {
     const int at = b - lens_b;
     return at >= 0 && at < kLens ? sh.lens[at] : read_length(b);
   }
-  __device__ __forceinline__ int tiles_of(int n) const { return (n + C::kKeys - 1) / C::kKeys; }
+  __device__ __forceinline__ int tiles_of(int n) const {  // (n is up to 2^31 - 1)
+    return n / C::kKeys + (n % C::kKeys > 0);
+  }
 
   // ------------------------------------------------------- loading warps
   __device__ void enter(Walker& w, int b) const {
@@ -1036,9 +1039,9 @@ struct Decoder : std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>> {
   };
   __device__ __forceinline__ Key find_key(const Walker& w, int key) const {
     Key k{0, -1};
-    const int i = w.t * C::kKeys + key;
-    if (i < w.vis.n) {
-      const int j = i < w.vis.n_sink ? i : i + w.vis.gap;
+    const uint32_t i = (uint32_t)w.t * C::kKeys + key;  // past 2^31 in the last tile
+    if (i < (uint32_t)w.vis.n) {
+      const int j = (int)i < w.vis.n_sink ? (int)i : (int)i + w.vis.gap;
       const int col = j / p.page_size;
       k.slot = j - col * p.page_size;
       k.page = p.table[w.b * p.t_sb + col];
@@ -1252,7 +1255,7 @@ struct Decoder : std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>> {
         run += u;
       }
       sh.b = b;
-      sh.rest = (int)(first - run);
+      sh.rest = first - run;
     }
     __syncthreads();
     if (p.B > kLens) {  // keep the lengths that this run meets first
@@ -1264,8 +1267,8 @@ struct Decoder : std::conditional_t<(C::kFma > 0), FmaMath<C>, MmaMath<C>> {
     }
     Walker w;
     enter(w, sh.b);
-    w.sub = share.whole ? sh.rest : sh.rest / w.nt;
-    w.t = share.whole ? 0 : sh.rest % w.nt;
+    w.sub = (int)(share.whole ? sh.rest : sh.rest / w.nt);
+    w.t = share.whole ? 0 : (int)(sh.rest % w.nt);
     int n = (int)(end - first);  // tiles of the run
     if (share.whole) {
       Walker x = w;

@@ -192,6 +192,24 @@ def test_offsets_past_32_bits(cuda):
     _check(q, kp, vp, table, lens, out, lse)
 
 
+@pytest.mark.parametrize("dtype,short", [("bf16", 0), ("bf16", 60), ("fp32", 0)])
+def test_lengths_up_to_the_last_positions(cuda, dtype, short):
+    """A sequence that ends within a tile of 2^31 positions, all of them one page:
+    the output is that page's (short: of the page without its last slots, in all but
+    a 42966th of the weight). Each of some 10^5 additions rounds by 2^-24: 1e-4
+    covers them with the short page's 3e-5."""
+    import torch
+    from enilnets_b200 import kernels
+    page, pages = 49981, 42966  # 2^31 - 2
+    q, kp, vp, _, _ = _case(80, [page], 2, 1, 8, page, dtype, spare=0)
+    table = torch.zeros((1, pages), dtype=torch.int32, device="cuda")
+    out, lse = kernels.attention_decode_paged(q, kp, vp, table, _i32([page * pages - short]),
+                                              out_dtype=torch.float32, return_lse=True)
+    want, one = ref.paged_decode(_np(q), _np(kp), _np(vp), np.zeros((1, 1), int), [page])
+    assert np.abs(_np(out) - want).max() <= 1e-4
+    assert np.abs(_np(lse) - one - np.log(pages)).max() <= 1e-4
+
+
 def test_extreme_scores(cuda):
     """Scores far apart: the largest takes all, nothing overflows; equal
     scores average; -inf and +inf keys in masked slots do not leak."""
