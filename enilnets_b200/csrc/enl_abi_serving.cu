@@ -48,10 +48,10 @@ int check_pool(const char* fn, const void* k, const void* v, int64_t sp, int64_t
   return ENL_OK;
 }
 
-// (token, head) pairs are numbered with 32 bits.
+// (token, head) pairs are numbered with 32 bits, those that fill up a last block too.
 int check_units(const char* fn, int32_t batch, int32_t seq, int32_t num_heads) {
-  if ((long long)batch * seq * num_heads > 0x7fffffffll)
-    return fail(ENL_ERR_UNSUPPORTED, "%s: batch * seq * num_heads = %lld exceeds 2^31 - 1", fn,
+  if ((long long)batch * seq * num_heads > 0x7fffffffll - 256)
+    return fail(ENL_ERR_UNSUPPORTED, "%s: batch * seq * num_heads = %lld exceeds 2^31 - 257", fn,
                 (long long)batch * seq * num_heads);
   return ENL_OK;
 }

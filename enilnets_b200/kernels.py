@@ -722,6 +722,7 @@ def linear_attention(phi_q: torch.Tensor, phi_k: torch.Tensor, v: torch.Tensor, 
 # A decode step makes several of these calls per layer, each a few microseconds
 # of GPU time, so their host side is kept short: one test per operand (the
 # message is built only on failure), one struct built from positional values.
+_MAX = 0x7fffffff  # of a count in a struct: what ctypes would cut off silently is checked
 _DENSE = torch.contiguous_format  # (empty_like: two thirds of new_empty's host time)
 # (A torch without these, as one built without CUDA, still imports the package.)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
@@ -743,6 +744,8 @@ def _device_of(name: str, t, dims: str) -> int:
     if not isinstance(t, torch.Tensor) or t.dim() != dims.count(",") + 1 or \
             t.dtype not in _DTYPES or not t.is_cuda:
         raise ValueError(f"{name} must be a bf16/fp32 ({dims}) CUDA tensor, got {_describe(t)}")
+    if max(t.shape) > _MAX:
+        raise ValueError(f"{name} must have dimensions below 2^31, got {_describe(t)}")
     dev = t.get_device()
     if dev != _current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
@@ -1055,7 +1058,8 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
             q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(), v_pages.data_ptr(), ps[0], ps[1],
             ps[2], pool[0], pool[2], block_table.data_ptr(), block_table.stride(0),
             block_table.shape[1], lens, out.data_ptr(), os_[0], os_[1],
-            None if lse is None else lse.data_ptr(), B, H, pool[1], D, int(window), int(sinks),
+            None if lse is None else lse.data_ptr(), B, H, pool[1], D, min(int(window), _MAX),
+            min(int(sinks), _MAX),
             slopes, 1.0 / math.sqrt(D) if scale is None else float(scale), _DTYPES[dt],
             _DTYPES[out.dtype])
         lib = nat.load()
@@ -1117,7 +1121,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     else:
         o_ptr = _require_vector("out", out, B, torch.int64, dev)
     a = nat.SampleArgs(logits.data_ptr(), st[0], _DTYPES[logits.dtype], B, V, u_ptr, t_ptr, k_ptr,
-                       p_ptr, m_ptr, float(t_all), min(int(k_all), 0x7fffffff), float(p_all),
+                       p_ptr, m_ptr, float(t_all), min(int(k_all), _MAX), float(p_all),
                        float(m_all), o_ptr)
     status = nat.load().enl_sample_tokens(ctypes.byref(a), _raw_stream(dev))
     if status:

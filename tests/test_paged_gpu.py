@@ -99,6 +99,17 @@ def test_window_and_sinks(cuda, dtype, window, sinks):
     _check(*case, out, lse, window=window, sinks=sinks)
 
 
+def test_windows_past_32_bits(cuda):
+    """A window of 2^32 sees everything, 2^32 first tokens are all of them."""
+    import torch
+    case = _case(4, [1, 300, 77], 8, 4, 64, 16, "bf16")
+    want, lse = _run(case)
+    for kw in (dict(window=1 << 32), dict(window=(1 << 32) + 3, sinks=1),
+               dict(window=2, sinks=1 << 32)):
+        out, got = _run(case, **kw)
+        assert torch.equal(out, want) and torch.equal(got, lse), kw
+
+
 def test_alibi_scale_and_window(cuda):
     import torch
     case = _case(3, [400, 31, 1], 8, 4, 128, 16, "fp32")

@@ -350,6 +350,21 @@ def test_backward_refuses_inputs_of_other_types(cuda):
             kernels.qk_norm_rope_backward(dq, dk, dq.half(), dk.half(), rope=tables, out=out)
 
 
+def test_counts_past_32_bits_are_refused(cuda):
+    """A broadcast view of 2^32 + 1 tokens is no call for one token."""
+    import torch
+    from enilnets_b200 import kernels
+    S = (1 << 32) + 1
+    q, k = (torch.ones((1, 1, h, 64), device="cuda") for h in (2, 1))
+    far = [t.expand(1, S, -1, -1) for t in (q, k)]
+    w = torch.full((64,), 2.0, device="cuda")
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        kernels.qk_norm_rope(*far, w, w, out=tuple(far))
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        kernels.qk_norm_rope_backward(*far, *far, w, w, out=tuple(far))
+    assert (q == 1).all() and (k == 1).all()
+
+
 def test_empty_batches(cuda):
     import torch
     from enilnets_b200 import kernels

@@ -66,6 +66,20 @@ def test_norm_rope_refusals(change, message):
         _call("enl_qk_norm_rope", a)
 
 
+@pytest.mark.parametrize("seq,heads", [((1 << 31) - 1, 1), ((1 << 31) - 256, 1), (1 << 28, 8)])
+def test_norm_rope_refuses_more_pairs_than_it_numbers(seq, heads):
+    a = _rope_args()
+    a.seq, a.num_heads, a.num_kv_heads = seq, heads, 1
+    with pytest.raises(ValueError, match="exceeds 2\\^31 - 257"):
+        _call("enl_qk_norm_rope", a)
+    b = _native.QkNormRopeBackwardArgs()
+    b.batch, b.seq, b.num_heads, b.num_kv_heads, b.head_dim = 1, seq, heads, 1, 64
+    b.rope_cos = b.rope_sin = 256
+    b.rope_rows = 4
+    with pytest.raises(ValueError, match="exceeds 2\\^31 - 257"):
+        _call("enl_qk_norm_rope_backward", b)
+
+
 def test_norm_rope_empty_calls_launch_nothing():
     a = _rope_args()
     a.seq = 0
