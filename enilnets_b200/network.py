@@ -80,9 +80,17 @@ def dense(x, layer):
 
 
 def embed(tokens, layer):
-    """Table lookup by integer token ids (nn/forward.py:414-419)."""
+    """Table lookup by integer token ids (nn/forward.py:414-419); IndexError for
+    ids outside the table."""
     import torch
-    ids = to_device(np.asarray(tokens, dtype=np.int64), torch.int64)
+    host = np.asarray(tokens, dtype=np.int64)
+    rows = len(layer["weights"])
+    low, high = (host.min(), host.max()) if host.size else (0, -1)
+    if high >= rows or low < -rows:
+        # As NumPy's lookup; on the device it would be a failed assertion that
+        # takes the context with it.
+        raise IndexError(f"token ids from {low} to {high} for an embedding of {rows} rows")
+    ids = to_device(host, torch.int64)
     if ids.dim() == 1:
         ids = ids.reshape(-1, 1)
     return WEIGHTS.get(layer["weights"], torch.float32)[ids]

@@ -292,3 +292,10 @@ def test_package_imports_with_a_torch_built_without_cuda():
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
                          cwd=Path(__file__).resolve().parent.parent)
     assert out.returncode == 0 and out.stdout.strip() == "1", out.stderr
+
+
+@pytest.mark.parametrize("ids", [[[50]], [[3, 1 << 40]], [[-51, 0]]])
+def test_token_ids_outside_the_embedding_are_refused_on_the_host(ids):
+    from enilnets_b200 import network
+    with pytest.raises(IndexError, match="50 rows"):
+        network.embed(ids, {"weights": np.zeros((50, 8), np.float32)})
